@@ -235,6 +235,85 @@ int nxv_random(void* out, unsigned int n, unsigned int seed, unsigned int dist,
 int nxv_random_f64(void* out, unsigned long n, unsigned int seed, unsigned int dist,
                    const char* spv_path);
 
+/* ---- Network ends: layer norm, dropout, linear cross entropy (NEW) ------
+ * With no counterpart in the reference's shim: what a network over classes
+ * or tokens needs around its products (Axon's layer_norm, dropout and
+ * categorical cross entropy run op by op on an Nx backend).  dtype 0 f32,
+ * 1 f64, 2 bf16.  Tensors are dense row-major at any element-aligned
+ * address; 16-byte aligned rows are faster.  Outputs share no memory with
+ * other arguments unless said so (-3).
+ *
+ * Workspaces: a `workspace` handle of at least the size that the matching
+ * nxv_*_workspace function gives, on a 256-byte boundary; what it holds does
+ * not matter, and calls that may overlap (two streams, two captured graphs)
+ * need one each.  NULL takes the stream's library scratch, which stays
+ * allocated; a call being captured into a CUDA graph must bring its own
+ * (-3 otherwise). */
+
+/* Layer norm of every row of x [rows, cols]: mean, rstd = 1 / sqrt(var + eps)
+ * (var = mean of (x - mean)^2), y = (x - mean) rstd gamma + beta.  gamma, beta
+ * [cols] and y have x's type; mean and rstd [rows] are f32 (f64 for f64) and
+ * all arithmetic is in their type.  y may be x.  cols > 0, eps >= 0.
+ * spv: layer_norm.spv. */
+int nxv_layer_norm(void* y, void* mean, void* rstd,
+                   void* x, void* gamma, void* beta,
+                   unsigned int rows, unsigned int cols, double eps,
+                   unsigned int dtype, const char* spv_path);
+
+unsigned long nxv_layer_norm_grad_workspace(unsigned int rows, unsigned int cols,
+                                            unsigned int dtype);
+
+/* Its gradients: with xh = (x - mean) rstd and g = dy gamma,
+ * dx = rstd (g - mean(g) - xh mean(g xh)) [rows, cols] (may be dy or x),
+ * dgamma = sum_rows dy xh, dbeta = sum_rows dy [cols], added in a fixed order
+ * (bit-reproducible) in f32 (f64) and rounded once; zeros for rows = 0.
+ * spv: layer_norm_grad.spv. */
+int nxv_layer_norm_grad(void* dx, void* dgamma, void* dbeta, void* workspace,
+                        void* dy, void* x, void* gamma, void* mean, void* rstd,
+                        unsigned int rows, unsigned int cols,
+                        unsigned int dtype, const char* spv_path);
+
+/* Dropout: out_i = x_i / (1 - p) where element offset + i of nxv_random's
+ * uniform stream of this seed is >= p, else 0 (whatever x_i is).  The mask is
+ * not stored: the gradient is the same call on the incoming gradient.  A
+ * tensor processed in parts takes the parts' offsets.  0 <= p <= 1,
+ * offset + n <= 2^32.  out may be x.  spv: dropout.spv. */
+int nxv_dropout(void* out, void* x, unsigned long n, double p,
+                unsigned int seed, unsigned long offset,
+                unsigned int dtype, const char* spv_path);
+
+/* grad: 0 for nxv_linear_cross_entropy, 1 for its gradient.  0 bytes for
+ * arguments that the call would refuse. */
+unsigned long nxv_linear_cross_entropy_workspace(unsigned int n, unsigned int vocab,
+                                                 unsigned int dim, unsigned int dtype,
+                                                 unsigned int grad);
+
+/* Softmax cross entropy of the linear layer z = x w^T, x [n, dim], w [vocab,
+ * dim] (one row per class), without storing z: lse_i = log sum_v exp z_iv and
+ * loss_i = lse_i - z_i,labels_i, f32 [n].  labels: int32 or int64 (index_bytes);
+ * a label outside [0, vocab) marks a row without a target (loss 0).  dtype 0
+ * f32 or 2 bf16 (tcgen05; f32 as six bf16 partial products, f32 accuracy).
+ * As logsumexp.spv: a row whose logits hold a NaN or +inf, or only -inf, has
+ * lse NaN; in f32 an infinity in x or w makes every logit it meets NaN.
+ * vocab, dim > 0.  spv: linear_cross_entropy.spv. */
+int nxv_linear_cross_entropy(void* loss, void* lse, void* workspace,
+                             void* x, void* w, void* labels,
+                             unsigned int n, unsigned int vocab, unsigned int dim,
+                             unsigned int dtype, unsigned int index_bytes,
+                             const char* spv_path);
+
+/* Its gradients for the incoming gradient dloss of every row's loss, f32 [n],
+ * and the forward call's lse: G = (exp(z - lse) - [v = label]) dloss (0 for a
+ * row without a target, whatever its x holds), dx = G w [n, dim], dw = G^T x
+ * [vocab, dim] in x's type.  The vocabulary is processed in pieces; z is
+ * computed again, and G of one piece is held in the workspace (bf16 G for
+ * bf16).  Bit-reproducible.  spv: linear_cross_entropy_grad.spv. */
+int nxv_linear_cross_entropy_grad(void* dx, void* dw, void* workspace,
+                                  void* dloss, void* x, void* w, void* labels, void* lse,
+                                  unsigned int n, unsigned int vocab, unsigned int dim,
+                                  unsigned int dtype, unsigned int index_bytes,
+                                  const char* spv_path);
+
 /* ---- Fused HMC primitives (shim.h:169-189) ----------------------------- */
 
 /* Partial sums 0.5*sum(p^2*inv_mass), one f32 per 256-element group

@@ -57,6 +57,13 @@ SIGNATURES: dict[str, tuple] = {
     "nxv_matmul_batched": (C.c_int, [vp, vp, vp, u32, u32, u32, u32, u32, cstr]),
     "nxv_random": (C.c_int, [vp, u32, u32, u32, cstr]),
     "nxv_random_f64": (C.c_int, [vp, ul, u32, u32, cstr]),
+    "nxv_layer_norm": (C.c_int, [vp] * 6 + [u32, u32, f64, u32, cstr]),
+    "nxv_layer_norm_grad_workspace": (ul, [u32, u32, u32]),
+    "nxv_layer_norm_grad": (C.c_int, [vp] * 9 + [u32, u32, u32, cstr]),
+    "nxv_dropout": (C.c_int, [vp, vp, ul, f64, u32, ul, u32, cstr]),
+    "nxv_linear_cross_entropy_workspace": (ul, [u32] * 5),
+    "nxv_linear_cross_entropy": (C.c_int, [vp] * 6 + [u32] * 5 + [cstr]),
+    "nxv_linear_cross_entropy_grad": (C.c_int, [vp] * 8 + [u32] * 5 + [cstr]),
     "nxv_kinetic_energy": (C.c_int, [vp, vp, vp, u32, cstr]),
     "nxv_normal_logpdf": (C.c_int, [vp, vp, vp, vp, u32, cstr]),
     "nxv_leapfrog_normal": (C.c_int, [vp, vp, vp, vp, vp, u32, f32, f32, f32, cstr]),

@@ -17,8 +17,15 @@
 //                 exact transform)
 // One thread per four f32 outputs (two counters) or per f64 output, with
 // vector stores when aligned.
+//
+// Dropout draws its mask from the f32 uniform stream above: element i of the
+// tensor is kept when the uniform of stream element offset + i is >= p, so the
+// mask of (seed, offset) is the one that a comparison of nxv_random's output
+// with p would give, for every type, and is never stored: the gradient draws
+// it again.
 #include "kernels.h"
 
+#include <cuda_bf16.h>
 #include <math.h>
 
 namespace nxv {
@@ -257,7 +264,86 @@ __global__ void k_random_f64(double* __restrict__ out, size_t n, uint32_t seed, 
     }
 }
 
+// ---- dropout ------------------------------------------------------------------
+//
+// y_i = x_i * scale where (word >> 8) >= thresh, else 0 (whatever x_i is, NaN
+// and infinities included).  thresh = ceil(p 2^24): the comparison of the
+// uniform (word >> 8) 2^-24 with p, in whole numbers.  f32 arithmetic for f32
+// and bf16 (bf16 rounded once at the store), f64 for f64.
+__device__ __forceinline__ float drop_scaled(float x, double, float s) { return __fmul_rn(x, s); }
+__device__ __forceinline__ double drop_scaled(double x, double s, float) { return __dmul_rn(x, s); }
+__device__ __forceinline__ __nv_bfloat16 drop_scaled(__nv_bfloat16 x, double, float s) {
+    return __float2bfloat16_rn(__fmul_rn(__bfloat162float(x), s));
+}
+
+template <typename T>
+__device__ __forceinline__ T drop_one(T x, uint32_t w, uint32_t thresh, double s64, float s32) {
+    return (w >> 8) >= thresh ? drop_scaled(x, s64, s32) : T(0.0f);
+}
+
+// A thread takes VEC consecutive elements (16 bytes) of VEC / 2 counters; with
+// an odd offset (ODD) their words lie in VEC / 2 + 1 counters.  The last n % VEC
+// elements, and every element of a tensor that is not 16-byte aligned
+// (VEC = 1), go one by one.
+template <typename T, int VEC, bool ODD>
+__global__ void __launch_bounds__(256)
+k_dropout(T* y, const T* x, size_t n, uint32_t thresh, double s64, float s32, uint32_t seed,
+          uint64_t offset) {
+    const size_t stride = (size_t)gridDim.x * blockDim.x;
+    const size_t t0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    size_t done = 0;
+    if constexpr (VEC > 1) {
+        struct alignas(16) V {
+            T e[VEC];
+        };
+        const size_t nv = n / VEC;
+        for (size_t q = t0; q < nv; q += stride) {
+            V v = reinterpret_cast<const V*>(x)[q];
+            const uint32_t c0 = (uint32_t)((offset + q * VEC) >> 1);
+            uint32_t w[VEC + 2];
+#pragma unroll
+            for (int k = 0; k < VEC / 2 + (ODD ? 1 : 0); k++)
+                philox2x32(c0 + k, 0u, seed, w[2 * k], w[2 * k + 1]);
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                v.e[e] = drop_one(v.e[e], w[e + (ODD ? 1 : 0)], thresh, s64, s32);
+            reinterpret_cast<V*>(y)[q] = v;
+        }
+        done = nv * VEC;
+    }
+    for (size_t i = done + t0; i < n; i += stride) {
+        const uint64_t s = offset + i;
+        uint32_t w0, w1;
+        philox2x32((uint32_t)(s >> 1), 0u, seed, w0, w1);
+        y[i] = drop_one(x[i], (s & 1) ? w1 : w0, thresh, s64, s32);
+    }
+}
+
+template <typename T>
+void dropout_t(Ctx& c, T* y, const T* x, size_t n, double p, uint32_t seed, uint64_t offset) {
+    constexpr int V = 16 / sizeof(T);
+    const uint32_t thresh = (uint32_t)ceil(p * 0x1.0p24);  // p 2^24 is exact
+    const double s64 = p < 1.0 ? 1.0 / (1.0 - p) : 0.0;    // p = 1 keeps nothing
+    const float s32 = (float)s64;
+    const bool vec = ((((uintptr_t)x) | ((uintptr_t)y)) & 15) == 0;
+    const unsigned g = grid_for(c, vec ? (n + V - 1) / V : n, 256, 8);
+    if (!vec) k_dropout<T, 1, false><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
+    else if (offset & 1) k_dropout<T, V, true><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
+    else k_dropout<T, V, false><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
+    count_launch();
+}
+
 }  // namespace
+
+int launch_dropout(Ctx& c, int dt, void* y, const void* x, size_t n, double p, uint32_t seed,
+                   uint64_t offset) {
+    if (n == 0) return OK;
+    if (dt == F32) dropout_t(c, (float*)y, (const float*)x, n, p, seed, offset);
+    else if (dt == F64) dropout_t(c, (double*)y, (const double*)x, n, p, seed, offset);
+    else dropout_t(c, (__nv_bfloat16*)y, (const __nv_bfloat16*)x, n, p, seed, offset);
+    pdl_record_all(c);
+    return finish(c);
+}
 
 int launch_random(Ctx& c, int dt, void* out, size_t n, uint32_t seed, unsigned dist) {
     if (n == 0) return OK;

@@ -4,7 +4,9 @@
 
 namespace nxv {
 
-enum DType : int { F32 = 0, F64 = 1 };
+// BF16: layer norm, dropout and the linear cross entropy only.
+enum DType : int { F32 = 0, F64 = 1, BF16 = 2 };
+inline size_t dtype_bytes(int dt) { return dt == F64 ? 8 : dt == F32 ? 4 : 2; }
 
 // f32 elementwise transcendentals (exp log sigmoid tanh erf expm1 pow) use
 // the f32 library functions by default (2-4 ulp, the precision class of the
@@ -50,6 +52,36 @@ int launch_kinetic_energy(Ctx& c, void* out, const void* p, const void* m, size_
 
 // random (k_philox.cu)
 int launch_random(Ctx& c, int dt, void* out, size_t n, uint32_t seed, unsigned dist);
+// y = x / (1 - p) where the uniform of stream element offset + i is >= p, else 0.
+int launch_dropout(Ctx& c, int dt, void* y, const void* x, size_t n, double p, uint32_t seed,
+                   uint64_t offset);
+
+// layer norm over the rows of [rows, cols] (k_norm.cu); mean, rstd and the
+// workspace are f32 (f64 for f64).
+int launch_layer_norm(Ctx& c, int dt, void* y, void* mean, void* rstd, const void* x,
+                      const void* gamma, const void* beta, unsigned rows, unsigned cols,
+                      double eps);
+unsigned norm_grad_blocks(unsigned rows);
+size_t norm_grad_workspace(unsigned rows, unsigned cols, int dt);
+int launch_layer_norm_grad(Ctx& c, int dt, void* dx, void* dgamma, void* dbeta, void* ws,
+                           const void* dy, const void* x, const void* gamma, const void* mean,
+                           const void* rstd, unsigned rows, unsigned cols);
+
+// softmax cross entropy of the linear layer z = x w^T (k_xent.cu).
+struct XentP {
+    const void* x;       // [n, dim]
+    const void* w;       // [vocab, dim]
+    const void* labels;  // [n], int32 or int64
+    int index_bytes;
+    unsigned n, vocab, dim;
+    int dt;              // F32 or BF16
+};
+size_t xent_workspace(const XentP& p, bool grad);
+int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws);
+int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dloss,
+                     const void* lse, void* ws);
+// Reads and clears the flag of its kernels' bounded waits (1 = one ran out).
+int xent_error();
 
 // leapfrog chains (k_leapfrog.cu)
 enum Family : int { FAM_NORMAL = 0, FAM_EXP = 1, FAM_STUDENTT = 2, FAM_CAUCHY = 3,

@@ -253,6 +253,15 @@ int sync(Ctx& c) {
     return OK;
 }
 
+bool capturing(Ctx& c) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c.stream, &st) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return st != cudaStreamCaptureStatusNone;
+}
+
 void* scratch(Ctx& c, size_t bytes, int slot) {
     if (bytes == 0) bytes = 256;
     std::lock_guard<std::mutex> lk(g_scratch_mu);

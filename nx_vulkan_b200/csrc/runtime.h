@@ -102,6 +102,9 @@ struct ScratchGuard {
     explicit ScratchGuard(Ctx& c) : lk(c.dev->scratch_mu) {}
 };
 
+// True while c.stream is being captured into a CUDA graph.
+bool capturing(Ctx& c);
+
 // Error reporting.
 void set_error(const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);

@@ -6,6 +6,7 @@
 // spv basename to a kernel family, checks buffer sizes against the element
 // counts it is asked to touch (the reference trusted the caller here), and
 // launches on the current device's stream.
+#include <math.h>
 #include <string.h>
 
 #include "../../include/nx_vulkan_shim.h"
@@ -465,6 +466,237 @@ int nxv_random_f64(void* out, unsigned long n, unsigned int seed, unsigned int d
     return launch_random(c, F64, dptr(out), n, seed, dist);
 }
 
+// ---- layer norm, dropout, linear cross entropy ------------------------------------------
+
+namespace {
+
+int dtype_ok(unsigned dtype, unsigned most, const char* what) {
+    if (dtype <= most) return OK;
+    set_error("%s: dtype %u out of range 0..%u", what, dtype, most);
+    return E_ARG;
+}
+
+// Two buffers of an op that must not share memory (sizes: the bytes used).
+bool share(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = (uintptr_t)dptr(a), y = (uintptr_t)dptr(b);
+    return na && nb && x < y + nb && y < x + na;
+}
+
+struct Span {
+    const void* h;
+    size_t bytes;
+    const char* what;
+    size_t align;  // the element's size
+};
+
+// Every span fits its buffer and starts on an element; no output (the first
+// n_out spans) shares memory with another span, but for the pairs of spans in
+// `same` (bit i * 8 + j), which may be one and the same buffer.
+int check_spans(const char* op, const Span* s, int n, int n_out, uint64_t same = 0) {
+    for (int i = 0; i < n; i++) {
+        if (nbytes(s[i].h) < s[i].bytes) {
+            set_error("%s %s: buffer of %zu bytes, op needs %zu", op, s[i].what, nbytes(s[i].h),
+                      s[i].bytes);
+            return E_ARG;
+        }
+        if ((uintptr_t)dptr(s[i].h) % s[i].align) {
+            set_error("%s %s: address not a multiple of %zu", op, s[i].what, s[i].align);
+            return E_ARG;
+        }
+    }
+    for (int i = 0; i < n_out; i++)
+        for (int j = i + 1; j < n; j++) {
+            if (!share(s[i].h, s[i].bytes, s[j].h, s[j].bytes)) continue;
+            if (((same >> (i * 8 + j)) & 1) && dptr(s[i].h) == dptr(s[j].h)) continue;
+            set_error("%s: %s shares memory with %s", op, s[i].what, s[j].what);
+            return E_ARG;
+        }
+    return OK;
+}
+
+// The caller's workspace, or library scratch of the stream (slot 0; the caller
+// holds a ScratchGuard).  A captured graph keeps the workspace's address, and
+// library scratch may move and is shared by the stream's ops, so a capture
+// must bring its own.
+int get_workspace(Ctx& c, void* handle, size_t bytes, const char* op, void** out) {
+    if (handle) {
+        if (nbytes(handle) < bytes || ((uintptr_t)dptr(handle) & 255)) {
+            set_error("%s workspace: buffer of %zu bytes, op needs %zu, on a 256-byte boundary", op,
+                      nbytes(handle), bytes);
+            return E_ARG;
+        }
+        *out = dptr(handle);
+        return OK;
+    }
+    if (capturing(c)) {
+        set_error("%s: a call captured into a CUDA graph needs a workspace of its own (%zu bytes)",
+                  op, bytes);
+        return E_ARG;
+    }
+    *out = scratch(c, bytes);
+    return *out ? OK : E_CUDA;
+}
+
+}  // namespace
+
+int nxv_layer_norm(void* y, void* mean, void* rstd, void* x, void* gamma, void* beta,
+                   unsigned int rows, unsigned int cols, double eps, unsigned int dtype,
+                   const char* spv_path) {
+    if (!y || !mean || !rstd || !x || !gamma || !beta || !spv_path) return E_NULL;
+    std::string k = spv_base(spv_path);
+    if (k != "layer_norm.spv") return bad_kernel(k);
+    if (int rc = dtype_ok(dtype, BF16, "layer_norm")) return rc;
+    if (cols == 0 || !(eps >= 0.0 && eps < HUGE_VAL)) {
+        set_error("layer_norm: cols %u must be positive, eps %g finite and not negative", cols, eps);
+        return E_ARG;
+    }
+    BEGIN(y, mean, rstd, x, gamma, beta);
+    const size_t es = dtype_bytes((int)dtype), as = dtype == F64 ? 8 : 4;
+    const size_t m = (size_t)rows * cols * es;
+    const Span s[] = {{y, m, "y", es},           {mean, rows * as, "mean", as},
+                      {rstd, rows * as, "rstd", as}, {x, m, "x", es},
+                      {gamma, cols * es, "gamma", es}, {beta, cols * es, "beta", es}};
+    if (int rc = check_spans("layer_norm", s, 6, 3, 1ull << 3 /* y may be x */)) return rc;
+    return launch_layer_norm(c, (int)dtype, dptr(y), dptr(mean), dptr(rstd), dptr(x), dptr(gamma),
+                             dptr(beta), rows, cols, eps);
+}
+
+unsigned long nxv_layer_norm_grad_workspace(unsigned int rows, unsigned int cols,
+                                            unsigned int dtype) {
+    return dtype > BF16 ? 0 : norm_grad_workspace(rows, cols, (int)dtype);
+}
+
+int nxv_layer_norm_grad(void* dx, void* dgamma, void* dbeta, void* workspace, void* dy, void* x,
+                        void* gamma, void* mean, void* rstd, unsigned int rows, unsigned int cols,
+                        unsigned int dtype, const char* spv_path) {
+    if (!dx || !dgamma || !dbeta || !dy || !x || !gamma || !mean || !rstd || !spv_path)
+        return E_NULL;
+    std::string k = spv_base(spv_path);
+    if (k != "layer_norm_grad.spv") return bad_kernel(k);
+    if (int rc = dtype_ok(dtype, BF16, "layer_norm_grad")) return rc;
+    if (cols == 0) {
+        set_error("layer_norm_grad: cols must be positive");
+        return E_ARG;
+    }
+    BEGIN(dx, dgamma, dbeta, workspace, dy, x, gamma, mean, rstd);
+    const size_t es = dtype_bytes((int)dtype), as = dtype == F64 ? 8 : 4;
+    const size_t m = (size_t)rows * cols * es, v = cols * es, w = norm_grad_workspace(rows, cols, (int)dtype);
+    Span s[9] = {{dx, m, "dx", es},          {dgamma, v, "dgamma", es},
+                 {dbeta, v, "dbeta", es},    {dy, m, "dy", es},
+                 {x, m, "x", es},            {gamma, v, "gamma", es},
+                 {mean, rows * as, "mean", as}, {rstd, rows * as, "rstd", as}};
+    int n = 8, n_out = 3;
+    // dx may be dy or x
+    uint64_t same = (1ull << 3) | (1ull << 4);
+    if (workspace) {  // an output too: put first
+        for (int i = n; i > 0; i--) s[i] = s[i - 1];
+        s[0] = {workspace, w, "workspace", 4};
+        n++, n_out++;
+        same = (1ull << (8 + 4)) | (1ull << (8 + 5));
+    }
+    if (int rc = check_spans("layer_norm_grad", s, n, n_out, same)) return rc;
+    ScratchGuard guard(c);
+    void* ws;
+    if (int rc = get_workspace(c, workspace, w, "layer_norm_grad", &ws)) return rc;
+    return launch_layer_norm_grad(c, (int)dtype, dptr(dx), dptr(dgamma), dptr(dbeta), ws, dptr(dy),
+                                  dptr(x), dptr(gamma), dptr(mean), dptr(rstd), rows, cols);
+}
+
+int nxv_dropout(void* out, void* x, unsigned long n, double p, unsigned int seed,
+                unsigned long offset, unsigned int dtype, const char* spv_path) {
+    if (!out || !x || !spv_path) return E_NULL;
+    std::string k = spv_base(spv_path);
+    if (k != "dropout.spv") return bad_kernel(k);
+    if (int rc = dtype_ok(dtype, BF16, "dropout")) return rc;
+    if (!(p >= 0.0 && p <= 1.0)) {
+        set_error("dropout: p %g out of range 0..1", p);
+        return E_ARG;
+    }
+    if (n > 0x100000000ul || offset > 0x100000000ul - n) {
+        set_error("dropout: elements %lu + %lu pass the stream's 2^32", offset, n);
+        return E_ARG;
+    }
+    BEGIN(out, x);
+    const size_t es = dtype_bytes((int)dtype);
+    const Span s[] = {{out, n * es, "out", es}, {x, n * es, "x", es}};
+    if (int rc = check_spans("dropout", s, 2, 1, 1ull << 1 /* out may be x */)) return rc;
+    return launch_dropout(c, (int)dtype, dptr(out), dptr(x), n, p, seed, offset);
+}
+
+static int xent_args(unsigned n, unsigned vocab, unsigned dim, unsigned dtype,
+                     unsigned index_bytes) {
+    if (dtype != F32 && dtype != BF16) {
+        set_error("linear_cross_entropy: dtype %u is not 0 (f32) or 2 (bf16)", dtype);
+        return E_ARG;
+    }
+    const unsigned most = 0x7ffffe00u;
+    if (vocab == 0 || dim == 0 || n > most || vocab > most || dim > most ||
+        (index_bytes != 4 && index_bytes != 8)) {
+        set_error("linear_cross_entropy: n %u / vocab %u / dim %u / index_bytes %u out of range", n,
+                  vocab, dim, index_bytes);
+        return E_ARG;
+    }
+    return OK;
+}
+
+unsigned long nxv_linear_cross_entropy_workspace(unsigned int n, unsigned int vocab,
+                                                 unsigned int dim, unsigned int dtype,
+                                                 unsigned int grad) {
+    if (xent_args(n, vocab, dim, dtype, 8) != OK) return 0;
+    XentP p{nullptr, nullptr, nullptr, 8, n, vocab, dim, (int)dtype};
+    return xent_workspace(p, grad != 0);
+}
+
+int nxv_linear_cross_entropy(void* loss, void* lse, void* workspace, void* x, void* w,
+                             void* labels, unsigned int n, unsigned int vocab, unsigned int dim,
+                             unsigned int dtype, unsigned int index_bytes, const char* spv_path) {
+    if (!loss || !lse || !x || !w || !labels || !spv_path) return E_NULL;
+    std::string k = spv_base(spv_path);
+    if (k != "linear_cross_entropy.spv") return bad_kernel(k);
+    if (int rc = xent_args(n, vocab, dim, dtype, index_bytes)) return rc;
+    BEGIN(loss, lse, workspace, x, w, labels);
+    XentP p{dptr(x), dptr(w), dptr(labels), (int)index_bytes, n, vocab, dim, (int)dtype};
+    const size_t es = dtype_bytes((int)dtype), need_ws = xent_workspace(p, false);
+    const Span s[] = {{loss, (size_t)n * 4, "loss", 4},
+                      {lse, (size_t)n * 4, "lse", 4},
+                      {workspace ? workspace : loss, workspace ? need_ws : 0, "workspace", 1},
+                      {x, (size_t)n * dim * es, "x", es},
+                      {w, (size_t)vocab * dim * es, "w", es},
+                      {labels, (size_t)n * index_bytes, "labels", index_bytes}};
+    if (int rc = check_spans("linear_cross_entropy", s, 6, 3)) return rc;
+    ScratchGuard guard(c);
+    void* ws;
+    if (int rc = get_workspace(c, workspace, need_ws, "linear_cross_entropy", &ws)) return rc;
+    return launch_xent(c, p, dptr(loss), dptr(lse), ws);
+}
+
+int nxv_linear_cross_entropy_grad(void* dx, void* dw, void* workspace, void* dloss, void* x,
+                                  void* w, void* labels, void* lse, unsigned int n,
+                                  unsigned int vocab, unsigned int dim, unsigned int dtype,
+                                  unsigned int index_bytes, const char* spv_path) {
+    if (!dx || !dw || !dloss || !x || !w || !labels || !lse || !spv_path) return E_NULL;
+    std::string k = spv_base(spv_path);
+    if (k != "linear_cross_entropy_grad.spv") return bad_kernel(k);
+    if (int rc = xent_args(n, vocab, dim, dtype, index_bytes)) return rc;
+    BEGIN(dx, dw, workspace, dloss, x, w, labels, lse);
+    XentP p{dptr(x), dptr(w), dptr(labels), (int)index_bytes, n, vocab, dim, (int)dtype};
+    const size_t es = dtype_bytes((int)dtype), need_ws = xent_workspace(p, true);
+    const size_t nx = (size_t)n * dim * es, nw = (size_t)vocab * dim * es;
+    const Span s[] = {{dx, nx, "dx", es},
+                      {dw, nw, "dw", es},
+                      {workspace ? workspace : dw, workspace ? need_ws : 0, "workspace", 1},
+                      {x, nx, "x", es},
+                      {w, nw, "w", es},
+                      {dloss, (size_t)n * 4, "dloss", 4},
+                      {labels, (size_t)n * index_bytes, "labels", index_bytes},
+                      {lse, (size_t)n * 4, "lse", 4}};
+    if (int rc = check_spans("linear_cross_entropy_grad", s, 8, 3)) return rc;
+    ScratchGuard guard(c);
+    void* ws;
+    if (int rc = get_workspace(c, workspace, need_ws, "linear_cross_entropy_grad", &ws)) return rc;
+    return launch_xent_grad(c, p, dptr(dx), dptr(dw), dptr(dloss), dptr(lse), ws);
+}
+
 // ---- HMC primitives ---------------------------------------------------------------------
 
 int nxv_kinetic_energy(void* out, void* p, void* inv_mass, unsigned int n, const char* spv_path) {
@@ -736,6 +968,10 @@ int nxv_synchronize(void) {
     int rc = sync(c);
     if (rc == OK && tc_gemm_error()) {
         set_error("tensor-core GEMM: a bounded pipeline wait ran out; results are invalid");
+        return E_CUDA;
+    }
+    if (rc == OK && xent_error()) {
+        set_error("linear cross entropy: a bounded pipeline wait ran out; results are invalid");
         return E_CUDA;
     }
     if (rc == OK && lr_traj_error()) {

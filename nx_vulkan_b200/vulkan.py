@@ -626,6 +626,162 @@ def fused_chain_imm(a, operands: Sequence, ops: Sequence, *, dtype="f32"):
     return _dispatch([out], rc)
 
 
+# ---- network ends: layer norm, dropout, linear cross entropy --------------------------------
+#
+# What a network over classes or tokens needs around its products; the
+# reference has no shader for them (Axon's layers run op by op on the backend).
+# dtype: "f32", "f64" or "bf16".  `out=` takes the caller's buffers (e.g.
+# wrap_tensor) in the order of the result; `workspace=` a buffer of the size
+# that the matching *_workspace function gives, for calls that may overlap with
+# others of the stream or are captured into a CUDA graph.  A captured call
+# needs both: memory of the pool may be handed to another call while the graph
+# still uses it.
+
+DTYPES = {"f32": 0, "f64": 1, "bf16": 2}
+_DTYPE_BYTES = {"f32": 4, "f64": 8, "bf16": 2}
+
+
+def _out_buffers(out, sizes):
+    """The caller's output buffers (checked) or new ones; (buffers, None) or (None, error)."""
+    if out is None:
+        bufs = [_alloc(n) for n in sizes]
+        return (None, (ERROR, "alloc_failed")) if None in bufs else (bufs, None)
+    if len(out) != len(sizes) or any(o.n_bytes < n for o, n in zip(out, sizes)):
+        return None, (ERROR, "size_mismatch")
+    return list(out), None
+
+
+def _dispatch_bufs(bufs, given, rc):
+    if given is None:
+        return _dispatch(bufs, rc)
+    return (OK, bufs[0] if len(bufs) == 1 else tuple(bufs)) if rc == 0 else (ERROR, "dispatch_failed")
+
+
+def _u32(*vals):
+    return all(0 <= v < 1 << 32 for v in vals)
+
+
+def layer_norm(x, gamma, beta, rows, cols, eps=1e-5, dtype="f32", out=None):
+    """Layer norm of the rows of x [rows, cols] with weights gamma, beta [cols].
+
+    Returns y (x's type) and every row's mean and 1 / sqrt(var + eps) (f32; f64
+    for f64).  y may be x (out=)."""
+    if dtype not in DTYPES or not _u32(rows, cols) or cols == 0 or not 0.0 <= eps < math.inf:
+        return (ERROR, "bad_op")
+    es, st = _DTYPE_BYTES[dtype], 8 if dtype == "f64" else 4
+    if x.n_bytes != rows * cols * es or gamma.n_bytes != cols * es or beta.n_bytes != cols * es:
+        return (ERROR, "size_mismatch")
+    bufs, err = _out_buffers(out, (rows * cols * es, rows * st, rows * st))
+    if err:
+        return err
+    rc = _lib().nxv_layer_norm(bufs[0].handle, bufs[1].handle, bufs[2].handle, x.handle,
+                               gamma.handle, beta.handle, rows, cols, eps, DTYPES[dtype],
+                               b"layer_norm.spv")
+    return _dispatch_bufs(bufs, out, rc)
+
+
+def layer_norm_grad_workspace(rows, cols, dtype="f32") -> int:
+    """Bytes of layer_norm_grad's workspace."""
+    return int(_lib().nxv_layer_norm_grad_workspace(rows, cols, DTYPES[dtype]))
+
+
+def layer_norm_grad(dy, x, gamma, mean, rstd, rows, cols, dtype="f32", out=None, workspace=None):
+    """Gradients of layer_norm from dy [rows, cols] and the forward call's mean
+    and rstd: dx [rows, cols] (may be dy or x, out=), dgamma and dbeta [cols]."""
+    if dtype not in DTYPES or not _u32(rows, cols) or cols == 0:
+        return (ERROR, "bad_op")
+    es, st = _DTYPE_BYTES[dtype], 8 if dtype == "f64" else 4
+    n = rows * cols * es
+    if (dy.n_bytes != n or x.n_bytes != n or gamma.n_bytes != cols * es
+            or mean.n_bytes != rows * st or rstd.n_bytes != rows * st):
+        return (ERROR, "size_mismatch")
+    bufs, err = _out_buffers(out, (n, cols * es, cols * es))
+    if err:
+        return err
+    rc = _lib().nxv_layer_norm_grad(bufs[0].handle, bufs[1].handle, bufs[2].handle,
+                                    workspace.handle if workspace is not None else None, dy.handle,
+                                    x.handle, gamma.handle, mean.handle, rstd.handle, rows, cols,
+                                    DTYPES[dtype], b"layer_norm_grad.spv")
+    return _dispatch_bufs(bufs, out, rc)
+
+
+def dropout(x, p, seed, offset=0, dtype="f32", out=None):
+    """x / (1 - p) where element offset + i of uniform(seed=seed) is >= p, else 0.
+
+    The mask is never stored: the gradient is dropout(dy, p, seed, offset).
+    `out=` may be x."""
+    if dtype not in DTYPES or not 0.0 <= p <= 1.0 or not _u32(seed):
+        return (ERROR, "bad_op")
+    es = _DTYPE_BYTES[dtype]
+    n = x.n_bytes // es
+    if n * es != x.n_bytes:
+        return (ERROR, "size_mismatch")
+    if offset < 0 or offset + n > 1 << 32:
+        return (ERROR, "bad_op")
+    o = _out_buffer(out, x.n_bytes)
+    if o is None:
+        return (ERROR, "alloc_failed" if out is None else "size_mismatch")
+    rc = _lib().nxv_dropout(o.handle, x.handle, n, p, seed, offset, DTYPES[dtype], b"dropout.spv")
+    return _dispatch_into(o, out, rc)
+
+
+def _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes):
+    if dtype not in ("f32", "bf16") or index_bytes not in (4, 8) or not _u32(n, vocab, dim):
+        return (ERROR, "bad_op")
+    if vocab == 0 or dim == 0:
+        return (ERROR, "bad_op")
+    es = _DTYPE_BYTES[dtype]
+    if (x.n_bytes != n * dim * es or w.n_bytes != vocab * dim * es
+            or labels.n_bytes != n * index_bytes):
+        return (ERROR, "size_mismatch")
+    return None
+
+
+def linear_cross_entropy_workspace(n, vocab, dim, dtype="f32", grad=False) -> int:
+    """Bytes of the workspace of linear_cross_entropy (or of its gradient)."""
+    return int(_lib().nxv_linear_cross_entropy_workspace(n, vocab, dim, DTYPES[dtype], int(grad)))
+
+
+def linear_cross_entropy(x, w, labels, n, vocab, dim, dtype="f32", index_bytes=8, out=None,
+                         workspace=None):
+    """Softmax cross entropy of z = x w^T (x [n, dim], w [vocab, dim]) against
+    integer labels [n], without storing z: every row's loss and log sum of
+    exponentials, f32 [n].  A label outside [0, vocab) marks a row without a
+    target (loss 0).  dtype "f32" or "bf16"."""
+    err = _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes)
+    if err:
+        return err
+    bufs, err = _out_buffers(out, (n * 4, n * 4))
+    if err:
+        return err
+    rc = _lib().nxv_linear_cross_entropy(bufs[0].handle, bufs[1].handle,
+                                         workspace.handle if workspace is not None else None,
+                                         x.handle, w.handle, labels.handle, n, vocab, dim,
+                                         DTYPES[dtype], index_bytes, b"linear_cross_entropy.spv")
+    return _dispatch_bufs(bufs, out, rc)
+
+
+def linear_cross_entropy_grad(dloss, x, w, labels, lse, n, vocab, dim, dtype="f32", index_bytes=8,
+                              out=None, workspace=None):
+    """Gradients of linear_cross_entropy from dloss (f32 [n], the gradient of
+    every row's loss: 1 / n for their mean) and the forward call's lse: dx [n,
+    dim] and dw [vocab, dim] in x's type."""
+    err = _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes)
+    if err:
+        return err
+    if dloss.n_bytes != n * 4 or lse.n_bytes != n * 4:
+        return (ERROR, "size_mismatch")
+    bufs, err = _out_buffers(out, (x.n_bytes, w.n_bytes))
+    if err:
+        return err
+    rc = _lib().nxv_linear_cross_entropy_grad(bufs[0].handle, bufs[1].handle,
+                                              workspace.handle if workspace is not None else None,
+                                              dloss.handle, x.handle, w.handle, labels.handle,
+                                              lse.handle, n, vocab, dim, DTYPES[dtype], index_bytes,
+                                              b"linear_cross_entropy_grad.spv")
+    return _dispatch_bufs(bufs, out, rc)
+
+
 # ---- HMC primitives (lib/nx_vulkan.ex:540-580; lib.rs:1082-1241) ----------------------------
 
 def kinetic_energy(p, inv_mass):
