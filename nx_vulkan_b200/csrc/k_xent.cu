@@ -39,11 +39,14 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-constexpr int BM = 128, BN = 256, BK = 64;  // BK bf16 = one 128-byte swizzle row
-constexpr int ST = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, ST_BYTES = A_BYTES + B_BYTES;
+// A CTA stages 128 rows of A and 128 of B, 64 of K deep.  Alone (CG = 1) it
+// makes a 128 x 128 tile; a pair of CTAs (CG = 2, tcgen05 cta_group::2) makes a
+// 256 x 256 tile, each holding the accumulator of its own 128 rows.
+constexpr int BT = 128, BK = 64;  // BK bf16 = one 128-byte swizzle row
+constexpr int ST = 6;
+constexpr int OP_BYTES = BT * BK * 2, ST_BYTES = 2 * OP_BYTES;
 constexpr int SMEM = ST * ST_BYTES + 1024 + 256;
-constexpr uint32_t TMEM_COLS = 512;  // two 128 x 256 f32 accumulators
+constexpr int kThreads = 384;  // producer of A, MMA issuer, allocator, producer of B, 8 epilogue warps
 
 __device__ int g_xent_error;
 
@@ -55,28 +58,35 @@ __device__ __forceinline__ uint32_t su32(const void* p) {
 __device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes)
+__device__ __forceinline__ void mbar_expect_tx(uint32_t b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes)
                  : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+// The address of the same shared-memory object in the pair's CTA 0.
+__device__ __forceinline__ uint32_t in_leader(uint32_t p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(p));
+    return r;
 }
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t b) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(su32(b)), "r"(parity)
+        : "r"(b), "r"(parity)
         : "memory");
     return ok != 0;
 }
-// Bounded wait (a few seconds at most); false when it runs out or when another
+// Bounded wait (seconds at most); false when it runs out or when another
 // warp of the CTA has given up.
-__device__ __noinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* err) {
-    for (uint32_t i = 0; i < (1u << 24); i++) {
+__device__ __noinline__ bool mbar_wait_long(uint32_t b, uint32_t parity, volatile int* err) {
+    for (uint32_t i = 0; i < (1u << 22); i++) {
         if (mbar_try(b, parity)) return true;
         if (i > 256) {
             if (*err) return false;
@@ -87,14 +97,26 @@ __device__ __noinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile in
     atomicExch(&g_xent_error, 1);
     return false;
 }
+__device__ __forceinline__ bool mbar_wait(uint32_t b, uint32_t parity, volatile int* err) {
+    return mbar_try(b, parity) || mbar_wait_long(b, parity, err);
+}
 
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                         uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(su32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(su32(bar))
-        : "memory");
+// Into this CTA's shared memory; the bytes count on the leader's barrier.
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            ".cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
 }
 
 // Shared-memory operand descriptor, 128-byte swizzle (layout type 2), sm_100
@@ -104,39 +126,58 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int 
 //   MN-major: blocks of 64 M (or N) elements x BK rows of K; the blocks are
 //     BK * 128 bytes apart (leading offset), 8-row groups along K 1024 bytes
 //     apart (stride offset); a K step of 16 advances by two groups.
-template <bool MN>
-__device__ __forceinline__ uint64_t sdesc(uint32_t saddr) {
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, bool mn) {
     uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(MN ? (BK * 128) >> 4 : 1) << 16;
+    d |= (uint64_t)(mn ? (BK * 128) >> 4 : 1) << 16;
     d |= (uint64_t)(1024 >> 4) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
     return d;
 }
-template <bool MN>
-constexpr uint64_t kstep() { return MN ? 2048 >> 4 : 32 >> 4; }
+__device__ __forceinline__ uint64_t kstep(bool mn) { return mn ? 2048 >> 4 : 32 >> 4; }
 
 // Instruction descriptor, kind::f16: D f32 (bits 4-5 = 1), A and B bf16
 // (bits 7-9, 10-12 = 1), bits 15 / 16: A / B MN-major, N >> 3 at bit 17,
 // M >> 4 at bit 24.
-template <bool A_MN, bool B_MN>
-constexpr uint32_t idesc() {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+template <int CG>
+__device__ __forceinline__ uint32_t idesc(bool a_mn, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(BT * CG >> 3) << 17) | ((uint32_t)(BT * CG >> 4) << 24);
 }
 
+template <int CG>
 __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t id,
                                           uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(id), "r"(acc));
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(acc));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(acc));
 }
-__device__ __forceinline__ void umma_commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     su32(b))
-                 : "memory");
+// Arrives on the barrier (of both CTAs of a pair) when every product issued
+// so far has completed.
+template <int CG>
+__device__ __forceinline__ void umma_commit(uint32_t b) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+            "[%0], %1;" ::"r"(b),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b)
+                     : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 #define TC_BEFORE() asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory")
@@ -185,47 +226,101 @@ __device__ __forceinline__ long long label_at(const void* labels, int bytes, siz
 
 // ---- the product kernel ---------------------------------------------------------
 
-enum Epi : int { EPI_LSE = 0, EPI_G = 1, EPI_OUT = 2 };
+enum Kind : int { LSE = 0, GRAD = 1, OUT = 2 };
 
-struct GemmArgs {
-    int M, N, K;       // D[M, N] = A[M, K] B[N, K]^T (either may be stored K-first)
-    int nprod;         // 1, or 6 for operands in three planes
-    long long col0;    // LSE, G: the class of column 0
+struct Job {
+    int kind;
+    int M, N, K;          // D[M, N] = A[M, K] B[N, K]^T
+    int a_mn, b_mn;       // the operand is stored K rows of M (N) values
+    uint32_t tm, tiles;   // row tiles, all tiles
+    long long col0;       // LSE, GRAD: the class of column 0
     // LSE
-    float* part_m;     // [column tile][M]
+    float* part_m;        // [column segment of 64 CG classes][M]
     float* part_s;
-    float* zlabel;     // [M]
-    // LSE, G
+    float* zlabel;        // [M]
+    // LSE, GRAD
     const void* labels;
     int index_bytes;
     long long vocab;
-    // G
+    // GRAD
     const float* lse;
     const float* dloss;
-    bf16* g;           // planes of [M][ldg]
+    bf16* g;              // planes of [M][ldg]
     long long ldg, gplane;
-    int planes;
     // OUT
-    float* acc;        // f32 [M][ldo]
-    void* out;         // f32 or bf16 [M][ldo]
+    const float* acc_in;  // f32 [M][ldo] to add, or null
+    void* out;            // [M][ldo]
     int out_bf16;
     long long ldo;
-    int mode;          // 0 out = D, 1 acc = D, 2 acc += D, 3 out = acc + D
 };
 
-__device__ __forceinline__ int prod_a(int p, int nprod) { return nprod == 1 ? 0 : (0x001102 >> (4 * p)) & 3; }
-__device__ __forceinline__ int prod_b(int p, int nprod) { return nprod == 1 ? 0 : (0x010120 >> (4 * p)) & 3; }
+constexpr int kMaxJobs = 3;
+struct alignas(64) Work {
+    CUtensorMap map[2 * kMaxJobs];  // A, B of every job
+    Job job[kMaxJobs];
+    int jobs;
+    uint32_t tiles;
+};
 
-// The row's maximum and sum of exponentials over the tile's columns.
-__device__ __forceinline__ void epi_lse(const GemmArgs& g, uint32_t tm, int row, int n0, int nt) {
+// The six partial products of f32, the smallest first.
+__device__ __forceinline__ int prod_a(int p) { return (0x001102 >> (4 * p)) & 3; }
+__device__ __forceinline__ int prod_b(int p) { return (0x010120 >> (4 * p)) & 3; }
+
+// 16 bytes x 2 of a row, with the widest store its address allows.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8], int align) {
+    if (align >= 32) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]),
+                     "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// One thread's row of a tile: 32 columns at a time go through chunk().
+// n0: the columns' first column of D; left: columns of D from there.
+struct Row {
+    const Job& g;
+    const int row, n0, left;
+    const bool live;
+    // LSE
     float m = -INFINITY, s = 0.0f, zl = 0.0f;
-    const int left = min(BN, g.N - n0);
-    const bool live = row < g.M;
-    const long long lab =
-        live ? label_at(g.labels, g.index_bytes, row) - (g.col0 + n0) : -1;  // column of the tile
-    for (int c0 = 0; c0 < left; c0 += 32) {
-        float v[32];
-        tmem_ld32(v, tm + c0);
+    long long lab = -1;  // the label's column, from n0
+    // GRAD
+    float lse = 0.0f, dl = 0.0f;
+    bool has = false;
+    int align = 0;
+
+    __device__ __forceinline__ Row(const Job& j, int r, int n) : g(j), row(r), n0(n), left(j.N - n), live(r < j.M) {
+        if (g.kind == OUT) {
+            const int es = g.out_bf16 ? 2 : 4;
+            const uintptr_t a = (uintptr_t)g.out | (uintptr_t)(g.ldo * es) | (uintptr_t)g.acc_in |
+                                (uintptr_t)(g.acc_in ? g.ldo * 4 : 0);
+            align = (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 4;
+        } else if (live) {
+            const long long l = label_at(g.labels, g.index_bytes, row);
+            has = l >= 0 && l < g.vocab;
+            lab = has ? l - (g.col0 + n0) : -1;
+            if (g.kind == GRAD) {
+                lse = g.lse[row];
+                dl = g.dloss[row];
+            }
+        }
+    }
+
+    __device__ __forceinline__ void chunk(float (&v)[32], int c0) {
+        if (c0 >= left) return;
+        if (g.kind == LSE) chunk_lse(v, c0);
+        else if (g.kind == GRAD) chunk_grad(v, c0);
+        else chunk_out(v, c0);
+    }
+
+    __device__ __forceinline__ void chunk_lse(float (&v)[32], int c0) {
         if (c0 + 32 > left) {
 #pragma unroll
             for (int e = 0; e < 32; e++)
@@ -250,135 +345,127 @@ __device__ __forceinline__ void epi_lse(const GemmArgs& g, uint32_t tm, int row,
         for (int e = 0; e < 32; e++) t[e & 3] += ex2(fmaf(v[e], kLog2e, -ref));
         s += (t[0] + t[1]) + (t[2] + t[3]);
     }
-    if (live) {
-        g.part_m[(size_t)nt * g.M + row] = m;
-        g.part_s[(size_t)nt * g.M + row] = s;
-        if (lab >= 0 && lab < left) g.zlabel[row] = zl;
-    }
-}
 
-__device__ __forceinline__ void epi_g(const GemmArgs& g, uint32_t tm, int row, int n0) {
-    const int left = min(BN, g.N - n0);
-    const bool live = row < g.M;
-    float lse = 0.0f, dl = 0.0f;
-    long long lab = -1;
-    bool has = false;
-    if (live) {
-        const long long l = label_at(g.labels, g.index_bytes, row);
-        has = l >= 0 && l < g.vocab;
-        lab = has ? l - (g.col0 + n0) : -1;
-        lse = g.lse[row];
-        dl = g.dloss[row];
-    }
-    for (int c0 = 0; c0 < left; c0 += 32) {
-        float v[32];
-        tmem_ld32(v, tm + c0);
-        if (!live) continue;
+    __device__ __forceinline__ void chunk_grad(float (&v)[32], int c0) {
+        if (!live) return;
 #pragma unroll
         for (int e = 0; e < 32; e++) {
             float p = ex2((v[e] - lse) * kLog2e);
             if (c0 + e == lab) p -= 1.0f;
             v[e] = has ? p * dl : 0.0f;
         }
+        // ldg covers whole tiles, so the columns past N have room; no product reads them
         bf16* dst = g.g + (size_t)row * g.ldg + n0 + c0;
-        if (g.planes == 1) {
+        if (g.gplane == 0) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint4 o;
-                __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&o);
+            for (int q = 0; q < 2; q++) {
+                uint32_t u[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    h[e] = __floats2bfloat162_rn(v[q * 8 + 2 * e], v[q * 8 + 2 * e + 1]);
-                reinterpret_cast<uint4*>(dst)[q] = o;
+                for (int e = 0; e < 8; e++) u[e] = pack2(v[q * 16 + 2 * e], v[q * 16 + 2 * e + 1]);
+                store32(dst + q * 16, u, 32);
             }
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint4 o[3];
+            for (int q = 0; q < 2; q++) {
+                uint32_t u[3][8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    bf16 b[3];
-                    split3(v[q * 8 + e], b[0], b[1], b[2]);
+                    bf16 a[3], b[3];
+                    split3(v[q * 16 + 2 * e], a[0], a[1], a[2]);
+                    split3(v[q * 16 + 2 * e + 1], b[0], b[1], b[2]);
 #pragma unroll
-                    for (int k = 0; k < 3; k++) reinterpret_cast<bf16*>(&o[k])[e] = b[k];
+                    for (int k = 0; k < 3; k++) {
+                        __nv_bfloat162 h = __halves2bfloat162(a[k], b[k]);
+                        u[k][e] = *reinterpret_cast<uint32_t*>(&h);
+                    }
                 }
 #pragma unroll
-                for (int k = 0; k < 3; k++) reinterpret_cast<uint4*>(dst + k * g.gplane)[q] = o[k];
+                for (int k = 0; k < 3; k++) store32(dst + k * g.gplane + q * 16, u[k], 32);
             }
         }
     }
-}
 
-__device__ __forceinline__ void epi_out(const GemmArgs& g, uint32_t tm, int row, int n0) {
-    const int left = min(BN, g.N - n0);
-    const bool live = row < g.M;
-    const bool vec = (g.ldo & 7) == 0 &&
-                     ((((uintptr_t)(g.mode == 0 || g.mode == 3 ? g.out : g.acc)) |
-                       ((uintptr_t)(g.mode == 0 ? nullptr : g.acc))) & 15) == 0;
-    for (int c0 = 0; c0 < left; c0 += 32) {
-        float v[32];
-        tmem_ld32(v, tm + c0);
-        if (!live) continue;
+    __device__ __forceinline__ void chunk_out(float (&v)[32], int c0) {
+        if (!live) return;
         const size_t at = (size_t)row * g.ldo + n0 + c0;
-        const bool whole = vec && c0 + 32 <= left;
-        if (g.mode >= 2) {
+        const bool whole = align >= 16 && c0 + 32 <= left;
+        if (g.acc_in) {
             if (whole) {
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    const float4 a = reinterpret_cast<const float4*>(g.acc + at)[q];
+                    const float4 a = reinterpret_cast<const float4*>(g.acc_in + at)[q];
                     v[4 * q] += a.x, v[4 * q + 1] += a.y, v[4 * q + 2] += a.z, v[4 * q + 3] += a.w;
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; e++)
-                    if (c0 + e < left) v[e] += g.acc[at + e];
+                    if (c0 + e < left) v[e] += g.acc_in[at + e];
             }
         }
-        const bool to_acc = g.mode == 1 || g.mode == 2;
-        if (to_acc || !g.out_bf16) {
-            float* o = to_acc ? g.acc + at : (float*)g.out + at;
-            if (whole) {
-#pragma unroll
-                for (int q = 0; q < 8; q++)
-                    reinterpret_cast<float4*>(o)[q] =
-                        make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                    if (c0 + e < left) o[e] = v[e];
-            }
-        } else {
+        if (g.out_bf16) {
             bf16* o = (bf16*)g.out + at;
             if (whole) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint4 u;
-                    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+                for (int q = 0; q < 2; q++) {
+                    uint32_t u[8];
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        h[e] = __floats2bfloat162_rn(v[q * 8 + 2 * e], v[q * 8 + 2 * e + 1]);
-                    reinterpret_cast<uint4*>(o)[q] = u;
+                    for (int e = 0; e < 8; e++) u[e] = pack2(v[q * 16 + 2 * e], v[q * 16 + 2 * e + 1]);
+                    store32(o + q * 16, u, align);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; e++)
                     if (c0 + e < left) o[e] = __float2bfloat16_rn(v[e]);
             }
+        } else {
+            float* o = (float*)g.out + at;
+            if (whole) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t u[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) u[e] = __float_as_uint(v[q * 8 + e]);
+                    store32(o + q * 8, u, align);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                    if (c0 + e < left) o[e] = v[e];
+            }
         }
     }
-}
 
-// Persistent: CTA b computes tiles b, b + gridDim.x, ... (row tile fastest, so
-// that the CTAs at work share the column operand's tiles in L2).
-//   warp 0 lane 0: TMA producer, ST stages of A (128 x 64) and B (256 x 64);
-//   warp 1 lane 0: MMA issuer into one of two accumulators in tensor memory;
-//   warps 4-7: epilogue of the other accumulator (warp q reads lanes 32 q ..).
-// Every wait is bounded; on a timeout each role stops, outstanding loads and
-// products are waited for (bounded), tensor memory is freed and g_xent_error set.
-template <int EPI, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(256, 1)
-k_xgemm(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensorMap mB,
-        const GemmArgs g) {
+    // width: the columns of the segment
+    __device__ __forceinline__ void done(int width) {
+        if (g.kind != LSE || !live || left <= 0) return;
+        const size_t at = (size_t)(n0 / width) * g.M + row;
+        g.part_m[at] = m;
+        g.part_s[at] = s;
+        if (lab >= 0 && lab < min(width, left)) g.zlabel[row] = zl;
+    }
+};
+
+// Persistent: CTA (pair) b computes tiles b, b + CTAs (pairs), ... of the
+// jobs one after the other (row tile fastest, so that the CTAs at work share
+// the column operand's tiles in L2).  Jobs of one launch do not depend on each
+// other; the host puts the one with the longest K first, so that the short
+// tiles fill the last wave.
+//   warps 0 and 3, lane 0: TMA producers, ST stages of 128 rows of A and of B;
+//   warp 1 lane 0 (of the leader): MMA issuer into one of two accumulators;
+//   warps 4-11: epilogue of the other (warp w: lanes 32 (w % 4), column half (w - 4) / 4).
+// SIX (f32): the six partial products, one k-block of all of them at a time:
+// the tensor core's sums lose up to a step of the running sum per product,
+// with a bias, so every k-block's sum is added to f32 registers by the
+// epilogue warps (round to nearest) while the next one is made.  Measured for
+// 2048 x 10007 x 1000: error of the gradients 1.9e-5 without, see below.
+// Every wait is bounded; on a timeout each role stops, loads and products in
+// flight are waited for (bounded), tensor memory is freed and g_xent_error set.
+template <int CG, bool SIX>
+__global__ void __launch_bounds__(kThreads, 1)
+k_xgemm(const __grid_constant__ Work W) {
+    constexpr int NC = BT * CG;       // accumulator columns
+    constexpr int HALF = NC / 2;      // columns of one epilogue warp
+    constexpr uint32_t COLS = 2 * NC; // tensor memory columns
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (su32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * ST_BYTES);
@@ -390,9 +477,8 @@ k_xgemm(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensor
     __shared__ volatile int s_err;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int KB = (g.K + BK - 1) / BK, KT = KB * g.nprod;
-    const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
-    const long long tiles = (long long)tm * tn;
+    const int rank = CG == 2 ? (blockIdx.x & 1) : 0;
+    const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
 
     if (tid == 0) {
         s_err = 0;
@@ -402,120 +488,200 @@ k_xgemm(const __grid_constant__ CUtensorMap mA, const __grid_constant__ CUtensor
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 128);
+            mbar_init(&acc_empty[b], 8 * CG);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         su32(tmem_slot)),
-                     "r"(TMEM_COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             su32(tmem_slot)),
+                         "r"(COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             su32(tmem_slot)),
+                         "r"(COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     TC_BEFORE();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();  // the peer's barriers are ready
     TC_AFTER();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        int it = 0;
+    // shared-memory addresses of the barriers (8 bytes each)
+    const uint32_t b_full = su32(full), b_empty = su32(empty), b_accf = su32(acc_full),
+                   b_acce = su32(acc_empty), ring = su32(smem);
+
+    if ((warp == 0 || warp == 3) && lane == 0) {
+        // One thread per operand: issuing a load takes ~150 cycles of a
+        // thread, and a stage is to be filled every 512 cycles.
+        const int is_b = warp == 3;
+        const uint32_t b_out = CG == 2 ? in_leader(b_full) : b_full;
+        uint32_t s = 0, par = 1, issued = 0;  // the first pass over the ring finds it empty
         bool ok = true;
-        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const int m0 = (int)(t % tm) * BM, n0 = (int)(t / tm) * BN;
-            for (int v = 0; v < KT; v++, it++) {
-                const int s = it % ST;
-                if (it >= ST && !mbar_wait(&empty[s], ((it / ST) + 1) & 1, &s_err)) {
-                    ok = false;
-                    break;
-                }
-                const int p = v / KB, k0 = (v - p * KB) * BK;
-                const int za = prod_a(p, g.nprod), zb = prod_b(p, g.nprod);
-                unsigned char* a = smem + s * ST_BYTES;
-                unsigned char* b = a + A_BYTES;
-                mbar_expect_tx(&full[s], ST_BYTES);
-                if constexpr (A_MN) {
+        for (uint32_t t = first; t < W.tiles && ok; t += step) {
+            uint32_t j = 0, lt = t;
+            while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
+            const uint32_t tm = W.job[j].tm;
+            const CUtensorMap* map = &W.map[2 * j + is_b];
+            const bool mn = is_b ? W.job[j].b_mn : W.job[j].a_mn;
+            const int r0 = (int)((is_b ? lt / tm : lt % tm) * NC + rank * BT);
+            const int K = W.job[j].K;
+            for (int k0 = 0; k0 < K && ok; k0 += BK) {
 #pragma unroll
-                    for (int j = 0; j < BM / 64; j++)
-                        tma_load(a + j * (BK * 128), &mA, m0 + j * 64, k0, za, &full[s]);
-                } else {
-                    tma_load(a, &mA, k0, m0, za, &full[s]);
-                }
-                if constexpr (B_MN) {
-#pragma unroll
-                    for (int j = 0; j < BN / 64; j++)
-                        tma_load(b + j * (BK * 128), &mB, n0 + j * 64, k0, zb, &full[s]);
-                } else {
-                    tma_load(b, &mB, k0, n0, zb, &full[s]);
+                for (int p = 0; p < (SIX ? 6 : 1); p++) {
+                    if (!mbar_wait(b_empty + s * 8, par, &s_err)) {
+                        ok = false;
+                        break;
+                    }
+                    const int z = !SIX ? 0 : is_b ? prod_b(p) : prod_a(p);
+                    const uint32_t dst = ring + s * ST_BYTES + is_b * OP_BYTES, bar = b_out + s * 8;
+                    if (rank == 0 && !is_b) mbar_expect_tx(b_full + s * 8, ST_BYTES * CG);
+                    if (mn) {
+                        tma_load<CG>(dst, map, r0, k0, z, bar);
+                        tma_load<CG>(dst + BK * 128, map, r0 + 64, k0, z, bar);
+                    } else {
+                        tma_load<CG>(dst, map, k0, r0, z, bar);
+                    }
+                    issued++;
+                    if (++s == ST) s = 0, par ^= 1;
                 }
             }
         }
-        // every load lands before the CTA's shared memory goes away (at once,
-        // unless a role has given up)
-        for (int i = it > ST ? it - ST : 0; i < it; i++)
-            for (uint32_t w = 0; w < (1u << 22) && !mbar_try(&full[i % ST], (i / ST) & 1); w++)
-                __nanosleep(100);
-    } else if (warp == 1 && lane == 0) {
-        int it = 0, i = 0;
+        // The last stages are read (and the pair's arrivals here made) before
+        // the CTA's shared memory goes away; after a timeout, the loads land.
+        for (uint32_t i = 0; i < ST && i < issued && ok; i++) {
+            if (s == 0) s = ST, par ^= 1;
+            s--;
+            ok = mbar_wait(b_empty + s * 8, par ^ 1, &s_err);
+        }
+        if (!ok)  // a millisecond, in which every load in flight has long landed
+            for (int w = 0; w < 1000; w++) __nanosleep(1000);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        uint32_t s = 0, par = 0, ph = 0;
         bool ok = true;
-        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x, i++) {
-            const int buf = i & 1;
-            if (i >= 2 && !mbar_wait(&acc_empty[buf], ((i >> 1) + 1) & 1, &s_err)) {
-                ok = false;
-                break;
-            }
-            TC_AFTER();
-            const uint32_t d = tmem + buf * BN;
-            for (int v = 0; v < KT; v++, it++) {
-                const int s = it % ST;
-                if (!mbar_wait(&full[s], (it / ST) & 1, &s_err)) {
+        for (uint32_t t = first; t < W.tiles && ok; t += step) {
+            uint32_t j = 0, lt = t;
+            while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
+            const bool a_mn = W.job[j].a_mn, b_mn = W.job[j].b_mn;
+            const uint32_t id = idesc<CG>(a_mn, b_mn);
+            const uint64_t ka = kstep(a_mn), kb = kstep(b_mn);
+            const uint64_t da0 = sdesc(ring, a_mn), db0 = sdesc(ring + OP_BYTES, b_mn);
+            const int KB = (W.job[j].K + BK - 1) / BK;
+            const int phases = SIX ? KB : 1, per = SIX ? 6 : KB;
+            for (int f = 0; f < phases && ok; f++, ph++) {
+                const uint32_t buf = ph & 1;
+                // the first two phases find the accumulators free
+                if (!mbar_wait(b_acce + buf * 8, ((ph >> 1) + 1) & 1, &s_err)) {
                     ok = false;
                     break;
                 }
                 TC_AFTER();
-                const uint32_t a = su32(smem + s * ST_BYTES);
-                const uint64_t da = sdesc<A_MN>(a), db = sdesc<B_MN>(a + A_BYTES);
+                const uint32_t d = tmem + buf * NC;
+                for (int v = 0; v < per; v++) {
+                    if (!mbar_wait(b_full + s * 8, par, &s_err)) {
+                        ok = false;
+                        break;
+                    }
+                    TC_AFTER();
+                    const uint64_t at = (uint64_t)(s * (ST_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < BK / 16; k++)
-                    umma_bf16(d, da + k * kstep<A_MN>(), db + k * kstep<B_MN>(),
-                              idesc<A_MN, B_MN>(), (v | k) ? 1u : 0u);
-                umma_commit(&empty[s]);
+                    for (int k = 0; k < BK / 16; k++)
+                        umma_bf16<CG>(d, da0 + at + k * ka, db0 + at + k * kb, id, (v | k) ? 1u : 0u);
+                    umma_commit<CG>(b_empty + s * 8);
+                    if (++s == ST) s = 0, par ^= 1;
+                }
+                if (ok) umma_commit<CG>(b_accf + buf * 8);
             }
-            if (ok) umma_commit(&acc_full[buf]);
         }
         if (!ok) {  // products in flight end before tensor memory is freed
-            umma_commit(drain);
-            for (uint32_t w = 0; w < (1u << 22) && !mbar_try(drain, 0); w++) __nanosleep(100);
+            umma_commit<CG>(su32(drain));
+            for (uint32_t w = 0; w < (1u << 14) && !mbar_try(su32(drain), 0); w++) __nanosleep(100);
         }
     } else if (warp >= 4) {
-        const int q = warp - 4;
-        int i = 0;
-        for (long long t = blockIdx.x; t < tiles; t += gridDim.x, i++) {
-            const int m0 = (int)(t % tm) * BM, nt = (int)(t / tm), n0 = nt * BN;
-            const int buf = i & 1;
-            const bool ok = mbar_wait(&acc_full[buf], (i >> 1) & 1, &s_err);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            TC_AFTER();
-            const uint32_t src = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
-            const int row = m0 + q * 32 + lane;
-            if constexpr (EPI == EPI_LSE) epi_lse(g, src, row, n0, nt);
-            else if constexpr (EPI == EPI_G) epi_g(g, src, row, n0);
-            else epi_out(g, src, row, n0);
-            TC_BEFORE();
-            mbar_arrive(&acc_empty[buf]);
+        const int q = warp & 3, h = (warp - 4) >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + h * HALF;
+        const uint32_t b_free = in_leader(b_acce);
+        uint32_t ph = 0;
+        bool ok = true;
+        for (uint32_t t = first; t < W.tiles && ok; t += step) {
+            uint32_t j = 0, lt = t;
+            while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
+            const Job& g = W.job[j];
+            const int row = (int)(lt % g.tm * NC) + rank * BT + q * 32 + lane;
+            const int n0 = (int)(lt / g.tm * NC) + h * HALF;
+            if constexpr (SIX) {
+                const int KB = (g.K + BK - 1) / BK;
+                float acc[HALF];
+#pragma unroll
+                for (int e = 0; e < HALF; e++) acc[e] = 0.0f;
+                for (int f = 0; f < KB; f++, ph++) {
+                    const uint32_t buf = ph & 1;
+                    ok = __all_sync(0xffffffffu, mbar_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err));
+                    if (!ok) break;
+                    TC_AFTER();
+#pragma unroll
+                    for (int c = 0; c < HALF / 32; c++) {
+                        float v[32];
+                        tmem_ld32(v, lanes + buf * NC + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) acc[c * 32 + e] += v[e];
+                    }
+                    TC_BEFORE();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(b_free + buf * 8);
+                }
+                if (!ok) break;
+                Row r(g, row, n0);
+#pragma unroll
+                for (int c = 0; c < HALF / 32; c++) {
+                    float v[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = acc[c * 32 + e];
+                    r.chunk(v, c * 32);
+                }
+                r.done(HALF);
+            } else {
+                const uint32_t buf = ph & 1;
+                Row r(g, row, n0);
+                ok = __all_sync(0xffffffffu, mbar_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err));
+                if (!ok) break;
+                ph++;
+                TC_AFTER();
+#pragma unroll 1
+                for (int c = 0; c < HALF / 32; c++) {
+                    float v[32];
+                    tmem_ld32(v, lanes + buf * NC + c * 32);
+                    r.chunk(v, c * 32);
+                }
+                TC_BEFORE();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_leader(b_free + buf * 8);
+                r.done(HALF);
+            }
         }
     }
     __syncwarp();
     TC_BEFORE();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     if (warp == 2) {
         TC_AFTER();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"(TMEM_COLS)
-                     : "memory");
+        if constexpr (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS)
+                         : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS)
+                         : "memory");
     }
+    if constexpr (CG == 2) cluster_sync();
 }
 
 // ---- small kernels -----------------------------------------------------------------
@@ -622,41 +788,79 @@ int make_map(CUtensorMap* map, const void* base, size_t cols, size_t rows, size_
     return OK;
 }
 
-template <int EPI, bool A_MN, bool B_MN>
-int run_gemm(Ctx& c, const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g) {
-    NXV_CK(cudaFuncSetAttribute(k_xgemm<EPI, A_MN, B_MN>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-    const long long tiles = (long long)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
-    const unsigned grid = (unsigned)std::min<long long>(tiles, c.dev->sm_count);
-    k_xgemm<EPI, A_MN, B_MN><<<grid, 256, SMEM, c.stream>>>(a, b, g);
+template <int CG, bool SIX>
+int launch_work(Ctx& c, const Work& w) {
+    NXV_CK(cudaFuncSetAttribute(k_xgemm<CG, SIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min<uint32_t>(w.tiles, c.dev->sm_count / CG) * CG));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NXV_CK(cudaLaunchKernelEx(&cfg, k_xgemm<CG, SIX>, w));
     count_launch();
     return OK;
+}
+
+int run_work(Ctx& c, const Work& w, int cg, bool six) {
+    if (cg == 2) return six ? launch_work<2, true>(c, w) : launch_work<2, false>(c, w);
+    return six ? launch_work<1, true>(c, w) : launch_work<1, false>(c, w);
+}
+
+// Adds a job; jobs with a longer K come first.
+void add_job(Work& w, Job j, const CUtensorMap& a, const CUtensorMap& b, int cg) {
+    const int t = BT * cg;
+    j.tm = (j.M + t - 1) / t;
+    j.tiles = j.tm * ((j.N + t - 1) / t);  // below 2^31: the entry points check
+    int at = w.jobs;
+    while (at > 0 && w.job[at - 1].K < j.K) {
+        w.job[at] = w.job[at - 1];
+        w.map[2 * at] = w.map[2 * at - 2];
+        w.map[2 * at + 1] = w.map[2 * at - 1];
+        at--;
+    }
+    w.job[at] = j;
+    w.map[2 * at] = a;
+    w.map[2 * at + 1] = b;
+    w.jobs++;
+    w.tiles += j.tiles;
 }
 
 size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 // How a call uses its workspace.  The vocabulary is cut into pieces of vp
-// classes (a multiple of the column tile) so that the piece's G, and its
-// packed w where w cannot be read in place, stay within a fixed budget.
+// classes (a multiple of the widest tile) so that a piece's G, and its packed
+// w where w cannot be read in place, stay within a fixed budget.  The gradient
+// holds two pieces: a launch makes G of one while it multiplies the other.
 struct Plan {
-    int planes;
-    size_t dp;               // packed row length
+    int planes, cg;
+    size_t dp;                // packed row length
     size_t vp, pieces;
-    size_t xp, wp, g, ldg, acc, pm, ps, zl, total;  // byte offsets; ldg in elements
+    size_t seg;               // classes of one (maximum, sum) entry
+    size_t xp, wp[2], g[2], ldg, acc, pm, ps, zl, total;  // byte offsets; ldg in elements
 };
 
-constexpr size_t kPieceBytes = (size_t)256 << 20;
+constexpr size_t kPieceBytes = (size_t)128 << 20;
+constexpr size_t kTile = 2 * BT;
 
 Plan make_plan(const XentP& p, bool grad) {
     Plan q{};
     q.planes = p.dt == F32 ? 3 : 1;
+    q.cg = p.n > BT && p.vocab > BT ? 2 : 1;
+    q.seg = (size_t)BT * q.cg / 2;
     q.dp = up(p.dim, 8);
     const size_t per_class = (size_t)q.planes * 2 * (q.dp + (grad ? (size_t)p.n : 0));
-    size_t vp = std::max<size_t>(kPieceBytes / per_class / BN * BN, 4 * BN);
-    const size_t all = up(p.vocab, BN);
+    size_t vp = std::max<size_t>(kPieceBytes / per_class / kTile * kTile, 4 * kTile);
+    const size_t all = up(p.vocab, kTile);
     vp = std::min(vp, all);
     q.pieces = (p.vocab + vp - 1) / vp;
-    q.vp = up((p.vocab + q.pieces - 1) / q.pieces, BN);
+    q.vp = up((p.vocab + q.pieces - 1) / q.pieces, kTile);
     q.pieces = (p.vocab + q.vp - 1) / q.vp;
     q.ldg = q.vp;
     size_t at = 0;
@@ -666,14 +870,16 @@ Plan make_plan(const XentP& p, bool grad) {
         return o;
     };
     q.xp = take((size_t)q.planes * 2 * p.n * q.dp);
-    q.wp = take((size_t)q.planes * 2 * q.vp * q.dp);
+    for (int b = 0; b < 2; b++)
+        q.wp[b] = b < (grad ? (int)q.pieces : 1) ? take((size_t)q.planes * 2 * q.vp * q.dp) : q.wp[0];
     if (grad) {
-        q.g = take((size_t)q.planes * 2 * p.n * q.ldg);
-        q.acc = take(p.dt == BF16 ? (size_t)4 * p.n * p.dim : 0);
+        for (int b = 0; b < 2; b++)
+            q.g[b] = b < (int)q.pieces ? take((size_t)q.planes * 2 * p.n * q.ldg) : q.g[0];
+        q.acc = take(p.dt == BF16 && q.pieces > 1 ? (size_t)4 * p.n * p.dim : 0);
     } else {
-        const size_t tiles = all / BN;
-        q.pm = take(4 * tiles * p.n);
-        q.ps = take(4 * tiles * p.n);
+        const size_t segs = (p.vocab + q.seg - 1) / q.seg;
+        q.pm = take(4 * segs * p.n);
+        q.ps = take(4 * segs * p.n);
         q.zl = take((size_t)4 * p.n);
     }
     q.total = at;
@@ -726,11 +932,11 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     }
     CUtensorMap ma, mb;
     int rc;
-    if ((rc = make_map(&ma, xp, p.dim, p.n, q.dp, q.planes, (size_t)p.n * q.dp, BM))) return rc;
-    GemmArgs g{};
+    if ((rc = make_map(&ma, xp, p.dim, p.n, q.dp, q.planes, (size_t)p.n * q.dp, BT))) return rc;
+    Job g{};
+    g.kind = LSE;
     g.M = (int)p.n;
     g.K = (int)p.dim;
-    g.nprod = q.planes == 3 ? 6 : 1;
     g.zlabel = (float*)(base + q.zl);
     g.labels = p.labels;
     g.index_bytes = p.index_bytes;
@@ -740,21 +946,23 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
         const size_t nv = std::min<size_t>(vp, p.vocab - v0);
         const bf16* wp = (const bf16*)p.w;
         if (!wip) {
-            wp = (bf16*)(base + q.wp);
+            wp = (bf16*)(base + q.wp[0]);
             pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * dtype_bytes(p.dt), nv, (int)q.dp,
                  false);
         }
-        if ((rc = make_map(&mb, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BN))) return rc;
+        if ((rc = make_map(&mb, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BT))) return rc;
         g.N = (int)nv;
         g.col0 = (long long)v0;
-        g.part_m = (float*)(base + q.pm) + v0 / BN * p.n;
-        g.part_s = (float*)(base + q.ps) + v0 / BN * p.n;
-        if ((rc = run_gemm<EPI_LSE, false, false>(c, ma, mb, g))) return rc;
+        g.part_m = (float*)(base + q.pm) + v0 / q.seg * p.n;
+        g.part_s = (float*)(base + q.ps) + v0 / q.seg * p.n;
+        Work w{};
+        add_job(w, g, ma, mb, q.cg);
+        if ((rc = run_work(c, w, q.cg, q.planes == 3))) return rc;
     }
     k_xent_join<<<(p.n + 31) / 32, dim3(32, 8), 0, c.stream>>>(
         (float*)loss, (float*)lse, (const float*)(base + q.pm), (const float*)(base + q.ps),
         (const float*)(base + q.zl), p.labels, p.index_bytes, p.vocab, p.n,
-        (int)((p.vocab + BN - 1) / BN));
+        (int)((p.vocab + q.seg - 1) / q.seg));
     count_launch();
     pdl_record_all(c);
     return finish(c);
@@ -768,64 +976,73 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
     }
     const Plan q = make_plan(p, true);
     char* base = (char*)ws;
-    const bool wip = in_place(p, p.w);
+    const bool wip = in_place(p, p.w), six = q.planes == 3;
+    const size_t es = dtype_bytes(p.dt);
     bf16* xp = (bf16*)(base + q.xp);
-    bf16* gp = (bf16*)(base + q.g);
     pack(c, p, xp, p.x, p.n, (int)q.dp, true);
     const size_t xplane = (size_t)p.n * q.dp, gplane = (size_t)p.n * q.ldg;
     CUtensorMap mxk, mxn, mwk, mwn, mgk, mgm;
     int rc;
     // x: K-major A of z = x w^T, and N-major B of dw = G^T x
-    if ((rc = make_map(&mxk, xp, p.dim, p.n, q.dp, q.planes, xplane, BM))) return rc;
+    if ((rc = make_map(&mxk, xp, p.dim, p.n, q.dp, q.planes, xplane, BT))) return rc;
     if ((rc = make_map(&mxn, xp, p.dim, p.n, q.dp, q.planes, xplane, BK))) return rc;
-    GemmArgs z{};
+    Job z{};
+    z.kind = GRAD;
     z.M = (int)p.n;
     z.K = (int)p.dim;
-    z.nprod = q.planes == 3 ? 6 : 1;
     z.labels = p.labels;
     z.index_bytes = p.index_bytes;
     z.vocab = p.vocab;
     z.lse = (const float*)lse;
     z.dloss = (const float*)dloss;
-    z.g = gp;
     z.ldg = (long long)q.ldg;
-    z.gplane = (long long)gplane;
-    z.planes = q.planes;
-    for (size_t v0 = 0, i = 0; v0 < p.vocab; v0 += q.vp, i++) {
-        const size_t nv = std::min<size_t>(q.vp, p.vocab - v0);
-        const bf16* wp = (const bf16*)p.w + (wip ? v0 * p.dim : 0);
-        if (!wip) {
-            wp = (bf16*)(base + q.wp);
-            pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * dtype_bytes(p.dt), nv, (int)q.dp,
-                 false);
+    z.gplane = six ? (long long)gplane : 0;
+    // launch i: G of piece i, and the products of piece i - 1
+    for (size_t i = 0; i <= q.pieces; i++) {
+        Work w{};
+        if (i > 0) {
+            const size_t v0 = (i - 1) * q.vp, nv = std::min<size_t>(q.vp, p.vocab - v0);
+            const bool first = i == 1, last = i == q.pieces;
+            const bf16* gp = (const bf16*)(base + q.g[(i - 1) & 1]);
+            const bf16* wp = wip ? (const bf16*)p.w + v0 * p.dim : (bf16*)(base + q.wp[(i - 1) & 1]);
+            if ((rc = make_map(&mwn, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BK))) return rc;
+            if ((rc = make_map(&mgk, gp, nv, p.n, q.ldg, q.planes, gplane, BT))) return rc;
+            if ((rc = make_map(&mgm, gp, nv, p.n, q.ldg, q.planes, gplane, BK))) return rc;
+            Job o{};
+            o.kind = OUT;
+            o.ldo = p.dim;
+            o.N = (int)p.dim;
+            o.b_mn = 1;
+            // dx += G w: K runs over the piece's classes; the sum so far is f32
+            o.M = (int)p.n;
+            o.K = (int)nv;
+            o.out_bf16 = !six && last;
+            o.out = six || last ? dx : base + q.acc;
+            o.acc_in = first ? nullptr : six ? (const float*)dx : (const float*)(base + q.acc);
+            add_job(w, o, mgk, mwn, q.cg);
+            // dw = G^T x: K runs over the tokens
+            o.M = (int)nv;
+            o.K = (int)p.n;
+            o.a_mn = 1;
+            o.out_bf16 = !six;
+            o.out = (char*)dw + v0 * p.dim * es;
+            o.acc_in = nullptr;
+            add_job(w, o, mgm, mxn, q.cg);
         }
-        if ((rc = make_map(&mwk, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BN))) return rc;
-        if ((rc = make_map(&mwn, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BK))) return rc;
-        if ((rc = make_map(&mgk, gp, nv, p.n, q.ldg, q.planes, gplane, BM))) return rc;
-        if ((rc = make_map(&mgm, gp, nv, p.n, q.ldg, q.planes, gplane, BK))) return rc;
-        z.N = (int)nv;
-        z.col0 = (long long)v0;
-        if ((rc = run_gemm<EPI_G, false, false>(c, mxk, mwk, z))) return rc;
-        GemmArgs o{};
-        o.nprod = z.nprod;
-        o.out_bf16 = p.dt == BF16;
-        o.ldo = p.dim;
-        // dx += G w: K runs over the piece's classes
-        o.M = (int)p.n;
-        o.N = (int)p.dim;
-        o.K = (int)nv;
-        const bool first = i == 0, last = v0 + nv == p.vocab;
-        o.out = dx;
-        o.acc = p.dt == BF16 ? (float*)(base + q.acc) : (float*)dx;
-        o.mode = p.dt == F32 ? (first ? 1 : 2) : first ? (last ? 0 : 1) : (last ? 3 : 2);
-        if ((rc = run_gemm<EPI_OUT, false, true>(c, mgk, mwn, o))) return rc;
-        // dw = G^T x: K runs over the tokens
-        o.M = (int)nv;
-        o.K = (int)p.n;
-        o.out = (char*)dw + v0 * p.dim * dtype_bytes(p.dt);
-        o.acc = nullptr;
-        o.mode = 0;
-        if ((rc = run_gemm<EPI_OUT, true, true>(c, mgm, mxn, o))) return rc;
+        if (i < q.pieces) {
+            const size_t v0 = i * q.vp, nv = std::min<size_t>(q.vp, p.vocab - v0);
+            const bf16* wp = (const bf16*)p.w + (wip ? v0 * p.dim : 0);
+            if (!wip) {
+                wp = (bf16*)(base + q.wp[i & 1]);
+                pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * es, nv, (int)q.dp, false);
+            }
+            if ((rc = make_map(&mwk, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BT))) return rc;
+            z.N = (int)nv;
+            z.col0 = (long long)v0;
+            z.g = (bf16*)(base + q.g[i & 1]);
+            add_job(w, z, mxk, mwk, q.cg);
+        }
+        if ((rc = run_work(c, w, q.cg, six))) return rc;
     }
     pdl_record_all(c);
     return finish(c);
