@@ -11,20 +11,25 @@
 // the backward pass because it is not kept: 8 n vocab dim in all, on the
 // tcgen05 tensor cores.  All go through one kernel, k_xgemm, with an epilogue
 // each:
-//   LSE  the maximum and the sum of exponentials of every row over the tile's
-//        classes (8 bytes per row and tile instead of the logits) and the
-//        label's logit; a small kernel joins the tiles;
-//   G    G as bf16 for one piece of the vocabulary at a time;
-//   OUT  dx += G_piece w_piece in f32, and dw_piece = G_piece^T x.
+//   LSE   the maximum and the sum of exponentials of every row over a segment
+//         of classes (8 bytes per row and segment instead of the logits) and
+//         the label's logit; a small kernel joins the segments;
+//   GRAD  P = exp(z - lse) - [v = label] for one piece of the vocabulary at a
+//         time, as bf16;
+//   OUT   dx = dloss (sum over pieces of P w), the sum in f32, and
+//         dw_piece = P^T (dloss x).
 //
-// Types.  bf16: the operands go to the tensor core as they are; G is rounded
-// to bf16 once (2^-8 relative to each entry at most, like the operands of the
-// products that follow it), sums are f32.  f32: every f32 value is the sum
-// of three bf16 values, b0 = bf16(v), b1 = bf16(v - b0), b2 = bf16(v - b0 - b1)
-// (exact but for values below 2^-110), and a product is the six partial
-// products b_i b_j with i + j <= 2, the smallest first; the three left out are
-// below 2^-24 of the product.  bf16 has f32's exponent range, so no scaling is
-// needed, and six bf16 products cost what three TF32 products cost.
+// Types.  bf16: the operands go to the tensor core as they are; sums are f32.
+// Two roundings to bf16 stand between the inputs and the sums of the gradient
+// (2^-8 relative to each term at most, like the rounding of the inputs): P
+// without the factor dloss, so that the label's entry, near -1, is nearly exact
+// (with it, all rows of a mean loss would round the same value, by up to 2^-8),
+// and dloss x, in units of the largest dloss, which leaves x as it is for a mean.
+// f32: every f32 value is the sum of three bf16 values, b0 = bf16(v),
+// b1 = bf16(v - b0), b2 = bf16(v - b0 - b1) (exact but for values below 2^-110),
+// and a product is the six partial products b_i b_j with i + j <= 2; the three
+// left out are below 2^-24 of the product.  bf16 has f32's exponent range, so
+// no scaling is needed, and six bf16 products cost what three TF32 products cost.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -175,6 +180,21 @@ __device__ __forceinline__ void umma_commit(uint32_t b) {
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b)
                      : "memory");
 }
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A whole warp's wait: the same answer in every lane, so that the loops around
+// it stay uniform and their addresses in uniform registers.
+__device__ __forceinline__ bool warp_wait(uint32_t b, uint32_t parity, volatile int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, err));
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -244,11 +264,12 @@ struct Job {
     long long vocab;
     // GRAD
     const float* lse;
-    const float* dloss;
     bf16* g;              // planes of [M][ldg]
     long long ldg, gplane;
     // OUT
     const float* acc_in;  // f32 [M][ldo] to add, or null
+    const float* dloss;   // [M]: the rows' factors, 0 for a row without a target; or null
+    const float* factor;  // one factor of all, or null
     void* out;            // [M][ldo]
     int out_bf16;
     long long ldo;
@@ -292,9 +313,11 @@ struct Row {
     float m = -INFINITY, s = 0.0f, zl = 0.0f;
     long long lab = -1;  // the label's column, from n0
     // GRAD
-    float lse = 0.0f, dl = 0.0f;
-    bool has = false;
+    float lse = 0.0f;
+    // OUT
+    float dl = 0.0f;
     int align = 0;
+    bool has = false;
 
     __device__ __forceinline__ Row(const Job& j, int r, int n) : g(j), row(r), n0(n), left(j.N - n), live(r < j.M) {
         if (g.kind == OUT) {
@@ -302,14 +325,13 @@ struct Row {
             const uintptr_t a = (uintptr_t)g.out | (uintptr_t)(g.ldo * es) | (uintptr_t)g.acc_in |
                                 (uintptr_t)(g.acc_in ? g.ldo * 4 : 0);
             align = (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 4;
-        } else if (live) {
+        }
+        if (live && (g.kind != OUT || g.dloss)) {
             const long long l = label_at(g.labels, g.index_bytes, row);
             has = l >= 0 && l < g.vocab;
             lab = has ? l - (g.col0 + n0) : -1;
-            if (g.kind == GRAD) {
-                lse = g.lse[row];
-                dl = g.dloss[row];
-            }
+            if (g.kind == GRAD) lse = g.lse[row];
+            if (g.kind == OUT) dl = g.dloss[row];
         }
     }
 
@@ -352,7 +374,7 @@ struct Row {
         for (int e = 0; e < 32; e++) {
             float p = ex2((v[e] - lse) * kLog2e);
             if (c0 + e == lab) p -= 1.0f;
-            v[e] = has ? p * dl : 0.0f;
+            v[e] = has ? p : 0.0f;
         }
         // ldg covers whole tiles, so the columns past N have room; no product reads them
         bf16* dst = g.g + (size_t)row * g.ldg + n0 + c0;
@@ -401,6 +423,15 @@ struct Row {
                 for (int e = 0; e < 32; e++)
                     if (c0 + e < left) v[e] += g.acc_in[at + e];
             }
+        }
+        if (g.dloss) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = has ? v[e] * dl : 0.0f;
+        }
+        if (g.factor) {
+            const float f = *g.factor;
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] *= f;
         }
         if (g.out_bf16) {
             bf16* o = (bf16*)g.out + at;
@@ -476,7 +507,7 @@ k_xgemm(const __grid_constant__ Work W) {
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     __shared__ volatile int s_err;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = CG == 2 ? (blockIdx.x & 1) : 0;
     const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -519,10 +550,11 @@ k_xgemm(const __grid_constant__ Work W) {
     const uint32_t b_full = su32(full), b_empty = su32(empty), b_accf = su32(acc_full),
                    b_acce = su32(acc_empty), ring = su32(smem);
 
-    if ((warp == 0 || warp == 3) && lane == 0) {
-        // One thread per operand: issuing a load takes ~150 cycles of a
-        // thread, and a stage is to be filled every 512 cycles.
+    if (warp == 0 || warp == 3) {
+        // One warp per operand, one lane of it issuing: two loads of a stage
+        // by one thread would take as long as the stage's products.
         const int is_b = warp == 3;
+        const bool one = elect_one();
         const uint32_t b_out = CG == 2 ? in_leader(b_full) : b_full;
         uint32_t s = 0, par = 1, issued = 0;  // the first pass over the ring finds it empty
         bool ok = true;
@@ -537,18 +569,18 @@ k_xgemm(const __grid_constant__ Work W) {
             for (int k0 = 0; k0 < K && ok; k0 += BK) {
 #pragma unroll
                 for (int p = 0; p < (SIX ? 6 : 1); p++) {
-                    if (!mbar_wait(b_empty + s * 8, par, &s_err)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = warp_wait(b_empty + s * 8, par, &s_err);
+                    if (!ok) break;
                     const int z = !SIX ? 0 : is_b ? prod_b(p) : prod_a(p);
                     const uint32_t dst = ring + s * ST_BYTES + is_b * OP_BYTES, bar = b_out + s * 8;
-                    if (rank == 0 && !is_b) mbar_expect_tx(b_full + s * 8, ST_BYTES * CG);
-                    if (mn) {
-                        tma_load<CG>(dst, map, r0, k0, z, bar);
-                        tma_load<CG>(dst + BK * 128, map, r0 + 64, k0, z, bar);
-                    } else {
-                        tma_load<CG>(dst, map, k0, r0, z, bar);
+                    if (one) {
+                        if (rank == 0 && !is_b) mbar_expect_tx(b_full + s * 8, ST_BYTES * CG);
+                        if (mn) {
+                            tma_load<CG>(dst, map, r0, k0, z, bar);
+                            tma_load<CG>(dst + BK * 128, map, r0 + 64, k0, z, bar);
+                        } else {
+                            tma_load<CG>(dst, map, k0, r0, z, bar);
+                        }
                     }
                     issued++;
                     if (++s == ST) s = 0, par ^= 1;
@@ -560,11 +592,12 @@ k_xgemm(const __grid_constant__ Work W) {
         for (uint32_t i = 0; i < ST && i < issued && ok; i++) {
             if (s == 0) s = ST, par ^= 1;
             s--;
-            ok = mbar_wait(b_empty + s * 8, par ^ 1, &s_err);
+            ok = warp_wait(b_empty + s * 8, par ^ 1, &s_err);
         }
         if (!ok)  // a millisecond, in which every load in flight has long landed
             for (int w = 0; w < 1000; w++) __nanosleep(1000);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+        const bool one = elect_one();
         uint32_t s = 0, par = 0, ph = 0;
         bool ok = true;
         for (uint32_t t = first; t < W.tiles && ok; t += step) {
@@ -579,29 +612,28 @@ k_xgemm(const __grid_constant__ Work W) {
             for (int f = 0; f < phases && ok; f++, ph++) {
                 const uint32_t buf = ph & 1;
                 // the first two phases find the accumulators free
-                if (!mbar_wait(b_acce + buf * 8, ((ph >> 1) + 1) & 1, &s_err)) {
-                    ok = false;
-                    break;
-                }
+                ok = warp_wait(b_acce + buf * 8, ((ph >> 1) + 1) & 1, &s_err);
+                if (!ok) break;
                 TC_AFTER();
                 const uint32_t d = tmem + buf * NC;
                 for (int v = 0; v < per; v++) {
-                    if (!mbar_wait(b_full + s * 8, par, &s_err)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = warp_wait(b_full + s * 8, par, &s_err);
+                    if (!ok) break;
                     TC_AFTER();
-                    const uint64_t at = (uint64_t)(s * (ST_BYTES >> 4));
+                    if (one) {
+                        const uint64_t at = (uint64_t)(s * (ST_BYTES >> 4));
+                        const uint64_t da = da0 + at, db = db0 + at;
 #pragma unroll
-                    for (int k = 0; k < BK / 16; k++)
-                        umma_bf16<CG>(d, da0 + at + k * ka, db0 + at + k * kb, id, (v | k) ? 1u : 0u);
-                    umma_commit<CG>(b_empty + s * 8);
+                        for (int k = 0; k < BK / 16; k++)
+                            umma_bf16<CG>(d, da + k * ka, db + k * kb, id, (v | k) ? 1u : 0u);
+                        umma_commit<CG>(b_empty + s * 8);
+                    }
                     if (++s == ST) s = 0, par ^= 1;
                 }
-                if (ok) umma_commit<CG>(b_accf + buf * 8);
+                if (ok && one) umma_commit<CG>(b_accf + buf * 8);
             }
         }
-        if (!ok) {  // products in flight end before tensor memory is freed
+        if (!ok && one) {  // products in flight end before tensor memory is freed
             umma_commit<CG>(su32(drain));
             for (uint32_t w = 0; w < (1u << 14) && !mbar_try(su32(drain), 0); w++) __nanosleep(100);
         }
@@ -624,7 +656,7 @@ k_xgemm(const __grid_constant__ Work W) {
                 for (int e = 0; e < HALF; e++) acc[e] = 0.0f;
                 for (int f = 0; f < KB; f++, ph++) {
                     const uint32_t buf = ph & 1;
-                    ok = __all_sync(0xffffffffu, mbar_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err));
+                    ok = warp_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err);
                     if (!ok) break;
                     TC_AFTER();
 #pragma unroll
@@ -651,7 +683,7 @@ k_xgemm(const __grid_constant__ Work W) {
             } else {
                 const uint32_t buf = ph & 1;
                 Row r(g, row, n0);
-                ok = __all_sync(0xffffffffu, mbar_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err));
+                ok = warp_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err);
                 if (!ok) break;
                 ph++;
                 TC_AFTER();
@@ -686,66 +718,120 @@ k_xgemm(const __grid_constant__ Work W) {
 
 // ---- small kernels -----------------------------------------------------------------
 
-// Rows of src [rows][dim] as bf16 planes [planes][rows][ld] (1 plane: copied,
-// 3: split3); with labels, a row without a target becomes zeros, so that what
-// its x holds (NaN, infinities) never meets the zeros of its G row.
+// Rows of src [rows][dim] as bf16 planes [planes][rows][ld], ld = dim rounded
+// up to 64: a warp per row, a lane 8 consecutive values at a time (the columns
+// from dim on are written as zeros).  1 plane: rounded to bf16; 3: split3.
+// With scale, row i becomes (scale_i / *unit) x_i in f32 first, and a row without
+// a target becomes zeros, so that what its x holds (NaN, infinities) never meets
+// the zeros of its G row.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
 k_pack(bf16* __restrict__ dst, const T* __restrict__ src, long long rows, int dim, int ld,
-       const void* labels, int index_bytes, long long vocab) {
-    const long long total = rows * ld, plane = rows * ld;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / ld;
-        const int c = (int)(i - r * ld);
-        bool live = c < dim;
-        if (labels) {
+       int vec, const float* __restrict__ scale, const float* __restrict__ unit, const void* labels,
+       int index_bytes, long long vocab) {
+    const long long plane = rows * ld;
+    const int lane = threadIdx.x & 31;
+    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
+         r += (long long)gridDim.x * 8) {
+        float f = 1.0f;
+        bool has = true;
+        if (scale) {
             const long long l = label_at(labels, index_bytes, r);
-            live = live && l >= 0 && l < vocab;
+            has = l >= 0 && l < vocab;
+            f = __fdiv_rn(scale[r], *unit);
         }
-        if constexpr (PLANES == 1) {
-            dst[i] = live ? (bf16)src[r * dim + c] : __float2bfloat16_rn(0.0f);
-        } else {
-            bf16 b0, b1, b2;
-            split3(live ? (float)src[r * dim + c] : 0.0f, b0, b1, b2);
-            dst[i] = b0;
-            dst[plane + i] = b1;
-            dst[2 * plane + i] = b2;
+        const T* sr = src + r * dim;
+        bf16* dr = dst + r * ld;
+        for (int c = lane * 8; c < ld; c += 256) {
+            alignas(16) T in[8];
+            if (vec && c + 8 <= dim) {
+#pragma unroll
+                for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++)
+                    reinterpret_cast<uint4*>(in)[q] = reinterpret_cast<const uint4*>(sr + c)[q];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) in[e] = c + e < dim ? sr[c + e] : T(0.0f);
+            }
+            alignas(16) bf16 o[PLANES][8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float v = (float)in[e];
+                if (scale) v = has ? v * f : 0.0f;
+                if constexpr (PLANES == 1) o[0][e] = __float2bfloat16_rn(v);
+                else split3(v, o[0][e], o[1][e], o[2][e]);
+            }
+#pragma unroll
+            for (int k = 0; k < PLANES; k++)
+                *reinterpret_cast<uint4*>(dr + k * plane + c) = *reinterpret_cast<uint4*>(o[k]);
         }
     }
 }
 
-// lse and loss of every row from its tiles' maxima and sums: 8 strided
-// groups of tiles per row joined in a fixed order.
-__global__ void __launch_bounds__(256)
+// The largest |dloss| of the rows with a target, 1 where there is none that is
+// positive and finite: the unit that dloss x is taken in, so that the equal
+// dloss of a mean leaves x as it is, with no rounding.
+__global__ void __launch_bounds__(1024)
+k_xent_unit(float* __restrict__ unit, const float* __restrict__ dloss, const void* labels,
+            int index_bytes, long long vocab, long long n) {
+    __shared__ float s[32];
+    float m = 0.0f;
+    for (long long i = threadIdx.x; i < n; i += 1024) {
+        const long long l = label_at(labels, index_bytes, i);
+        if (l >= 0 && l < vocab) m = fmaxf(m, fabsf(dloss[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = s[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (threadIdx.x == 0) *unit = m > 0.0f && m < INFINITY ? m : 1.0f;
+    }
+}
+
+// lse and loss of every row from its segments' maxima and sums: 32 rows a
+// CTA, the segments in 32 strided groups per row, each group's maximum first
+// and then its sum against it (independent loads, no chain of exponentials),
+// the groups joined in a fixed order.
+__global__ void __launch_bounds__(1024)
 k_xent_join(float* __restrict__ loss, float* __restrict__ lse, const float* __restrict__ part_m,
             const float* __restrict__ part_s, const float* __restrict__ zlabel,
-            const void* labels, int index_bytes, long long vocab, long long n, int tiles) {
-    __shared__ float sm[8][33], ss[8][33];
-    const long long row = (long long)blockIdx.x * 32 + threadIdx.x;
+            const void* labels, int index_bytes, long long vocab, long long n, int segs) {
+    __shared__ float sm[32][33], ss[32][33];
+    const int tx = threadIdx.x, ty = threadIdx.y;
+    const long long row = (long long)blockIdx.x * 32 + tx;
     float m = -INFINITY, s = 0.0f;
-    auto join = [&](float om, float os) {
-        if (om > m) {
-            s = s * expf(m - om) + os;
-            m = om;
-        } else {
-            s += om == -INFINITY ? os : os * expf(om - m);
+    if (row < n) {
+#pragma unroll 4
+        for (int t = ty; t < segs; t += 32) m = fmaxf(m, part_m[(size_t)t * n + row]);
+        // while every segment's maximum is -inf, its sum is 0 or NaN: added as it is
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+        for (int t = ty; t < segs; t += 32) {
+            const float om = part_m[(size_t)t * n + row], os = part_s[(size_t)t * n + row];
+            s += om == -INFINITY ? os : os * ex2((om - ref) * kLog2e);
         }
-    };
-    if (row < n)
-        for (int t = threadIdx.y; t < tiles; t += 8)
-            join(part_m[(size_t)t * n + row], part_s[(size_t)t * n + row]);
-    sm[threadIdx.y][threadIdx.x] = m;
-    ss[threadIdx.y][threadIdx.x] = s;
+    }
+    sm[ty][tx] = m;
+    ss[ty][tx] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && row < n) {
-        for (int k = 1; k < 8; k++) join(sm[k][threadIdx.x], ss[k][threadIdx.x]);
+    // warp ty joins row ty of the CTA: lane k takes group k
+    const long long my = (long long)blockIdx.x * 32 + ty;
+    float gm = sm[tx][ty], gs = ss[tx][ty], top = gm;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    gs = gm == -INFINITY ? gs : gs * expf(gm - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) gs += __shfl_xor_sync(0xffffffffu, gs, o);
+    if (tx == 0 && my < n) {
         // no finite maximum (a row of -inf or NaN): log 0 would say -inf
-        const float ls = logf(s);
-        lse[row] = m == -INFINITY ? NAN : m + ls;
-        const long long l = label_at(labels, index_bytes, row);
-        // (m - z_label) + log s keeps small losses exact where lse - z_label cancels
-        loss[row] = l >= 0 && l < vocab ? (m == -INFINITY ? NAN : (m - zlabel[row]) + ls) : 0.0f;
+        const float ls = top == -INFINITY ? NAN : logf(gs);
+        lse[my] = top + ls;
+        const long long l = label_at(labels, index_bytes, my);
+        // (top - z_label) + log s keeps small losses exact where lse - z_label cancels
+        loss[my] = l >= 0 && l < vocab ? (top - zlabel[my]) + ls : 0.0f;
     }
 }
 
@@ -837,13 +923,13 @@ size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 // How a call uses its workspace.  The vocabulary is cut into pieces of vp
 // classes (a multiple of the widest tile) so that a piece's G, and its packed
 // w where w cannot be read in place, stay within a fixed budget.  The gradient
-// holds two pieces: a launch makes G of one while it multiplies the other.
+// holds two pieces: a launch makes P of one while it multiplies the other.
 struct Plan {
     int planes, cg;
     size_t dp;                // packed row length
     size_t vp, pieces;
     size_t seg;               // classes of one (maximum, sum) entry
-    size_t xp, wp[2], g[2], ldg, acc, pm, ps, zl, total;  // byte offsets; ldg in elements
+    size_t xp, sp, unit, wp[2], g[2], ldg, acc, pm, ps, zl, total;  // byte offsets; ldg in elements
 };
 
 constexpr size_t kPieceBytes = (size_t)128 << 20;
@@ -854,7 +940,9 @@ Plan make_plan(const XentP& p, bool grad) {
     q.planes = p.dt == F32 ? 3 : 1;
     q.cg = p.n > BT && p.vocab > BT ? 2 : 1;
     q.seg = (size_t)BT * q.cg / 2;
-    q.dp = up(p.dim, 8);
+    // whole 128-byte lines: a box row that straddles two costs two requests
+    // (2048 x 8192 x 1000 f32: 750 instead of 510 cycles per stage)
+    q.dp = up(p.dim, 64);
     const size_t per_class = (size_t)q.planes * 2 * (q.dp + (grad ? (size_t)p.n : 0));
     size_t vp = std::max<size_t>(kPieceBytes / per_class / kTile * kTile, 4 * kTile);
     const size_t all = up(p.vocab, kTile);
@@ -873,6 +961,8 @@ Plan make_plan(const XentP& p, bool grad) {
     for (int b = 0; b < 2; b++)
         q.wp[b] = b < (grad ? (int)q.pieces : 1) ? take((size_t)q.planes * 2 * q.vp * q.dp) : q.wp[0];
     if (grad) {
+        q.sp = take((size_t)q.planes * 2 * p.n * q.dp);
+        q.unit = take(4);
         for (int b = 0; b < 2; b++)
             q.g[b] = b < (int)q.pieces ? take((size_t)q.planes * 2 * p.n * q.ldg) : q.g[0];
         q.acc = take(p.dt == BF16 && q.pieces > 1 ? (size_t)4 * p.n * p.dim : 0);
@@ -886,19 +976,23 @@ Plan make_plan(const XentP& p, bool grad) {
     return q;
 }
 
-void pack(Ctx& c, const XentP& p, bf16* dst, const void* src, size_t rows, int ld, bool masked) {
-    const unsigned grid = grid_for(c, rows * ld, 256, 16);
-    const void* lab = masked ? p.labels : nullptr;
+// scale: the factors of the rows (dloss), in units of *unit; or null.
+void pack(Ctx& c, const XentP& p, bf16* dst, const void* src, size_t rows, int ld,
+          const void* scale, const float* unit) {
+    const unsigned grid = grid_for(c, rows, 8, 8);
+    const bool vec = ((uintptr_t)src & 15) == 0 && p.dim * dtype_bytes(p.dt) % 16 == 0;
     if (p.dt == F32)
-        k_pack<float, 3><<<grid, 256, 0, c.stream>>>(dst, (const float*)src, rows, p.dim, ld, lab,
+        k_pack<float, 3><<<grid, 256, 0, c.stream>>>(dst, (const float*)src, rows, p.dim, ld, vec,
+                                                     (const float*)scale, unit, p.labels,
                                                      p.index_bytes, p.vocab);
     else
-        k_pack<bf16, 1><<<grid, 256, 0, c.stream>>>(dst, (const bf16*)src, rows, p.dim, ld, lab,
+        k_pack<bf16, 1><<<grid, 256, 0, c.stream>>>(dst, (const bf16*)src, rows, p.dim, ld, vec,
+                                                    (const float*)scale, unit, p.labels,
                                                     p.index_bytes, p.vocab);
     count_launch();
 }
 
-// w can feed TMA where it lies when its rows start on 16-byte boundaries.
+// A tensor can feed TMA where it lies when its rows start on 16-byte boundaries.
 bool in_place(const XentP& p, const void* t) {
     return p.dt == BF16 && p.dim % 8 == 0 && ((uintptr_t)t & 15) == 0;
 }
@@ -928,11 +1022,12 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     const bf16* xp = (const bf16*)p.x;
     if (!xip) {
         xp = (bf16*)(base + q.xp);
-        pack(c, p, (bf16*)xp, p.x, p.n, (int)q.dp, false);
+        pack(c, p, (bf16*)xp, p.x, p.n, (int)q.dp, nullptr, nullptr);
     }
     CUtensorMap ma, mb;
     int rc;
-    if ((rc = make_map(&ma, xp, p.dim, p.n, q.dp, q.planes, (size_t)p.n * q.dp, BT))) return rc;
+    const size_t ldx = xip ? p.dim : q.dp, ldw = wip ? p.dim : q.dp;
+    if ((rc = make_map(&ma, xp, p.dim, p.n, ldx, q.planes, p.n * ldx, BT))) return rc;
     Job g{};
     g.kind = LSE;
     g.M = (int)p.n;
@@ -948,9 +1043,9 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
         if (!wip) {
             wp = (bf16*)(base + q.wp[0]);
             pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * dtype_bytes(p.dt), nv, (int)q.dp,
-                 false);
+                 nullptr, nullptr);
         }
-        if ((rc = make_map(&mb, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BT))) return rc;
+        if ((rc = make_map(&mb, wp, p.dim, nv, ldw, q.planes, nv * ldw, BT))) return rc;
         g.N = (int)nv;
         g.col0 = (long long)v0;
         g.part_m = (float*)(base + q.pm) + v0 / q.seg * p.n;
@@ -959,7 +1054,7 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
         add_job(w, g, ma, mb, q.cg);
         if ((rc = run_work(c, w, q.cg, q.planes == 3))) return rc;
     }
-    k_xent_join<<<(p.n + 31) / 32, dim3(32, 8), 0, c.stream>>>(
+    k_xent_join<<<(p.n + 31) / 32, dim3(32, 32), 0, c.stream>>>(
         (float*)loss, (float*)lse, (const float*)(base + q.pm), (const float*)(base + q.ps),
         (const float*)(base + q.zl), p.labels, p.index_bytes, p.vocab, p.n,
         (int)((p.vocab + q.seg - 1) / q.seg));
@@ -978,14 +1073,25 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), six = q.planes == 3;
     const size_t es = dtype_bytes(p.dt);
-    bf16* xp = (bf16*)(base + q.xp);
-    pack(c, p, xp, p.x, p.n, (int)q.dp, true);
-    const size_t xplane = (size_t)p.n * q.dp, gplane = (size_t)p.n * q.ldg;
+    const bool xip = in_place(p, p.x);
+    const size_t ldx = xip ? p.dim : q.dp, ldw = wip ? p.dim : q.dp;
+    const bf16* xp = (const bf16*)p.x;
+    if (!xip) {
+        xp = (bf16*)(base + q.xp);
+        pack(c, p, (bf16*)xp, p.x, p.n, (int)q.dp, nullptr, nullptr);
+    }
+    bf16* sp = (bf16*)(base + q.sp);  // dloss x / unit
+    float* unit = (float*)(base + q.unit);
+    k_xent_unit<<<1, 1024, 0, c.stream>>>(unit, (const float*)dloss, p.labels, p.index_bytes,
+                                          p.vocab, p.n);
+    count_launch();
+    pack(c, p, sp, p.x, p.n, (int)q.dp, dloss, unit);
+    const size_t gplane = (size_t)p.n * q.ldg;
     CUtensorMap mxk, mxn, mwk, mwn, mgk, mgm;
     int rc;
-    // x: K-major A of z = x w^T, and N-major B of dw = G^T x
-    if ((rc = make_map(&mxk, xp, p.dim, p.n, q.dp, q.planes, xplane, BT))) return rc;
-    if ((rc = make_map(&mxn, xp, p.dim, p.n, q.dp, q.planes, xplane, BK))) return rc;
+    // x: K-major A of z = x w^T; dloss x: N-major B of dw = G^T (dloss x)
+    if ((rc = make_map(&mxk, xp, p.dim, p.n, ldx, q.planes, p.n * ldx, BT))) return rc;
+    if ((rc = make_map(&mxn, sp, p.dim, p.n, q.dp, q.planes, p.n * q.dp, BK))) return rc;
     Job z{};
     z.kind = GRAD;
     z.M = (int)p.n;
@@ -994,7 +1100,6 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
     z.index_bytes = p.index_bytes;
     z.vocab = p.vocab;
     z.lse = (const float*)lse;
-    z.dloss = (const float*)dloss;
     z.ldg = (long long)q.ldg;
     z.gplane = six ? (long long)gplane : 0;
     // launch i: G of piece i, and the products of piece i - 1
@@ -1005,7 +1110,7 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             const bool first = i == 1, last = i == q.pieces;
             const bf16* gp = (const bf16*)(base + q.g[(i - 1) & 1]);
             const bf16* wp = wip ? (const bf16*)p.w + v0 * p.dim : (bf16*)(base + q.wp[(i - 1) & 1]);
-            if ((rc = make_map(&mwn, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BK))) return rc;
+            if ((rc = make_map(&mwn, wp, p.dim, nv, ldw, q.planes, nv * ldw, BK))) return rc;
             if ((rc = make_map(&mgk, gp, nv, p.n, q.ldg, q.planes, gplane, BT))) return rc;
             if ((rc = make_map(&mgm, gp, nv, p.n, q.ldg, q.planes, gplane, BK))) return rc;
             Job o{};
@@ -1013,14 +1118,21 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             o.ldo = p.dim;
             o.N = (int)p.dim;
             o.b_mn = 1;
-            // dx += G w: K runs over the piece's classes; the sum so far is f32
+            // dx = dloss (sum of the pieces' G w): K runs over the piece's classes;
+            // the sum so far is f32
             o.M = (int)p.n;
             o.K = (int)nv;
             o.out_bf16 = !six && last;
             o.out = six || last ? dx : base + q.acc;
             o.acc_in = first ? nullptr : six ? (const float*)dx : (const float*)(base + q.acc);
+            o.dloss = last ? (const float*)dloss : nullptr;
+            o.labels = p.labels;
+            o.index_bytes = p.index_bytes;
+            o.vocab = p.vocab;
             add_job(w, o, mgk, mwn, q.cg);
-            // dw = G^T x: K runs over the tokens
+            o.dloss = nullptr;
+            o.factor = unit;
+            // dw = unit P^T (dloss x / unit): K runs over the tokens
             o.M = (int)nv;
             o.K = (int)p.n;
             o.a_mn = 1;
@@ -1034,9 +1146,9 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             const bf16* wp = (const bf16*)p.w + (wip ? v0 * p.dim : 0);
             if (!wip) {
                 wp = (bf16*)(base + q.wp[i & 1]);
-                pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * es, nv, (int)q.dp, false);
+                pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * es, nv, (int)q.dp, nullptr, nullptr);
             }
-            if ((rc = make_map(&mwk, wp, p.dim, nv, q.dp, q.planes, nv * q.dp, BT))) return rc;
+            if ((rc = make_map(&mwk, wp, p.dim, nv, ldw, q.planes, nv * ldw, BT))) return rc;
             z.N = (int)nv;
             z.col0 = (long long)v0;
             z.g = (bf16*)(base + q.g[i & 1]);

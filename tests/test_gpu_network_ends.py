@@ -466,7 +466,8 @@ def xgrad_check(torch, name, dl, x, w, labels, lse, dx, dw):
     within(torch, dx, want, H[name] * want.abs() + eg @ W.abs()
            + (six * (v / 16 + 1) + 8 + v / 1024) * 2.0 ** -23 * (gm @ W.abs()))
     want = g.t() @ X
-    within(torch, dw, want, H[name] * want.abs() + eg.t() @ X.abs()
+    # dloss x is rounded too, to the type of the products: one more half step of each term
+    within(torch, dw, want, H[name] * want.abs() + (eg + hg * gm).t() @ X.abs()
            + (six * (n / 16 + 1) + 8) * 2.0 ** -23 * (gm.t() @ X.abs()))
 
 
