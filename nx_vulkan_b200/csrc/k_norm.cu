@@ -13,15 +13,30 @@
 // from the centred values (two passes over registers, not E[x^2] - mean^2,
 // which cancels for rows with a large mean).
 //
-// Both directions are bound by memory: a row is read once, stays in the
-// registers of its CTA (or warp) and is written once.  A thread holds NV
-// pieces of VEC consecutive elements (16 bytes when every row starts on a
-// 16-byte boundary, else single elements); rows longer than the largest CTA
-// holds go through a looping variant that reads the row again from L2.
+// Both directions are bound by memory: a row is read once, stays in registers
+// and is written once.  What counts is how many bytes are in flight: forward a
+// warp loads a whole row of up to 8 KB before it waits for any of it, and 20 warps
+// an SM do so; backward, where the column sums take the registers, one CTA an SM
+// holds some rows while the next ones are on their way to L2.  Pairs of f32 values go
+// through the packed two-f32 instructions.
+// Measured: [32768, 4096] bf16 forward 89 us (6.0 TB/s; one row per 128 threads
+// of 4 pieces each 105, with barriers between few warps 120 to 160), [16384, 8192]
+// bf16 backward 168 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
+//
+// Pieces are 16 bytes.  In a row that does not start on a 16-byte boundary
+// thread i still holds columns [i V, (i + 1) V), V = 16 / element size: it reads
+// the two aligned pieces that hold them and shifts.  For a store a lane joins its
+// neighbour's last bytes with its own first ones into an aligned piece; what is
+// left at the ends of a warp's stretch and of the row is stored element by element.
+// An aligned piece at a row's end holds bytes of the next row, which are ignored; the
+// tensor's first and last row are read element by element, so that nothing outside
+// the tensor is touched.
 #include "kernels.h"
 #include "ops_common.cuh"
 
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 namespace nxv {
 
@@ -40,11 +55,233 @@ __device__ __forceinline__ void from_acc(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_acc(double& d, double v) { d = v; }
 __device__ __forceinline__ void from_acc(bf16& d, float v) { d = __float2bfloat16_rn(v); }
 
-// VEC consecutive elements, as one load or store.
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-    T e[VEC];
+// V consecutive columns of a row, as they lie in memory.
+template <typename T> constexpr int kV = 16 / sizeof(T);
+template <typename T>
+union Piece {
+    uint32_t w[4];
+    T e[kV<T>];
+    __device__ Piece() {}
 };
+
+// w[k] = the four bytes from byte 4 k + o of the 32 bytes a || b, 0 <= o < 16.
+// w may be a or b.
+__device__ __forceinline__ void shift_bytes(uint32_t (&w)[4], const uint32_t (&a)[4],
+                                            const uint32_t (&b)[4], unsigned o) {
+    uint32_t c[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    if (o & 8) {
+#pragma unroll
+        for (int k = 0; k < 6; k++) c[k] = c[k + 2];
+    }
+    if (o & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; k++) c[k] = c[k + 1];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(c[k], c[k + 1], (o & 3) * 8);
+}
+
+__device__ __forceinline__ void load16(uint32_t (&w)[4], const void* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+}
+
+// Two f32 values (or one f64) that one instruction works on.
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ unsigned long long bits(F2 a) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ F2 from_bits(unsigned long long r) {
+    F2 a;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+    return a;
+}
+__device__ __forceinline__ F2 vfma(F2 a, F2 b, F2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return from_bits(r);
+}
+__device__ __forceinline__ F2 vadd(F2 a, F2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return from_bits(r);
+}
+__device__ __forceinline__ F2 vmul(F2 a, F2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return from_bits(r);
+}
+__device__ __forceinline__ double vfma(double a, double b, double c) { return __fma_rn(a, b, c); }
+__device__ __forceinline__ double vadd(double a, double b) { return __dadd_rn(a, b); }
+__device__ __forceinline__ double vmul(double a, double b) { return __dmul_rn(a, b); }
+__device__ __forceinline__ F2 vset(float v, F2*) { return F2{v, v}; }
+__device__ __forceinline__ double vset(double v, double*) { return v; }
+__device__ __forceinline__ float vsum(F2 a) { return a.x + a.y; }
+__device__ __forceinline__ double vsum(double a) { return a; }
+
+template <typename T> struct Vec { using type = F2; };
+template <> struct Vec<double> { using type = double; };
+template <typename T> using vec_t = typename Vec<T>::type;
+template <typename T> constexpr int kN = sizeof(vec_t<T>) / sizeof(acc_t<T>);  // values of a vec
+template <typename T> constexpr int kP = kV<T> / kN<T>;                       // vecs of a piece
+
+__device__ __forceinline__ void unpack(F2 (&v)[4], const Piece<bf16>& p) {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        v[k] = F2{__uint_as_float(p.w[k] << 16), __uint_as_float(p.w[k] & 0xffff0000u)};
+}
+__device__ __forceinline__ void unpack(F2 (&v)[2], const Piece<float>& p) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) v[k] = F2{p.e[2 * k], p.e[2 * k + 1]};
+}
+__device__ __forceinline__ void unpack(double (&v)[2], const Piece<double>& p) {
+    v[0] = p.e[0], v[1] = p.e[1];
+}
+__device__ __forceinline__ void pack(Piece<bf16>& p, const F2 (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[k].x, v[k].y);
+        p.w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+__device__ __forceinline__ void pack(Piece<float>& p, const F2 (&v)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) p.e[2 * k] = v[k].x, p.e[2 * k + 1] = v[k].y;
+}
+__device__ __forceinline__ void pack(Piece<double>& p, const double (&v)[2]) {
+    p.e[0] = v[0], p.e[1] = v[1];
+}
+// Makes the compiler unpack p again at its next use instead of keeping the
+// wider values in registers.
+template <typename T>
+__device__ __forceinline__ void keep_packed(Piece<T>& p) {
+    asm volatile("" : "+r"(p.w[0]), "+r"(p.w[1]), "+r"(p.w[2]), "+r"(p.w[3]));
+}
+// v's values from element n on as zeros.
+__device__ __forceinline__ void keep_first(F2& v, int n) {
+    if (n < 2) v.y = 0.0f;
+    if (n < 1) v.x = 0.0f;
+}
+__device__ __forceinline__ void keep_first(double& v, int n) {
+    if (n < 1) v = 0.0;
+}
+
+// Piece i of the row of `cols` elements at p, zeros past the row.  edge: the
+// tensor's first or last row, or one that stands alone.  AL: every row starts on
+// a 16-byte boundary and is whole pieces long.
+template <typename T, bool AL>
+__device__ __forceinline__ void row_load(Piece<T>& v, const T* p, unsigned i, unsigned cols, bool edge) {
+    constexpr unsigned V = kV<T>;
+    if constexpr (AL) {
+        if (i * V < cols) load16(v.w, p + (size_t)i * V);
+        else v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
+    } else {
+        const unsigned s = (unsigned)((uintptr_t)p & 15);
+        if (s != 0 && !edge) {
+            const unsigned end = s + cols * (unsigned)sizeof(T);
+            const char* base = (const char*)p - s + 16 * (size_t)i;
+            uint32_t a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
+            if (16 * i < end) load16(a, base);
+            if (16 * i + 16 < end) load16(b, base + 16);
+            shift_bytes(v.w, a, b, s);
+            if (i * V + V > cols) {
+#pragma unroll
+                for (unsigned e = 0; e < V; e++)
+                    if (i * V + e >= cols) v.e[e] = T(0.0f);
+            }
+        } else if (s == 0 && i * V + V <= cols) {
+            load16(v.w, p + (size_t)i * V);
+        } else {
+#pragma unroll
+            for (unsigned e = 0; e < V; e++) v.e[e] = i * V + e < cols ? p[i * V + e] : T(0.0f);
+        }
+    }
+}
+
+// The same in two steps, for loads that are to be in flight for long: the piece
+// as the aligned pieces lie in memory (the first of its two), and, at its use, the
+// rest from the next lane (the last of the `width` lanes that hold the row's
+// consecutive pieces loads it).  Whole warps.
+template <typename T, bool AL>
+__device__ __forceinline__ void raw_load(Piece<T>& v, const T* p, unsigned i, unsigned cols, bool edge) {
+    const unsigned s = AL ? 0 : (unsigned)((uintptr_t)p & 15);
+    if (s == 0 || edge) {
+        row_load<T, AL>(v, p, i, cols, edge);
+    } else {
+        v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
+        if (16 * i < s + cols * (unsigned)sizeof(T)) load16(v.w, (const char*)p - s + 16 * (size_t)i);
+    }
+}
+template <typename T, bool AL>
+__device__ __forceinline__ void realign(Piece<T>& v, const T* p, unsigned i, unsigned cols, bool edge,
+                                        unsigned lane, unsigned width) {
+    constexpr unsigned V = kV<T>;
+    if constexpr (!AL) {
+        const unsigned s = edge ? 0 : (unsigned)((uintptr_t)p & 15);
+        uint32_t next[4], far[4] = {0, 0, 0, 0};
+        const bool last = lane + 1 == width;
+        if (last && s != 0 && 16 * i + 16 < s + cols * (unsigned)sizeof(T))
+            load16(far, (const char*)p - s + 16 * (size_t)i + 16);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            next[w] = __shfl_down_sync(0xffffffffu, v.w[w], 1);
+            if (last) next[w] = far[w];
+        }
+        if (s == 0) return;
+        shift_bytes(v.w, v.w, next, s);
+        if (i * V + V > cols) {
+#pragma unroll
+            for (unsigned e = 0; e < V; e++)
+                if (i * V + e >= cols) v.e[e] = T(0.0f);
+        }
+    }
+}
+
+// Stores piece i of the row at p; lane: the thread's place among the `width`
+// (at most 32) lanes of its warp that hold the row's consecutive pieces; live:
+// it has a row.  Whole warps.
+template <typename T, bool AL>
+__device__ __forceinline__ void row_store(T* p, const Piece<T>& v, unsigned i, unsigned cols,
+                                          unsigned lane, unsigned width, bool live) {
+    constexpr unsigned V = kV<T>;
+    if constexpr (AL) {
+        if (live && i * V < cols)
+            reinterpret_cast<uint4*>(p)[i] = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    } else {
+        const unsigned s = (unsigned)((uintptr_t)p & 15), bytes = cols * (unsigned)sizeof(T);
+        char* base = (char*)p - s;
+        uint32_t prev[4], out[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) prev[k] = __shfl_up_sync(0xffffffffu, v.w[k], 1);
+        if (!live || i * V >= cols) return;
+        if (s == 0) {
+            if (16 * i + 16 <= bytes) {
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+            } else {
+#pragma unroll
+                for (unsigned e = 0; e < V; e++)
+                    if (i * V + e < cols) p[i * V + e] = v.e[e];
+            }
+            return;
+        }
+        shift_bytes(out, prev, v.w, 16 - s);
+        // aligned piece i (the end of piece i - 1, the start of piece i): whole within the row
+        const bool mine = lane > 0 && 16 * i + 16 <= s + bytes;
+        const bool next = lane + 1 < width && 16 * i + 32 <= s + bytes;  // piece i + 1's lane will
+        if (mine) reinterpret_cast<uint4*>(base)[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        if (!mine || !next) {
+#pragma unroll
+            for (unsigned e = 0; e < V; e++) {
+                const bool head = e * sizeof(T) + s < 16;
+                if (i * V + e < cols && (head ? !mine : !next)) p[i * V + e] = v.e[e];
+            }
+        }
+    }
+}
 
 template <typename A>
 __device__ __forceinline__ A warp_sum(A v) {
@@ -53,337 +290,573 @@ __device__ __forceinline__ A warp_sum(A v) {
     return v;
 }
 
-// The sum of v over the threads of one row (blockDim.x of them), in a fixed
-// order, to every thread.  red: 2 x 32 values per row of the block, used in
-// turn so that one barrier per sum is enough.
-template <typename A, int K>
-__device__ __forceinline__ void row_sum(A (&v)[K], A* red, int& turn) {
-#pragma unroll
-    for (int k = 0; k < K; k++) v[k] = warp_sum(v[k]);
-    const int nw = blockDim.x >> 5;
-    if (nw == 1) return;
-    A* buf = red + (turn & 1) * (32 * K);
-    turn++;
-    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-    if (l == 0) {
-#pragma unroll
-        for (int k = 0; k < K; k++) buf[k * 32 + w] = v[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; k++) v[k] = warp_sum(l < nw ? buf[k * 32 + l] : A(0));
-}
-
 template <typename A>
 __device__ __forceinline__ A rsqrt_exact(A v) {
     return div_(A(1), sqrt_(v));
 }
 
-// One row per blockDim.x threads (blockDim.y rows per block; blockDim.y > 1
-// only with one warp per row).  NV = 0: the looping variant.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(1024)
-k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd,
-           const T* x, const T* __restrict__ gamma, const T* __restrict__ beta, unsigned rows,
-           unsigned cols, acc_t<T> eps) {
+// Forward: a row in the registers of a group of G = 32, 64, .. threads (blockDim.x),
+// blockDim.y rows a CTA (more than one only with one warp a row, where there
+// is no barrier).  Up to 16 pieces a thread are loaded before anything waits for
+// them: with 20 warps an SM, 160 KB in flight.
+template <typename T, int NV, bool AL>
+__global__ void __launch_bounds__(NV > 8 ? 512 : 1024)
+k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const T* x,
+           const T* __restrict__ gamma, const T* __restrict__ beta, unsigned rows, unsigned cols,
+           acc_t<T> eps) {
     using A = acc_t<T>;
-    using P = Pack<T, VEC>;
-    __shared__ A red[64];
-    int turn = 0;
+    using W = vec_t<T>;
+    constexpr int V = kV<T>, N = kN<T>, NP = kP<T>;
+    __shared__ A red[2][32];
+    const unsigned t = threadIdx.x, G = blockDim.x, lane = t & 31, warps = G >> 5;
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= rows) return;  // whole warps: blockDim.y > 1 has no barriers
-    const P* xr = reinterpret_cast<const P*>(x + row * cols);
-    P* yr = reinterpret_cast<P*>(y + row * cols);
-    const P* gp = reinterpret_cast<const P*>(gamma);
-    const P* bp = reinterpret_cast<const P*>(beta);
-    const unsigned nv = cols / VEC;  // exact: VEC > 1 only for cols % VEC == 0
-    const A inv = A(1) / A(cols);
-    if constexpr (NV > 0) {
-        P r[NV];
-        A s[1] = {A(0)};
+    const T* xr = x + row * cols;
+    Piece<T> p[NV];
+    const bool edge = row == 0 || row + 1 == rows;
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const unsigned i = threadIdx.x + k * blockDim.x;
-            if (i < nv) r[k] = xr[i];
-        }
+    for (int k = 0; k < NV; k++) raw_load<T, AL>(p[k], xr, t + k * G, cols, edge);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            if (threadIdx.x + k * blockDim.x < nv) {
+    for (int k = 0; k < NV; k++) realign<T, AL>(p[k], xr, t + k * G, cols, edge, lane, 32);
+    auto total = [&](A v, int which) {
+        v = warp_sum(v);
+        if (warps == 1) return v;
+        if (lane == 0) red[which][t >> 5] = v;
+        __syncthreads();
+        return warp_sum(lane < warps ? red[which][lane] : A(0));
+    };
+    W s = vset(A(0), (W*)0);
 #pragma unroll
-                for (int e = 0; e < VEC; e++) s[0] += to_acc(r[k].e[e]);
+    for (int k = 0; k < NV; k++) {
+        W v[NP];
+        unpack(v, p[k]);
+#pragma unroll
+        for (int e = 0; e < NP; e++) s = vadd(s, v[e]);  // zeros past the row
+    }
+    const A m = div_(total(vsum(s), 0), A(cols));
+    const W mm = vset(-m, (W*)0);
+    s = vset(A(0), (W*)0);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const unsigned at = (t + k * G) * V;
+        if (at < cols) {
+            W v[NP];
+            keep_packed(p[k]);
+            unpack(v, p[k]);
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                W c = vadd(v[e], mm);
+                if (!AL && at + V > cols) keep_first(c, (int)(cols - at) - e * N);
+                s = vfma(c, c, s);
             }
         }
-        row_sum<A, 1>(s, red, turn);
-        const A m = s[0] * inv;
-        s[0] = A(0);
+    }
+    const A rs = rsqrt_exact(div_(total(vsum(s), 1), A(cols)) + eps);
+    if (t == 0) {
+        mean[row] = m;
+        rstd[row] = rs;
+    }
+    const W rr = vset(rs, (W*)0);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            if (threadIdx.x + k * blockDim.x < nv) {
+    for (int k = 0; k < NV; k++) {
+        if (!AL || (t + k * G) * V < cols) {
+            Piece<T> g, b;
+            row_load<T, AL>(g, gamma, t + k * G, cols, true);
+            row_load<T, AL>(b, beta, t + k * G, cols, true);
+            W v[NP], gv[NP], bv[NP];
+            keep_packed(p[k]);
+            unpack(v, p[k]);
+            unpack(gv, g);
+            unpack(bv, b);
 #pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const A d = to_acc(r[k].e[e]) - m;
-                    s[0] += d * d;
-                }
-            }
-        }
-        row_sum<A, 1>(s, red, turn);
-        const A rs = rsqrt_exact(s[0] * inv + eps);
-        if (threadIdx.x == 0) {
-            mean[row] = m;
-            rstd[row] = rs;
-        }
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const unsigned i = threadIdx.x + k * blockDim.x;
-            if (i < nv) {
-                const P g = gp[i], b = bp[i];
-                P o;
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    from_acc(o.e[e], (to_acc(r[k].e[e]) - m) * rs * to_acc(g.e[e]) + to_acc(b.e[e]));
-                yr[i] = o;
-            }
-        }
-    } else {
-        A s[1] = {A(0)};
-        for (unsigned i = threadIdx.x; i < nv; i += blockDim.x) {
-            const P v = xr[i];
-#pragma unroll
-            for (int e = 0; e < VEC; e++) s[0] += to_acc(v.e[e]);
-        }
-        row_sum<A, 1>(s, red, turn);
-        const A m = s[0] * inv;
-        s[0] = A(0);
-        for (unsigned i = threadIdx.x; i < nv; i += blockDim.x) {
-            const P v = xr[i];
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const A d = to_acc(v.e[e]) - m;
-                s[0] += d * d;
-            }
-        }
-        row_sum<A, 1>(s, red, turn);
-        const A rs = rsqrt_exact(s[0] * inv + eps);
-        if (threadIdx.x == 0) {
-            mean[row] = m;
-            rstd[row] = rs;
-        }
-        for (unsigned i = threadIdx.x; i < nv; i += blockDim.x) {
-            const P v = xr[i], g = gp[i], b = bp[i];
-            P o;
-#pragma unroll
-            for (int e = 0; e < VEC; e++)
-                from_acc(o.e[e], (to_acc(v.e[e]) - m) * rs * to_acc(g.e[e]) + to_acc(b.e[e]));
-            yr[i] = o;
+            for (int e = 0; e < NP; e++) v[e] = vfma(vmul(vadd(v[e], mm), rr), gv[e], bv[e]);
+            pack(p[k], v);
+            row_store<T, AL>(y + row * cols, p[k], t + k * G, cols, lane, 32, true);
         }
     }
 }
 
-// Rows r = blockIdx.x, + gridDim.x, ...: a thread owns the same columns of
-// every row, so it adds up its columns' dy xh and dy in registers and writes
-// them once, as row blockIdx.x of the partial sums [2][gridDim.x][cols].
-// NV = 0: the looping variant, which adds into its partial row in memory.
-template <typename T, int VEC, int NV>
+// Rows that 512 threads cannot hold: three passes over the row.
+template <typename T>
 __global__ void __launch_bounds__(1024)
+k_norm_fwd_long(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const T* x,
+                const T* __restrict__ gamma, const T* __restrict__ beta, unsigned rows,
+                unsigned cols, acc_t<T> eps) {
+    using A = acc_t<T>;
+    __shared__ A red[2][32];
+    const unsigned lane = threadIdx.x & 31;
+    auto total = [&](A v, int which) {
+        v = warp_sum(v);
+        if (lane == 0) red[which][threadIdx.x >> 5] = v;
+        __syncthreads();
+        return warp_sum(red[which][lane]);
+    };
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * cols;
+        T* yr = y + row * cols;
+        A s = A(0);
+        for (unsigned i = threadIdx.x; i < cols; i += 1024) s += to_acc(xr[i]);
+        const A m = div_(total(s, 0), A(cols));
+        s = A(0);
+        for (unsigned i = threadIdx.x; i < cols; i += 1024) {
+            const A d = to_acc(xr[i]) - m;
+            s += d * d;
+        }
+        const A rs = rsqrt_exact(div_(total(s, 1), A(cols)) + eps);
+        if (threadIdx.x == 0) {
+            mean[row] = m;
+            rstd[row] = rs;
+        }
+        for (unsigned i = threadIdx.x; i < cols; i += 1024)
+            from_acc(yr[i], (to_acc(xr[i]) - m) * rs * to_acc(gamma[i]) + to_acc(beta[i]));
+    }
+}
+
+// Backward: how the rows are dealt out: G threads (a power of two, lg its
+// logarithm) take R rows at a time; rounds of all the CTA's groups.
+struct Deal {
+    unsigned rows, cols, G, lg, rounds;
+};
+constexpr int kBwdThreads = 512;
+
+// Brings rows [r0, r0 + n) into L2.
+template <typename T>
+__device__ __forceinline__ void prefetch_rows(const T* t, size_t r0, unsigned n, unsigned cols) {
+    const uintptr_t a = ((uintptr_t)(t + r0 * cols) + 15) & ~(uintptr_t)15;
+    const uintptr_t b = (uintptr_t)(t + (r0 + n) * cols) & ~(uintptr_t)15;
+    if (b > a)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"((uint32_t)(b - a)) : "memory");
+}
+
+// The sums of K = 2 or 4 values over the G threads of a row, in a fixed order, to
+// all of them.  Whole warps reduce by halving: the lanes part the values among
+// themselves first, 6 shuffles for 4 values instead of 20.  red: 16 warps' K
+// sums, by turns.  The whole CTA.
+template <typename A, int K>
+__device__ __forceinline__ void group_sum(A (&v)[K], unsigned G, A (*red)[16]) {
+    constexpr unsigned FULL = 0xffffffffu;
+    if (G < 32) {
+        for (unsigned o = G / 2; o > 0; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(FULL, v[k], o);
+        }
+        return;
+    }
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    A b;
+    constexpr unsigned part = K == 4 ? 8 : 16;  // lanes that end up with one value
+    if constexpr (K == 4) {
+        const bool h = lane & 16, q = lane & 8;
+        const A a0 = (h ? v[2] : v[0]) + __shfl_xor_sync(FULL, h ? v[0] : v[2], 16);
+        const A a1 = (h ? v[3] : v[1]) + __shfl_xor_sync(FULL, h ? v[1] : v[3], 16);
+        b = (q ? a1 : a0) + __shfl_xor_sync(FULL, q ? a0 : a1, 8);
+    } else {
+        const bool h = lane & 16;
+        b = (h ? v[1] : v[0]) + __shfl_xor_sync(FULL, h ? v[0] : v[1], 16);
+        b += __shfl_xor_sync(FULL, b, 8);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) b += __shfl_xor_sync(FULL, b, o);
+    if (G > 32) {
+        const unsigned nw = G >> 5, w0 = warp & ~(nw - 1), id = lane / part, j = lane % part;
+        if (j == 0) red[id][warp] = b;
+        __syncthreads();
+        b = j < nw ? red[id][w0 + j] : A(0);
+        if (part == 8 && nw == 16) b += red[id][w0 + 8 + j];
+#pragma unroll
+        for (unsigned o = part / 2; o > 0; o >>= 1) b += __shfl_xor_sync(FULL, b, o);
+    }
+#pragma unroll
+    for (int k = 0; k < K; k++) v[k] = __shfl_sync(FULL, b, k * part);
+}
+
+// Persistent; a thread holds the same columns of every row that its group takes,
+// so it adds up its columns' dy xh and dy in registers.  R rows at a time (bf16:
+// 2), while the next two rounds' come into L2.  At the end the groups' column
+// sums are added, in order, into row blockIdx.x of the partial sums
+// [2][gridDim.x][cols].  With t = x - mean, e = dy rstd:
+//   dgamma += e t,  dbeta += dy,  dx = e gamma - rstd c1 - t rstd^2 c2,
+// c1 = mean(dy gamma), c2 = mean(dy gamma t).
+template <typename T, int NV, int R, bool AL>
+__global__ void __launch_bounds__(kBwdThreads, 1)
 k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
            const T* __restrict__ gamma, const acc_t<T>* __restrict__ mean,
-           const acc_t<T>* __restrict__ rstd, unsigned rows, unsigned cols) {
+           const acc_t<T>* __restrict__ rstd, const __grid_constant__ Deal d) {
     using A = acc_t<T>;
-    using P = Pack<T, VEC>;
-    __shared__ A red[128];
-    int turn = 0;
-    const unsigned nv = cols / VEC;
+    using W = vec_t<T>;
+    constexpr int V = kV<T>, N = kN<T>, NP = kP<T>;
+    __shared__ A red[2][2 * R][16];
+    extern __shared__ __align__(16) unsigned char mem[];  // the groups' column sums
+    const unsigned tid = threadIdx.x, cols = d.cols, G = d.G;
     const A inv = A(1) / A(cols);
-    const P* gp = reinterpret_cast<const P*>(gamma);
-    A* pg = part + (size_t)blockIdx.x * cols;
-    A* pb = part + (size_t)(gridDim.x + blockIdx.x) * cols;
-    if constexpr (NV > 0) {
-        A ag[NV][VEC], ab[NV][VEC];
+    const unsigned t = tid & (G - 1), q = tid >> d.lg, groups = kBwdThreads >> d.lg;
+    const unsigned width = G < 32 ? G : 32, lane = t & (width - 1);
+    Piece<T> g[NV];
+    W ag[NV][NP], ab[NV][NP];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        row_load<T, AL>(g[k], gamma, t + k * G, cols, true);
+#pragma unroll
+        for (int e = 0; e < NP; e++) ag[k][e] = ab[k][e] = vset(A(0), (W*)0);
+    }
+    const unsigned per_round = groups * R;
+    auto prefetch = [&](unsigned u) {
+        if (u >= d.rounds) return;
+        const size_t r0 = (size_t)u * per_round;
+        const unsigned n = (unsigned)min((size_t)per_round, d.rows - r0);
+        prefetch_rows(x, r0, n, cols);
+        prefetch_rows(dy, r0, n, cols);
+    };
+    if (tid == 0) prefetch(blockIdx.x + gridDim.x);
+    for (unsigned u = blockIdx.x, turn = 0; u < d.rounds; u += gridDim.x, turn ^= 1) {
+        if (tid == 0) prefetch(u + 2 * gridDim.x);
+        // this group's rows; the last ones may lie past the tensor
+        const size_t row0 = (size_t)u * per_round + (size_t)q * R;
+        Piece<T> vx[R][NV], vd[R][NV];
+        A m[R], rs[R], sum[2 * R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const size_t row = row0 + r;
+            const bool live = row < d.rows, edge = row == 0 || row + 1 >= d.rows;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                if (live) {
+                    raw_load<T, AL>(vx[r][k], x + row * cols, t + k * G, cols, edge);
+                    raw_load<T, AL>(vd[r][k], dy + row * cols, t + k * G, cols, edge);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) vx[r][k].w[w] = vd[r][k].w[w] = 0;
+                }
+            }
+            m[r] = live ? mean[row] : A(0);
+            rs[r] = live ? rstd[row] : A(0);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const size_t row = row0 + r;
+            const bool edge = row == 0 || row + 1 >= d.rows;
+            const W mm = vset(-m[r], (W*)0), rr = vset(rs[r], (W*)0);
+            W a0 = vset(A(0), (W*)0), a1 = a0;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                realign<T, AL>(vx[r][k], x + row * cols, t + k * G, cols, edge, lane, width);
+                realign<T, AL>(vd[r][k], dy + row * cols, t + k * G, cols, edge, lane, width);
+                keep_packed(g[k]);
+                W xv[NP], dv[NP], gv[NP];
+                unpack(xv, vx[r][k]);
+                unpack(dv, vd[r][k]);
+                unpack(gv, g[k]);
+#pragma unroll
+                for (int e = 0; e < NP; e++) {
+                    // dy is zero past the row
+                    const W tt = vadd(xv[e], mm), w = vmul(dv[e], gv[e]);
+                    a0 = vadd(a0, w);
+                    a1 = vfma(w, tt, a1);
+                    ag[k][e] = vfma(vmul(dv[e], rr), tt, ag[k][e]);
+                    ab[k][e] = vadd(ab[k][e], dv[e]);
+                }
+            }
+            sum[2 * r] = vsum(a0), sum[2 * r + 1] = vsum(a1);
+        }
+        group_sum<A, 2 * R>(sum, G, red[turn]);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const size_t row = row0 + r;
+            const W mm = vset(-m[r], (W*)0), rr = vset(rs[r], (W*)0);
+            const W c1 = vset(-rs[r] * (sum[2 * r] * inv), (W*)0);
+            const W c2 = vset(-rs[r] * rs[r] * rs[r] * (sum[2 * r + 1] * inv), (W*)0);
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                W xv[NP], dv[NP], gv[NP];
+                keep_packed(vx[r][k]);
+                keep_packed(vd[r][k]);
+                keep_packed(g[k]);
+                unpack(xv, vx[r][k]);
+                unpack(dv, vd[r][k]);
+                unpack(gv, g[k]);
+#pragma unroll
+                for (int e = 0; e < NP; e++)
+                    xv[e] = vfma(vadd(xv[e], mm), c2, vfma(vmul(dv[e], rr), gv[e], c1));
+                pack(vx[r][k], xv);
+                row_store<T, AL>(dx + row * cols, vx[r][k], t + k * G, cols, lane, width, row < d.rows);
+            }
+        }
+    }
+    A* sh = reinterpret_cast<A*>(mem);
+    const unsigned pad = (NV * V) << d.lg;  // a group's columns
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        A* out = part + ((size_t)which * gridDim.x + blockIdx.x) * cols;
+        __syncthreads();
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) ag[k][e] = ab[k][e] = A(0);
-        for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-            const P* xr = reinterpret_cast<const P*>(x + row * cols);
-            const P* dr = reinterpret_cast<const P*>(dy + row * cols);
-            P* or_ = reinterpret_cast<P*>(dx + row * cols);
-            P rx[NV], rd[NV];
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const unsigned i = threadIdx.x + k * blockDim.x;
-                if (i < nv) {
-                    rx[k] = xr[i];
-                    rd[k] = dr[i];
-                }
-            }
-            const A m = mean[row], rs = rstd[row];
-            A s[2] = {A(0), A(0)};
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const unsigned i = threadIdx.x + k * blockDim.x;
-                if (i < nv) {
-                    const P g = gp[i];
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const A d = to_acc(rd[k].e[e]), xh = (to_acc(rx[k].e[e]) - m) * rs;
-                        const A w = d * to_acc(g.e[e]);
-                        s[0] += w;
-                        s[1] += w * xh;
-                        ag[k][e] += d * xh;
-                        ab[k][e] += d;
-                    }
-                }
-            }
-            row_sum<A, 2>(s, red, turn);
-            const A c1 = s[0] * inv, c2 = s[1] * inv;
-#pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const unsigned i = threadIdx.x + k * blockDim.x;
-                if (i < nv) {
-                    const P g = gp[i];
-                    P o;
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const A xh = (to_acc(rx[k].e[e]) - m) * rs;
-                        from_acc(o.e[e], rs * (to_acc(rd[k].e[e]) * to_acc(g.e[e]) - c1 - xh * c2));
-                    }
-                    or_[i] = o;
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const unsigned i = threadIdx.x + k * blockDim.x;
-            if (i < nv) {
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    pg[(size_t)i * VEC + e] = ag[k][e];
-                    pb[(size_t)i * VEC + e] = ab[k][e];
-                }
-            }
-        }
-    } else {
-        for (unsigned i = threadIdx.x; i < cols; i += blockDim.x) pg[i] = pb[i] = A(0);
-        for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-            const T* xr = x + row * cols;
-            const T* dr = dy + row * cols;
-            T* or_ = dx + row * cols;
-            const A m = mean[row], rs = rstd[row];
-            A s[2] = {A(0), A(0)};
-            // the thread that adds into column i is the same for every row
-            for (unsigned i = threadIdx.x; i < cols; i += blockDim.x) {
-                const A d = to_acc(dr[i]), xh = (to_acc(xr[i]) - m) * rs, w = d * to_acc(gamma[i]);
-                s[0] += w;
-                s[1] += w * xh;
-                pg[i] += d * xh;
-                pb[i] += d;
-            }
-            row_sum<A, 2>(s, red, turn);
-            const A c1 = s[0] * inv, c2 = s[1] * inv;
-            for (unsigned i = threadIdx.x; i < cols; i += blockDim.x) {
-                const A xh = (to_acc(xr[i]) - m) * rs;
-                from_acc(or_[i], rs * (to_acc(dr[i]) * to_acc(gamma[i]) - c1 - xh * c2));
-            }
+            for (int e = 0; e < NP; e++)
+                *reinterpret_cast<W*>(&sh[(size_t)q * pad + (t + k * G) * V + e * N]) = which ? ab[k][e] : ag[k][e];
+        __syncthreads();
+        for (unsigned c = tid; c < cols; c += kBwdThreads) {
+            A v = sh[c];
+            for (unsigned j = 1; j < groups; j++) v += sh[(size_t)j * pad + c];
+            out[c] = v;
         }
     }
 }
 
-// dgamma_j, dbeta_j: the P partial rows added in a fixed order (8 strided
+// A row's two sums over the 512 threads of a CTA: this thread's shares.
+template <typename T, bool AL>
+__device__ __forceinline__ void row_sums(acc_t<T> (&sum)[2], const T* px, const T* pd, const T* gamma,
+                                         acc_t<T> m, acc_t<T> rs, unsigned cols, bool edge) {
+    using A = acc_t<T>;
+    using W = vec_t<T>;
+    constexpr int V = kV<T>, NP = kP<T>, B = 4;
+    const unsigned nv = (cols + V - 1) / V;
+    const W mm = vset(-m, (W*)0), rr = vset(rs, (W*)0);
+    W a0 = vset(A(0), (W*)0), a1 = a0;
+    for (unsigned i0 = threadIdx.x; i0 < nv; i0 += B * 512) {
+        Piece<T> x[B], dy[B];
+#pragma unroll
+        for (int k = 0; k < B; k++) {
+            row_load<T, AL>(x[k], px, i0 + k * 512, cols, edge);
+            row_load<T, AL>(dy[k], pd, i0 + k * 512, cols, edge);
+        }
+#pragma unroll
+        for (int k = 0; k < B; k++) {
+            Piece<T> g;
+            row_load<T, AL>(g, gamma, i0 + k * 512, cols, true);
+            W xv[NP], dv[NP], gv[NP];
+            unpack(xv, x[k]);
+            unpack(dv, dy[k]);
+            unpack(gv, g);
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                const W w = vmul(dv[e], gv[e]);  // zero past the row
+                a0 = vadd(a0, w);
+                a1 = vfma(w, vmul(vadd(xv[e], mm), rr), a1);
+            }
+        }
+    }
+    sum[0] = warp_sum(vsum(a0)), sum[1] = warp_sum(vsum(a1));
+}
+
+// Rows that the threads of a CTA cannot hold the column sums of (x and dy are read
+// twice; blocks of rows that stay in L2 in between measured slower, the launches
+// too small: [4096, 12000] f32 221 us instead of 178): the two sums of
+// every row first, then a pass in which a CTA takes a strip of 256 pieces of
+// columns of the rows 4 blockIdx.y .., + 4 gridDim.y, ...
+template <typename T, bool AL>
+__global__ void __launch_bounds__(512)
+k_norm_bwd_sums(acc_t<T>* __restrict__ sums, const T* dy, const T* x, const T* __restrict__ gamma,
+                const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd, unsigned rows,
+                unsigned cols) {
+    using A = acc_t<T>;
+    __shared__ A p[2][16];
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        A s[2];
+        row_sums<T, AL>(s, x + row * cols, dy + row * cols, gamma, mean[row], rstd[row], cols,
+                        row == 0 || row + 1 == rows);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) p[0][threadIdx.x >> 5] = s[0], p[1][threadIdx.x >> 5] = s[1];
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            A v = A(0);
+            for (int k = 0; k < 16; k++) v += p[threadIdx.x][k];
+            sums[2 * row + threadIdx.x] = v;
+        }
+    }
+}
+
+template <typename T, bool AL>
+__global__ void __launch_bounds__(256)
+k_norm_bwd_strips(T* dx, acc_t<T>* __restrict__ part, const acc_t<T>* __restrict__ sums,
+                  const T* dy, const T* x, const T* __restrict__ gamma,
+                  const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd,
+                  unsigned rows, unsigned cols) {
+    using A = acc_t<T>;
+    using W = vec_t<T>;
+    constexpr int V = kV<T>, NP = kP<T>;
+    const A inv = A(1) / A(cols);
+    const unsigned i = blockIdx.x * 256 + threadIdx.x;
+    Piece<T> g;
+    row_load<T, AL>(g, gamma, i, cols, true);
+    W gv[NP], ag[NP], ab[NP];
+    unpack(gv, g);
+#pragma unroll
+    for (int e = 0; e < NP; e++) ag[e] = ab[e] = vset(A(0), (W*)0);
+    constexpr int R = 4;  // rows whose loads are in flight together
+    for (size_t row0 = (size_t)blockIdx.y * R; row0 < rows; row0 += (size_t)gridDim.y * R) {
+        Piece<T> px[R], pd[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const size_t row = row0 + r;
+            if (row >= rows) break;
+            const bool edge = row == 0 || row + 1 == rows;
+            row_load<T, AL>(px[r], x + row * cols, i, cols, edge);
+            row_load<T, AL>(pd[r], dy + row * cols, i, cols, edge);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const size_t row = row0 + r;
+            if (row >= rows) break;
+            const W mm = vset(-mean[row], (W*)0), rr = vset(rstd[row], (W*)0);
+            const W c1 = vset(-sums[2 * row] * inv, (W*)0), c2 = vset(-sums[2 * row + 1] * inv, (W*)0);
+            W xv[NP], dv[NP];
+            unpack(xv, px[r]);
+            unpack(dv, pd[r]);
+#pragma unroll
+            for (int e = 0; e < NP; e++) {
+                const W xh = vmul(vadd(xv[e], mm), rr);
+                ag[e] = vfma(dv[e], xh, ag[e]);
+                ab[e] = vadd(ab[e], dv[e]);
+                xv[e] = vmul(rr, vadd(vfma(xh, c2, vmul(dv[e], gv[e])), c1));
+            }
+            pack(px[r], xv);
+            row_store<T, AL>(dx + row * cols, px[r], i, cols, threadIdx.x & 31, 32, true);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        const unsigned c = i * V + e;
+        if (c < cols) {
+            part[(size_t)blockIdx.y * cols + c] = reinterpret_cast<const A*>(ag)[e];
+            part[(size_t)(gridDim.y + blockIdx.y) * cols + c] = reinterpret_cast<const A*>(ab)[e];
+        }
+    }
+}
+
+// dgamma_j, dbeta_j: the P partial rows added in a fixed order (32 strided
 // sums per column, then a tree); P = 0 gives zeros.  blockIdx.y: which of the two.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 k_norm_fold(T* __restrict__ dgamma, T* __restrict__ dbeta, const acc_t<T>* __restrict__ part,
             unsigned P, unsigned cols) {
     using A = acc_t<T>;
-    __shared__ A t[8][33];
+    __shared__ A t[32][33];
     const unsigned col = blockIdx.x * 32 + threadIdx.x;
     const A* p = part + (size_t)blockIdx.y * P * cols;
     A s = A(0);
-    if (col < cols)
-        for (unsigned r = threadIdx.y; r < P; r += 8) s += p[(size_t)r * cols + col];
+    if (col < cols) {
+#pragma unroll 4
+        for (unsigned r = threadIdx.y; r < P; r += 32) s += p[(size_t)r * cols + col];
+    }
     t[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && col < cols) {
-        A v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = t[k][threadIdx.x];
-        const A sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-        from_acc((blockIdx.y == 0 ? dgamma : dbeta)[col], sum);
-    }
+    // warp y folds column y of the block
+    const A sum = warp_sum(t[threadIdx.x][threadIdx.y]);
+    const unsigned c2 = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && c2 < cols) from_acc((blockIdx.y == 0 ? dgamma : dbeta)[c2], sum);
 }
 
-bool aligned16(std::initializer_list<const void*> ps) {
+template <typename T>
+bool all_aligned(unsigned cols, std::initializer_list<const void*> ps) {
+    if (cols % kV<T>) return false;
     for (const void* p : ps)
-        if (((uintptr_t)p) & 15) return false;
+        if ((uintptr_t)p & 15) return false;
     return true;
 }
 
-// Threads per row: enough warps that a thread holds at most NVMAX pieces.
-unsigned row_threads(size_t pieces, unsigned per_thread, unsigned most) {
-    size_t t = (pieces + per_thread - 1) / per_thread;
-    t = (t + 31) / 32 * 32;
-    return (unsigned)(t > most ? most : t);
-}
-
-template <typename T, int VEC>
+template <typename T, bool AL>
 void fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, const T* b,
-         unsigned rows, unsigned cols, double eps) {
-    const size_t nv = cols / VEC;
-    const auto e = (acc_t<T>)eps;
-    const unsigned tx = row_threads(nv, 4, 1024);
-    const unsigned ty = tx == 32 ? 4 : 1;
-    const dim3 blk(tx, ty), grid((rows + ty - 1) / ty);
-    const size_t k = (nv + tx - 1) / tx;
-    if (k <= 1) k_norm_fwd<T, VEC, 1><<<grid, blk, 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, e);
-    else if (k <= 2) k_norm_fwd<T, VEC, 2><<<grid, blk, 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, e);
-    else if (k <= 4) k_norm_fwd<T, VEC, 4><<<grid, blk, 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, e);
-    else if (k <= 8) k_norm_fwd<T, VEC, 8><<<grid, blk, 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, e);
-    else k_norm_fwd<T, VEC, 0><<<grid, blk, 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, e);
-    count_launch();
+         unsigned rows, unsigned cols, acc_t<T> eps) {
+    const size_t nv = ((size_t)cols + kV<T> - 1) / kV<T>;
+    if (nv > 16 * 512) {
+        k_norm_fwd_long<T><<<std::min(rows, (unsigned)c.dev->sm_count * 2), 1024, 0, c.stream>>>(
+            y, mean, rstd, x, g, b, rows, cols, eps);
+        return;
+    }
+    // Many rows: up to 16 pieces a thread, no barrier for rows of up to 8 KB.
+    // Few rows (less than 16 warps an SM with a warp each): 4, for latency.
+    const bool many = rows >= (unsigned)c.dev->sm_count * 16;
+    const unsigned per = many || nv > 4 * 512 ? 16 : 4;
+    const unsigned tx = (unsigned)((nv + per - 1) / per + 31) / 32 * 32;
+    const unsigned ty = tx == 32 ? 4 : 1, k = (unsigned)((nv + tx - 1) / tx);
+    auto f = k <= 1   ? k_norm_fwd<T, 1, AL>
+             : k <= 2 ? k_norm_fwd<T, 2, AL>
+             : k <= 4 ? k_norm_fwd<T, 4, AL>
+             : k <= 8 ? k_norm_fwd<T, 8, AL>
+                      : k_norm_fwd<T, 16, AL>;
+    f<<<(rows + ty - 1) / ty, dim3(tx, ty), 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, eps);
 }
 
 template <typename T>
 int fwd_t(Ctx& c, void* y, void* mean, void* rstd, const void* x, const void* g, const void* b,
           unsigned rows, unsigned cols, double eps) {
-    constexpr int V = 16 / sizeof(T);
     using A = acc_t<T>;
-    if (cols % V == 0 && aligned16({y, x, g, b}))
-        fwd<T, V>(c, (T*)y, (A*)mean, (A*)rstd, (const T*)x, (const T*)g, (const T*)b, rows, cols, eps);
-    else
-        fwd<T, 1>(c, (T*)y, (A*)mean, (A*)rstd, (const T*)x, (const T*)g, (const T*)b, rows, cols, eps);
+    auto f = all_aligned<T>(cols, {y, x, g, b}) ? fwd<T, true> : fwd<T, false>;
+    f(c, (T*)y, (A*)mean, (A*)rstd, (const T*)x, (const T*)g, (const T*)b, rows, cols, (A)eps);
+    count_launch();
     pdl_record_all(c);
     return finish(c);
 }
 
-template <typename T, int VEC>
-void bwd(Ctx& c, T* dx, acc_t<T>* part, const T* dy, const T* x, const T* g, const acc_t<T>* mean,
-         const acc_t<T>* rstd, unsigned rows, unsigned cols, unsigned P) {
-    const size_t nv = cols / VEC;
-    const unsigned tx = row_threads(nv, 2, 512);
-    const size_t k = (nv + tx - 1) / tx;
-    if (k <= 1) k_norm_bwd<T, VEC, 1><<<P, tx, 0, c.stream>>>(dx, part, dy, x, g, mean, rstd, rows, cols);
-    else if (k <= 2) k_norm_bwd<T, VEC, 2><<<P, tx, 0, c.stream>>>(dx, part, dy, x, g, mean, rstd, rows, cols);
-    else if (k <= 4) k_norm_bwd<T, VEC, 4><<<P, tx, 0, c.stream>>>(dx, part, dy, x, g, mean, rstd, rows, cols);
-    else k_norm_bwd<T, VEC, 0><<<P, 1024, 0, c.stream>>>(dx, part, dy, x, g, mean, rstd, rows, cols);
+// How the backward pass runs: by rows (strips = 0) or by strips; and the
+// partial rows of the weights' gradients that it leaves.
+struct BwdShape {
+    unsigned strips, grid, parts;
+    Deal deal;
+};
+constexpr unsigned kBwdCtas = 148;  // of a B200; fixed, as the workspace's size must not depend on the device
+template <typename T> constexpr int kPer = kV<T> == 8 ? 2 : 4;   // pieces a thread: at most 16 columns' sums
+template <typename T> constexpr int kRows = kV<T> == 8 ? 2 : 1;  // rows at a time
+template <typename T>
+BwdShape bwd_shape_t(unsigned rows, unsigned cols) {
+    const size_t nv = ((size_t)cols + kV<T> - 1) / kV<T>;
+    BwdShape q{};
+    if (nv > (size_t)kBwdThreads * kPer<T>) {
+        q.strips = (unsigned)((nv + 255) / 256);
+        q.grid = q.parts = std::min((rows + 3) / 4, (kBwdCtas * 4 + q.strips - 1) / q.strips);
+        return q;
+    }
+    Deal& d = q.deal;
+    d.rows = rows;
+    d.cols = cols;
+    for (d.G = 4, d.lg = 2; (size_t)d.G * kPer<T> < nv; d.lg++) d.G *= 2;
+    const size_t per_round = (size_t)(kBwdThreads / d.G) * kRows<T>;
+    d.rounds = (unsigned)((rows + per_round - 1) / per_round);
+    q.grid = q.parts = std::min(d.rounds, kBwdCtas);
+    return q;
+}
+BwdShape bwd_shape(unsigned rows, unsigned cols, int dt) {
+    return dt == F32 ? bwd_shape_t<float>(rows, cols) : dt == F64 ? bwd_shape_t<double>(rows, cols)
+                                                                  : bwd_shape_t<bf16>(rows, cols);
+}
+size_t bwd_part_bytes(const BwdShape& q, unsigned cols, int dt) {
+    return (size_t)2 * q.parts * cols * (dt == F64 ? 8 : 4);
+}
+
+template <typename T, bool AL>
+int bwd(Ctx& c, const BwdShape& q, T* dx, acc_t<T>* part, acc_t<T>* sums, const T* dy, const T* x,
+        const T* g, const acc_t<T>* mean, const acc_t<T>* rstd, unsigned rows, unsigned cols) {
+    if (q.strips) {
+        k_norm_bwd_sums<T, AL><<<std::min(rows, (unsigned)c.dev->sm_count * 4), 512, 0, c.stream>>>(
+            sums, dy, x, g, mean, rstd, rows, cols);
+        k_norm_bwd_strips<T, AL><<<dim3(q.strips, q.grid), 256, 0, c.stream>>>(
+            dx, part, sums, dy, x, g, mean, rstd, rows, cols);
+        count_launch(2);
+        return OK;
+    }
+    const bool one = ((size_t)cols + kV<T> - 1) / kV<T> <= q.deal.G;
+    auto f = one ? k_norm_bwd<T, 1, kRows<T>, AL> : k_norm_bwd<T, kPer<T>, kRows<T>, AL>;
+    const size_t bytes = (size_t)kBwdThreads * (one ? 1 : kPer<T>) * kV<T> * sizeof(acc_t<T>);
+    NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    f<<<q.grid, kBwdThreads, bytes, c.stream>>>(dx, part, dy, x, g, mean, rstd, q.deal);
     count_launch();
+    return OK;
 }
 
 template <typename T>
-int bwd_t(Ctx& c, void* dx, void* dg, void* db, void* ws, const void* dy, const void* x,
+int bwd_t(Ctx& c, int dt, void* dx, void* dg, void* db, void* ws, const void* dy, const void* x,
           const void* g, const void* mean, const void* rstd, unsigned rows, unsigned cols) {
-    constexpr int V = 16 / sizeof(T);
     using A = acc_t<T>;
-    const unsigned P = norm_grad_blocks(rows);
+    const BwdShape q = bwd_shape(rows, cols, dt);
     if (rows > 0) {
-        if (cols % V == 0 && aligned16({dx, dy, x, g}))
-            bwd<T, V>(c, (T*)dx, (A*)ws, (const T*)dy, (const T*)x, (const T*)g, (const A*)mean,
-                      (const A*)rstd, rows, cols, P);
-        else
-            bwd<T, 1>(c, (T*)dx, (A*)ws, (const T*)dy, (const T*)x, (const T*)g, (const A*)mean,
-                      (const A*)rstd, rows, cols, P);
+        auto f = all_aligned<T>(cols, {dx, dy, x, g}) ? bwd<T, true> : bwd<T, false>;
+        const int rc = f(c, q, (T*)dx, (A*)ws, (A*)((char*)ws + bwd_part_bytes(q, cols, dt)),
+                         (const T*)dy, (const T*)x, (const T*)g, (const A*)mean, (const A*)rstd, rows,
+                         cols);
+        if (rc) return rc;
     }
-    k_norm_fold<T><<<dim3((cols + 31) / 32, 2), dim3(32, 8), 0, c.stream>>>((T*)dg, (T*)db,
-                                                                           (const A*)ws, P, cols);
+    k_norm_fold<T><<<dim3((cols + 31) / 32, 2), dim3(32, 32), 0, c.stream>>>(
+        (T*)dg, (T*)db, (const A*)ws, q.parts, cols);
     count_launch();
     pdl_record_all(c);
     return finish(c);
@@ -391,11 +864,11 @@ int bwd_t(Ctx& c, void* dx, void* dg, void* db, void* ws, const void* dy, const 
 
 }  // namespace
 
-// Partial rows of the weight gradients: one per CTA of the backward kernel.
-unsigned norm_grad_blocks(unsigned rows) { return rows < 296 ? rows : 296; }
-
+// The backward kernel's partial rows of dgamma and dbeta, and for strips two
+// sums of every row.
 size_t norm_grad_workspace(unsigned rows, unsigned cols, int dt) {
-    return (size_t)2 * norm_grad_blocks(rows) * cols * (dt == F64 ? 8 : 4);
+    const BwdShape q = bwd_shape(rows, cols, dt);
+    return bwd_part_bytes(q, cols, dt) + (q.strips ? (size_t)2 * rows * (dt == F64 ? 8 : 4) : 0);
 }
 
 int launch_layer_norm(Ctx& c, int dt, void* y, void* mean, void* rstd, const void* x,
@@ -411,10 +884,10 @@ int launch_layer_norm_grad(Ctx& c, int dt, void* dx, void* dgamma, void* dbeta, 
                            const void* dy, const void* x, const void* gamma, const void* mean,
                            const void* rstd, unsigned rows, unsigned cols) {
     if (dt == F32)
-        return bwd_t<float>(c, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
+        return bwd_t<float>(c, dt, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
     if (dt == F64)
-        return bwd_t<double>(c, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
-    return bwd_t<bf16>(c, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
+        return bwd_t<double>(c, dt, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
+    return bwd_t<bf16>(c, dt, dx, dgamma, dbeta, ws, dy, x, gamma, mean, rstd, rows, cols);
 }
 
 }  // namespace nxv

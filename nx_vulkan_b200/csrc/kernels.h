@@ -61,7 +61,6 @@ int launch_dropout(Ctx& c, int dt, void* y, const void* x, size_t n, double p, u
 int launch_layer_norm(Ctx& c, int dt, void* y, void* mean, void* rstd, const void* x,
                       const void* gamma, const void* beta, unsigned rows, unsigned cols,
                       double eps);
-unsigned norm_grad_blocks(unsigned rows);
 size_t norm_grad_workspace(unsigned rows, unsigned cols, int dt);
 int launch_layer_norm_grad(Ctx& c, int dt, void* dx, void* dgamma, void* dbeta, void* ws,
                            const void* dy, const void* x, const void* gamma, const void* mean,

@@ -75,7 +75,8 @@ def place(torch, t, shift):
 # ---- layer norm ---------------------------------------------------------------
 
 NORM_SHAPES = [(1, 1), (1, 2), (4, 7), (5, 32), (9, 33), (3, 256), (7, 1000), (2, 1023), (300, 129),
-               (3, 4096), (2, 5001), (2, 8192), (1, 16384), (2, 20000), (1, 40001), (600, 64)]
+               (3, 4096), (2, 5001), (7, 5003), (2, 8192), (3, 12289), (1, 16384), (2, 20000), (1, 40001), (3, 70001),
+               (600, 64), (1200, 33), (700, 1025), (500, 20003)]
 
 
 def norm_run(nxv, torch, x, g, b, eps, name, y=None):
@@ -181,8 +182,8 @@ def grad_check(torch, name, dy, x, g, m, s, dx, dg, db):
     want = S * (w - a - xh * q)
     size = S * (w.abs() + w.abs().mean(1, keepdim=True) + xh.abs() * (w * xh).abs().mean(1, keepdim=True))
     within(torch, dx, want, H[name] * want.abs() + k * size)
-    # rows / 296 + 1 rows a thread, then 296 / 8 partial rows a thread and 3 levels, 4 roundings a term
-    kk = (r / 296 + 1 + 296 / 8 + 8) * U[name]
+    # at most r / 128 + 1 rows a thread, then 2400 / 32 partial rows a thread and 5 levels, 4 roundings a term
+    kk = (r / 128 + 1 + 2400 / 32 + 9) * U[name]
     within(torch, dg, (DY * xh).sum(0), H[name] * (DY * xh).sum(0).abs() + kk * (DY * xh).abs().sum(0))
     within(torch, db, DY.sum(0), H[name] * DY.sum(0).abs() + kk * DY.abs().sum(0))
 
@@ -715,13 +716,14 @@ def test_refusals_on_device(nxv, torch):
     lg = lambda dx, dg, ws: lib.nxv_layer_norm_grad(dx.handle, dg.handle, W(2500, 16).handle, ws, y.handle,  # noqa: E731
                                                     x.handle, v.handle, st[0].handle, st[1].handle, 4, 16, 0,
                                                     b"layer_norm_grad.spv")
-    dx, dg, ws = W(256, 64), W(2400, 16), W(2560, 128)
+    need = nxv.layer_norm_grad_workspace(4, 16) // 4
+    dx, dg, ws = W(256, 64), W(2400, 16), W(2560, need)
     assert lg(dx, dg, None) == 0 and lg(dx, dg, ws.handle) == 0 and lg(y, dg, ws.handle) == 0
     refused(lg(W(1028, 64), dg, None), "shares memory")
     refused(lg(dx, v, None), "shares memory")
-    refused(lg(dx, dg, W(2560, 64).handle), "workspace")
-    refused(lg(dx, dg, W(2562, 128).handle), "workspace")
-    refused(lg(dx, dg, W(0, 128).handle), "shares memory")
+    refused(lg(dx, dg, W(2560, need - 1).handle), "workspace")
+    refused(lg(dx, dg, W(2562, need).handle), "workspace")
+    refused(lg(dx, dg, W(0, need).handle), "shares memory")
     dr = lambda o, x: lib.nxv_dropout(o.handle, x.handle, 64, 0.5, 1, 0, 0, b"dropout.spv")  # noqa: E731
     assert dr(y, x) == 0 and dr(x, x) == 0
     refused(dr(W(1, 64), x), "shares memory")

@@ -74,7 +74,8 @@ def test_values_out_of_range(lib):
                                                  b"linear_cross_entropy_grad.spv") == -3
     assert lib.nxv_linear_cross_entropy_workspace(2, 0, 4, 0, 0) == 0
     assert lib.nxv_linear_cross_entropy_workspace(2, 3, 4, 0, 0) > 0
-    assert lib.nxv_layer_norm_grad_workspace(5, 7, 0) == 2 * 5 * 7 * 4
+    assert lib.nxv_layer_norm_grad_workspace(5, 7, 0) >= 2 * 7 * 4
+    assert lib.nxv_layer_norm_grad_workspace(5, 7, 3) == 0
 
 
 def test_the_mirror_refuses_too(lib):
