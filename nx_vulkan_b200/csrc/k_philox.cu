@@ -266,7 +266,7 @@ __global__ void k_random_f64(double* __restrict__ out, size_t n, uint32_t seed, 
 
 // ---- dropout ------------------------------------------------------------------
 //
-// y_i = x_i * scale where (word >> 8) >= thresh, else 0 (whatever x_i is, NaN
+// y_i = x_i / (1 - p) where (word >> 8) >= thresh, else 0 (whatever x_i is, NaN
 // and infinities included).  thresh = ceil(p 2^24): the comparison of the
 // uniform (word >> 8) 2^-24 with p, in whole numbers.  f32 arithmetic for f32
 // and bf16 (bf16 rounded once at the store), f64 for f64.
@@ -276,60 +276,111 @@ __device__ __forceinline__ __nv_bfloat16 drop_scaled(__nv_bfloat16 x, double, fl
     return __float2bfloat16_rn(__fmul_rn(__bfloat162float(x), s));
 }
 
+// The generator with its ten round keys at hand (they depend on the seed alone).
+struct PhiloxKeys {
+    uint32_t k[10];
+    __device__ __forceinline__ explicit PhiloxKeys(uint32_t seed) {
+#pragma unroll
+        for (int r = 0; r < 10; r++) k[r] = seed + (uint32_t)r * 0x9E3779B9u;
+    }
+    __device__ __forceinline__ void words(uint32_t c, uint32_t& o0, uint32_t& o1) const {
+        uint32_t x0 = c, x1 = 0;
+#pragma unroll
+        for (int r = 0; r < 10; r++) {
+            const unsigned long long prod = (unsigned long long)x0 * 0xD256D193ull;
+            x0 = (uint32_t)(prod >> 32) ^ k[r] ^ x1;
+            x1 = (uint32_t)prod;
+        }
+        o0 = x0;
+        o1 = x1;
+    }
+};
+
 template <typename T>
-__device__ __forceinline__ T drop_one(T x, uint32_t w, uint32_t thresh, double s64, float s32) {
-    return (w >> 8) >= thresh ? drop_scaled(x, s64, s32) : T(0.0f);
+__device__ __forceinline__ T drop_one(T x, uint32_t w, uint32_t least, double s64, float s32) {
+    return w >= least ? drop_scaled(x, s64, s32) : T(0.0f);
+}
+
+// The 16 bytes x at p[0 .. 3], whose elements' words are w.
+__device__ __forceinline__ void drop_16(uint32_t (&x)[4], const uint32_t* w, uint32_t least, double,
+                                        float s32, __nv_bfloat16) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float lo = __fmul_rn(__uint_as_float(x[k] << 16), s32);
+        const float hi = __fmul_rn(__uint_as_float(x[k] & 0xffff0000u), s32);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        uint32_t r = *reinterpret_cast<const uint32_t*>(&h);
+        if (w[2 * k] < least) r &= 0xffff0000u;
+        if (w[2 * k + 1] < least) r &= 0x0000ffffu;
+        x[k] = r;
+    }
+}
+__device__ __forceinline__ void drop_16(uint32_t (&x)[4], const uint32_t* w, uint32_t least, double,
+                                        float s32, float) {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        x[k] = w[k] >= least ? __float_as_uint(__fmul_rn(__uint_as_float(x[k]), s32)) : 0u;
+}
+__device__ __forceinline__ void drop_16(uint32_t (&x)[4], const uint32_t* w, uint32_t least, double s64,
+                                        float, double) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const double v = __dmul_rn(__hiloint2double((int)x[2 * k + 1], (int)x[2 * k]), s64);
+        x[2 * k] = w[k] >= least ? (uint32_t)__double2loint(v) : 0u;
+        x[2 * k + 1] = w[k] >= least ? (uint32_t)__double2hiint(v) : 0u;
+    }
 }
 
 // A thread takes VEC consecutive elements (16 bytes) of VEC / 2 counters; with
-// an odd offset (ODD) their words lie in VEC / 2 + 1 counters.  The last n % VEC
-// elements, and every element of a tensor that is not 16-byte aligned
-// (VEC = 1), go one by one.
+// an odd offset (ODD) their words lie in VEC / 2 + 1 counters.  The elements behind the last whole vector, and every element of a
+// tensor that is not 16-byte aligned (VEC = 1), go one by one.  least: the
+// smallest word that keeps its element, thresh << 8 (the eight low bits do not
+// count); none does for p = 1, where all is zeros.
 template <typename T, int VEC, bool ODD>
-__global__ void __launch_bounds__(256)
-k_dropout(T* y, const T* x, size_t n, uint32_t thresh, double s64, float s32, uint32_t seed,
+__global__ void __launch_bounds__(256, 6)
+k_dropout(T* y, const T* x, size_t n, uint32_t least, double s64, float s32, uint32_t seed,
           uint64_t offset) {
     const size_t stride = (size_t)gridDim.x * blockDim.x;
     const size_t t0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const PhiloxKeys keys(seed);
     size_t done = 0;
     if constexpr (VEC > 1) {
-        struct alignas(16) V {
-            T e[VEC];
-        };
+        constexpr int C = VEC / 2 + (ODD ? 1 : 0);
         const size_t nv = n / VEC;
         for (size_t q = t0; q < nv; q += stride) {
-            V v = reinterpret_cast<const V*>(x)[q];
+            const uint4 in = reinterpret_cast<const uint4*>(x)[q];
             const uint32_t c0 = (uint32_t)((offset + q * VEC) >> 1);
-            uint32_t w[VEC + 2];
+            uint32_t w[2 * C], v[4] = {in.x, in.y, in.z, in.w};
 #pragma unroll
-            for (int k = 0; k < VEC / 2 + (ODD ? 1 : 0); k++)
-                philox2x32(c0 + k, 0u, seed, w[2 * k], w[2 * k + 1]);
-#pragma unroll
-            for (int e = 0; e < VEC; e++)
-                v.e[e] = drop_one(v.e[e], w[e + (ODD ? 1 : 0)], thresh, s64, s32);
-            reinterpret_cast<V*>(y)[q] = v;
+            for (int k = 0; k < C; k++) keys.words(c0 + k, w[2 * k], w[2 * k + 1]);
+            drop_16(v, w + (ODD ? 1 : 0), least, s64, s32, T(0.0f));
+            reinterpret_cast<uint4*>(y)[q] = make_uint4(v[0], v[1], v[2], v[3]);
         }
         done = nv * VEC;
     }
     for (size_t i = done + t0; i < n; i += stride) {
         const uint64_t s = offset + i;
         uint32_t w0, w1;
-        philox2x32((uint32_t)(s >> 1), 0u, seed, w0, w1);
-        y[i] = drop_one(x[i], (s & 1) ? w1 : w0, thresh, s64, s32);
+        keys.words((uint32_t)(s >> 1), w0, w1);
+        y[i] = drop_one(x[i], (s & 1) ? w1 : w0, least, s64, s32);
     }
 }
 
 template <typename T>
 void dropout_t(Ctx& c, T* y, const T* x, size_t n, double p, uint32_t seed, uint64_t offset) {
     constexpr int V = 16 / sizeof(T);
-    const uint32_t thresh = (uint32_t)ceil(p * 0x1.0p24);  // p 2^24 is exact
-    const double s64 = p < 1.0 ? 1.0 / (1.0 - p) : 0.0;    // p = 1 keeps nothing
+    const uint32_t least = (uint32_t)ceil(p * 0x1.0p24) << 8;  // p 2^24 is exact
+    const double s64 = 1.0 / (1.0 - p);
     const float s32 = (float)s64;
     const bool vec = ((((uintptr_t)x) | ((uintptr_t)y)) & 15) == 0;
+    if (p >= 1.0) {
+        cudaMemsetAsync(y, 0, n * sizeof(T), c.stream);
+        return;
+    }
     const unsigned g = grid_for(c, vec ? (n + V - 1) / V : n, 256, 8);
-    if (!vec) k_dropout<T, 1, false><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
-    else if (offset & 1) k_dropout<T, V, true><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
-    else k_dropout<T, V, false><<<g, 256, 0, c.stream>>>(y, x, n, thresh, s64, s32, seed, offset);
+    if (!vec) k_dropout<T, 1, false><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
+    else if (offset & 1) k_dropout<T, V, true><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
+    else k_dropout<T, V, false><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
     count_launch();
 }
 
