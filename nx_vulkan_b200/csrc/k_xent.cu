@@ -36,7 +36,10 @@
 
 #include "kernels.h"
 
+#include <limits.h>
+
 #include <algorithm>
+#include <type_traits>
 
 namespace nxv {
 
@@ -253,6 +256,8 @@ struct Job {
     int M, N, K;          // D[M, N] = A[M, K] B[N, K]^T
     int a_mn, b_mn;       // the operand is stored K rows of M (N) values
     uint32_t tm, tiles;   // row tiles, all tiles
+    uint32_t plane;       // tiles of one slice of K
+    int kslice;           // the K of a slice, a multiple of BK
     long long col0;       // LSE, GRAD: the class of column 0
     // LSE
     float* part_m;        // [column segment of 64 CG classes][M]
@@ -267,6 +272,7 @@ struct Job {
     bf16* g;              // planes of [M][ldg]
     long long ldg, gplane;
     // OUT
+    // OUT: with slices, f32 [slice][M][ldo] each
     const float* acc_in;  // f32 [M][ldo] to add, or null
     const float* dloss;   // [M]: the rows' factors, 0 for a row without a target; or null
     const float* factor;  // one factor of all, or null
@@ -274,6 +280,12 @@ struct Job {
     int out_bf16;
     long long ldo;
 };
+
+// K blocks of tile lt of the job.
+__device__ __forceinline__ int k_blocks(const Job& g, uint32_t lt) {
+    const int first = (int)(lt / g.plane) * g.kslice;
+    return (min(g.K - first, g.kslice) + BK - 1) / BK;
+}
 
 constexpr int kMaxJobs = 3;
 struct alignas(64) Work {
@@ -315,11 +327,14 @@ struct Row {
     // GRAD
     float lse = 0.0f;
     // OUT
+    size_t row_at = 0;  // the row's first element in out and acc_in
     float dl = 0.0f;
     int align = 0;
     bool has = false;
 
-    __device__ __forceinline__ Row(const Job& j, int r, int n) : g(j), row(r), n0(n), left(j.N - n), live(r < j.M) {
+    __device__ __forceinline__ Row(const Job& j, int r, int n, uint32_t slice)
+        : g(j), row(r), n0(n), left(j.N - n), live(r < j.M) {
+        row_at = ((size_t)slice * g.M + row) * g.ldo;
         if (g.kind == OUT) {
             const int es = g.out_bf16 ? 2 : 4;
             const uintptr_t a = (uintptr_t)g.out | (uintptr_t)(g.ldo * es) | (uintptr_t)g.acc_in |
@@ -409,7 +424,7 @@ struct Row {
 
     __device__ __forceinline__ void chunk_out(float (&v)[32], int c0) {
         if (!live) return;
-        const size_t at = (size_t)row * g.ldo + n0 + c0;
+        const size_t at = row_at + n0 + c0;
         const bool whole = align >= 16 && c0 + 32 <= left;
         if (g.acc_in) {
             if (whole) {
@@ -561,12 +576,14 @@ k_xgemm(const __grid_constant__ Work W) {
         for (uint32_t t = first; t < W.tiles && ok; t += step) {
             uint32_t j = 0, lt = t;
             while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
-            const uint32_t tm = W.job[j].tm;
+            const uint32_t tm = W.job[j].tm, slice = lt / W.job[j].plane;
+            lt -= slice * W.job[j].plane;
             const CUtensorMap* map = &W.map[2 * j + is_b];
             const bool mn = is_b ? W.job[j].b_mn : W.job[j].a_mn;
             const int r0 = (int)((is_b ? lt / tm : lt % tm) * NC + rank * BT);
-            const int K = W.job[j].K;
-            for (int k0 = 0; k0 < K && ok; k0 += BK) {
+            const int first_k = (int)slice * W.job[j].kslice;
+            const int K = min(W.job[j].K, first_k + W.job[j].kslice);
+            for (int k0 = first_k; k0 < K && ok; k0 += BK) {
 #pragma unroll
                 for (int p = 0; p < (SIX ? 6 : 1); p++) {
                     ok = warp_wait(b_empty + s * 8, par, &s_err);
@@ -607,7 +624,7 @@ k_xgemm(const __grid_constant__ Work W) {
             const uint32_t id = idesc<CG>(a_mn, b_mn);
             const uint64_t ka = kstep(a_mn), kb = kstep(b_mn);
             const uint64_t da0 = sdesc(ring, a_mn), db0 = sdesc(ring + OP_BYTES, b_mn);
-            const int KB = (W.job[j].K + BK - 1) / BK;
+            const int KB = k_blocks(W.job[j], lt);
             const int phases = SIX ? KB : 1, per = SIX ? 6 : KB;
             for (int f = 0; f < phases && ok; f++, ph++) {
                 const uint32_t buf = ph & 1;
@@ -647,10 +664,12 @@ k_xgemm(const __grid_constant__ Work W) {
             uint32_t j = 0, lt = t;
             while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
             const Job& g = W.job[j];
+            const int KB = k_blocks(g, lt);
+            const uint32_t slice = lt / g.plane;
+            lt -= slice * g.plane;
             const int row = (int)(lt % g.tm * NC) + rank * BT + q * 32 + lane;
             const int n0 = (int)(lt / g.tm * NC) + h * HALF;
             if constexpr (SIX) {
-                const int KB = (g.K + BK - 1) / BK;
                 float acc[HALF];
 #pragma unroll
                 for (int e = 0; e < HALF; e++) acc[e] = 0.0f;
@@ -671,7 +690,7 @@ k_xgemm(const __grid_constant__ Work W) {
                     if (lane == 0) mbar_arrive_leader(b_free + buf * 8);
                 }
                 if (!ok) break;
-                Row r(g, row, n0);
+                Row r(g, row, n0, slice);
 #pragma unroll
                 for (int c = 0; c < HALF / 32; c++) {
                     float v[32];
@@ -682,7 +701,7 @@ k_xgemm(const __grid_constant__ Work W) {
                 r.done(HALF);
             } else {
                 const uint32_t buf = ph & 1;
-                Row r(g, row, n0);
+                Row r(g, row, n0, slice);
                 ok = warp_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err);
                 if (!ok) break;
                 ph++;
@@ -835,6 +854,256 @@ k_xent_join(float* __restrict__ loss, float* __restrict__ lse, const float* __re
     }
 }
 
+// ---- small problems ---------------------------------------------------------------
+//
+// For few multiply-adds per product the packing, the tensor maps and the
+// pipeline's start cost more than the products.  k_small does them with f32 FMAs straight from the tensors, a
+// TM x TN tile a CTA, KG groups of its threads taking every KG-th k of a chunk,
+// added in order at the end: two launches forward (tiles, join) and two or three
+// backward (P, both products, and where a long K is cut into slices, their sum).
+
+// The limits, from both paths' times, loss / gradient in us, small path first:
+// f32 16 x 200 x 100 10 / 15 and 23 / 39, 64 x 1001 x 1000 23 / 60 and 42 / 81, 512^3
+// 33 / 101 and 35 / 70; bf16 16 x 200 x 104 10 / 15 and 11 / 23, 64 x 1001 x 1000
+// 23 / 60 and 15 / 31.
+constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;
+constexpr int KC = 64;  // k of a chunk
+
+struct SmallJob {
+    int kind;
+    // LSE, GRAD: A [M][K] and B [N][K] of T; OUT: A f32, [M][K] or (a_mn) [K][M], B [K][N] of T
+    const void *A, *B;
+    int a_mn;
+    long long lda, ldb;
+    int M, N, K;
+    int tm, tn, tiles;    // tiles of one slice, and of all
+    int kslice;           // the k of a slice, a multiple of KC
+    const float* bscale;  // OUT: a factor of B's row k, 0 without a target; or null
+    // as in Job
+    float *part_m, *part_s, *zlabel;
+    const void* labels;
+    int index_bytes;
+    long long vocab;
+    const float *lse, *dloss;
+    float* p;             // GRAD: [M][N]
+    void* out;            // OUT: T [M][N], or f32 [slice][M][N] where `partial`
+    int partial;
+};
+struct SmallWork {
+    SmallJob job[2];
+    int jobs, tiles;
+};
+
+__device__ __forceinline__ float f32_of(float v) { return v; }
+__device__ __forceinline__ float f32_of(bf16 v) { return __bfloat162float(v); }
+
+// P: OUT jobs; else LSE or GRAD.
+template <typename T, bool P, int TM, int TN, int RM, int RN, int KG>
+__global__ void __launch_bounds__(TM / RM * (TN / RN) * KG)
+k_small(const __grid_constant__ SmallWork w) {
+    constexpr int GT = TM / RM * (TN / RN), NT = GT * KG;  // threads of a group, of the CTA
+    constexpr int LA = TM * KC / NT, LB = TN * KC / NT;
+    // the finished tile takes the place of the last chunk
+    static_assert(RM == 4 && (RN == 2 || RN == 4) && KC % KG == 0, "tile");
+    __shared__ union alignas(16) {
+        struct {
+            float a[KC][TM + 4], b[KC][TN + 4];
+        } in;
+        float z[TM][TN + 1];
+    } sh;
+    auto& sa = sh.in.a;
+    auto& sb = sh.in.b;
+    auto& z = sh.z;
+    const int tid = threadIdx.x;
+    int lt = blockIdx.x, ji = 0;
+    if (w.jobs > 1 && lt >= w.job[0].tiles) lt -= w.job[0].tiles, ji = 1;
+    const SmallJob& g = w.job[ji];
+    const int slice = lt / (g.tm * g.tn), in = lt - slice * (g.tm * g.tn);
+    const int m0 = in % g.tm * TM, n0 = in / g.tm * TN;
+    const int k_lo = slice * g.kslice, k_hi = min(g.K, k_lo + g.kslice);
+
+    // A thread's elements of a chunk: where they lie, where they go, their k.  K-major
+    // operands: a warp takes 4 rows x 8 k (whole sectors), and with a pitch of 4
+    // mod 32 floats its transposed stores meet 32 banks.
+    using TA = std::conditional_t<P, float, T>;
+    const bool a_mn = P && g.a_mn;
+    const TA* pa[LA];
+    const T* pb[LB];
+    int oa[LA], ob[LB], ka[LA], kb[LB];
+#pragma unroll
+    for (int i = 0; i < LA; i++) {
+        const int x = tid + i * NT;
+        const int r = a_mn ? x % TM : (x & 3) + 4 * ((x >> 5) / (KC / 8));
+        const int k = a_mn ? x / TM : ((x >> 2) & 7) + 8 * ((x >> 5) % (KC / 8));
+        pa[i] = (const TA*)g.A + (a_mn ? (size_t)(k_lo + k) * g.lda + m0 + r : (size_t)(m0 + r) * g.lda + k_lo + k);
+        oa[i] = k * (TM + 4) + r;
+        ka[i] = m0 + r < g.M ? k_lo + k : INT_MAX;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; i++) {
+        const int x = tid + i * NT;
+        const int r = P ? x % TN : (x & 3) + 4 * ((x >> 5) / (KC / 8));
+        const int k = P ? x / TN : ((x >> 2) & 7) + 8 * ((x >> 5) % (KC / 8));
+        pb[i] = (const T*)g.B + (P ? (size_t)(k_lo + k) * g.ldb + n0 + r : (size_t)(n0 + r) * g.ldb + k_lo + k);
+        ob[i] = k * (TN + 4) + r;
+        kb[i] = n0 + r < g.N ? k_lo + k : INT_MAX;
+    }
+    const size_t step_a = a_mn ? (size_t)KC * g.lda : KC, step_b = P ? (size_t)KC * g.ldb : KC;
+    float ra[LA], rb[LB];
+    // the next chunk, whose first k is kd further than the first one's
+    auto fetch = [&](int kd) {
+#pragma unroll
+        for (int i = 0; i < LA; i++) {
+            ra[i] = ka[i] < k_hi - kd ? f32_of(*pa[i]) : 0.0f;
+            pa[i] += step_a;
+        }
+#pragma unroll
+        for (int i = 0; i < LB; i++) {
+            const bool in = kb[i] < k_hi - kd;
+            float v = in ? f32_of(*pb[i]) : 0.0f;
+            pb[i] += step_b;
+            if (P && g.bscale && in) {
+                // a row without a target counts as zeros, whatever it holds
+                const long long l = label_at(g.labels, g.index_bytes, kb[i] + kd);
+                v = l >= 0 && l < g.vocab ? v * g.bscale[kb[i] + kd] : 0.0f;
+            }
+            rb[i] = v;
+        }
+    };
+    const int grp = tid / GT, gt = tid % GT;
+    const int mr = gt % (TM / RM) * RM, nr = gt / (TM / RM) * RN;
+    float acc[RM][RN];
+#pragma unroll
+    for (int i = 0; i < RM; i++)
+#pragma unroll
+        for (int j = 0; j < RN; j++) acc[i][j] = 0.0f;
+    fetch(0);
+    for (int k0 = k_lo; k0 < k_hi; k0 += KC) {
+        __syncthreads();  // the last chunk has been read
+#pragma unroll
+        for (int i = 0; i < LA; i++) sa[0][oa[i]] = ra[i];
+#pragma unroll
+        for (int i = 0; i < LB; i++) sb[0][ob[i]] = rb[i];
+        __syncthreads();
+        if (k0 + KC < k_hi) fetch(k0 + KC - k_lo);
+#pragma unroll
+        for (int k = grp; k < KC; k += KG) {
+            float a[RM], b[RN];
+            const float4 a4 = *reinterpret_cast<const float4*>(&sa[k][mr]);
+            a[0] = a4.x, a[1] = a4.y, a[2] = a4.z, a[3] = a4.w;
+            if constexpr (RN == 4) {
+                const float4 b4 = *reinterpret_cast<const float4*>(&sb[k][nr]);
+                b[0] = b4.x, b[1] = b4.y, b[2] = b4.z, b[3] = b4.w;
+            } else {
+                const float2 b2 = *reinterpret_cast<const float2*>(&sb[k][nr]);
+                b[0] = b2.x, b[1] = b2.y;
+            }
+#pragma unroll
+            for (int i = 0; i < RM; i++)
+#pragma unroll
+                for (int j = 0; j < RN; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        }
+    }
+    // the groups' sums, in order
+    for (int q = 0; q < KG; q++) {
+        __syncthreads();
+        if (grp == q) {
+#pragma unroll
+            for (int i = 0; i < RM; i++)
+#pragma unroll
+                for (int j = 0; j < RN; j++)
+                    z[mr + i][nr + j] = q == 0 ? acc[i][j] : z[mr + i][nr + j] + acc[i][j];
+        }
+    }
+    __syncthreads();
+    if (g.kind == LSE) {
+        // a warp per row, a lane per column (and its 32nd next ones)
+        const int lane = tid & 31;
+        for (int r = tid >> 5; r < TM; r += NT / 32) {
+            const int row = m0 + r;
+            if (row >= g.M) break;
+            float v[TN / 32], m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < TN / 32; j++) {
+                const int c = lane + 32 * j;
+                v[j] = n0 + c < g.N ? z[r][c] : -INFINITY;
+                m = fmaxf(m, v[j]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float ref = m == -INFINITY ? 0.0f : m;  // as in chunk_lse
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < TN / 32; j++) s += ex2((v[j] - ref) * kLog2e);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const long long l = label_at(g.labels, g.index_bytes, row) - n0;
+            if (lane == 0) {
+                g.part_m[(size_t)(n0 / TN) * g.M + row] = m;
+                g.part_s[(size_t)(n0 / TN) * g.M + row] = s;
+                if (l >= 0 && l < TN && n0 + l < g.N) g.zlabel[row] = z[r][l];
+            }
+        }
+        return;
+    }
+    for (int x = tid; x < TM * TN; x += NT) {
+        const int row = m0 + x / TN, col = n0 + x % TN;
+        if (row >= g.M || col >= g.N) continue;
+        float v = z[x / TN][x % TN];
+        const size_t at = (size_t)row * g.N + col;
+        if (g.kind == GRAD) {
+            const long long l = label_at(g.labels, g.index_bytes, row);
+            v = ex2((v - g.lse[row]) * kLog2e) - (l == col ? 1.0f : 0.0f);
+            g.p[at] = l >= 0 && l < g.vocab ? v : 0.0f;
+        } else if (g.partial) {
+            ((float*)g.out)[(size_t)slice * g.M * g.N + at] = v;
+        } else {
+            if (g.dloss) {
+                const long long l = label_at(g.labels, g.index_bytes, row);
+                v = l >= 0 && l < g.vocab ? v * g.dloss[row] : 0.0f;
+            }
+            if constexpr (sizeof(T) == 2) ((bf16*)g.out)[at] = __float2bfloat16_rn(v);
+            else ((float*)g.out)[at] = v;
+        }
+    }
+}
+
+// out = the slices' partial products added in order, times the rows' dloss.
+struct SumJob {
+    const float* part;
+    void* out;
+    const float* dloss;   // or null
+    const float* factor;  // of all, or null
+    long long M, N;
+    int slices;           // 0: no such job
+};
+struct SumWork {
+    SumJob job[2];
+    const void* labels;
+    int index_bytes;
+    long long vocab;
+};
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_sum(const __grid_constant__ SumWork w) {
+    const SumJob& g = w.job[blockIdx.y];
+    const long long n = g.M * g.N;
+    if (g.slices == 0) return;
+    const float f = g.factor ? *g.factor : 1.0f;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < g.slices; s++) v += g.part[s * n + i];
+        if (g.dloss) {
+            const long long r = i / g.N, l = label_at(w.labels, w.index_bytes, r);
+            v = l >= 0 && l < w.vocab ? v * g.dloss[r] : 0.0f;
+        }
+        v *= f;
+        if constexpr (sizeof(T) == 2) ((bf16*)g.out)[i] = __float2bfloat16_rn(v);
+        else ((float*)g.out)[i] = v;
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -899,13 +1168,27 @@ int run_work(Ctx& c, const Work& w, int cg, bool six) {
     return six ? launch_work<1, true>(c, w) : launch_work<1, false>(c, w);
 }
 
-// Adds a job; jobs with a longer K come first.
-void add_job(Work& w, Job j, const CUtensorMap& a, const CUtensorMap& b, int cg) {
+// Slices of the K of an [M, N] product of few tiles, so that it does not run on a
+// few SMs while the others wait: each slice is at least 16 k-blocks.
+int out_slices(size_t M, size_t N, size_t K, int cg) {
+    const size_t t = (size_t)BT * cg, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
+    const size_t units = 148 / cg, kb = (K + BK - 1) / BK;
+    if (tiles * 2 > units || kb < 32) return 1;
+    return (int)std::min(units / tiles, kb / 16);
+}
+
+// The K of one of `slices` slices.
+int slice_k(size_t K, int slices) { return (int)(((K + slices - 1) / slices + BK - 1) / BK * BK); }
+
+// Adds a job; jobs with a longer K come first.  kslice: 0 for all of K.
+void add_job(Work& w, Job j, const CUtensorMap& a, const CUtensorMap& b, int cg, int kslice = 0) {
     const int t = BT * cg;
     j.tm = (j.M + t - 1) / t;
-    j.tiles = j.tm * ((j.N + t - 1) / t);  // below 2^31: the entry points check
+    j.plane = j.tm * ((j.N + t - 1) / t);  // below 2^31: the entry points check
+    j.kslice = kslice ? kslice : slice_k(j.K, 1);
+    j.tiles = j.plane * ((j.K + j.kslice - 1) / j.kslice);
     int at = w.jobs;
-    while (at > 0 && w.job[at - 1].K < j.K) {
+    while (at > 0 && w.job[at - 1].kslice < j.kslice) {
         w.job[at] = w.job[at - 1];
         w.map[2 * at] = w.map[2 * at - 2];
         w.map[2 * at + 1] = w.map[2 * at - 1];
@@ -929,7 +1212,8 @@ struct Plan {
     size_t dp;                // packed row length
     size_t vp, pieces;
     size_t seg;               // classes of one (maximum, sum) entry
-    size_t xp, sp, unit, wp[2], g[2], ldg, acc, pm, ps, zl, total;  // byte offsets; ldg in elements
+    size_t xp, sp, unit, wp[2], g[2], ldg, acc, px, pw, pm, ps, zl, total;  // byte offsets; ldg in elements
+    int sx, sw, ksx, ksw;     // slices of K of dx and of dw, and their length
 };
 
 constexpr size_t kPieceBytes = (size_t)128 << 20;
@@ -965,7 +1249,15 @@ Plan make_plan(const XentP& p, bool grad) {
         q.unit = take(4);
         for (int b = 0; b < 2; b++)
             q.g[b] = b < (int)q.pieces ? take((size_t)q.planes * 2 * p.n * q.ldg) : q.g[0];
-        q.acc = take(p.dt == BF16 && q.pieces > 1 ? (size_t)4 * p.n * p.dim : 0);
+        // (the last piece, if shorter, fills fewer slices of dx's sums)
+        const size_t most = std::min<size_t>(q.vp, p.vocab);
+        q.ksx = slice_k(most, out_slices(p.n, p.dim, most, q.cg));
+        q.sx = (int)((most + q.ksx - 1) / q.ksx);
+        q.ksw = slice_k(p.n, out_slices(most, p.dim, p.n, q.cg));
+        q.sw = (int)((p.n + q.ksw - 1) / q.ksw);
+        q.acc = take(p.dt == BF16 && q.pieces > 1 && q.sx == 1 ? (size_t)4 * p.n * p.dim : 0);
+        q.px = take(q.sx > 1 ? (size_t)4 * q.sx * p.n * p.dim : 0);
+        q.pw = take(q.sw > 1 ? (size_t)4 * q.sw * q.vp * p.dim : 0);
     } else {
         const size_t segs = (p.vocab + q.seg - 1) / q.seg;
         q.pm = take(4 * segs * p.n);
@@ -997,9 +1289,196 @@ bool in_place(const XentP& p, const void* t) {
     return p.dt == BF16 && p.dim % 8 == 0 && ((uintptr_t)t & 15) == 0;
 }
 
+void join(Ctx& c, const XentP& p, void* loss, void* lse, const float* pm, const float* ps,
+          const float* zl, size_t segs) {
+    k_xent_join<<<(p.n + 31) / 32, dim3(32, 32), 0, c.stream>>>((float*)loss, (float*)lse, pm, ps, zl,
+                                                                p.labels, p.index_bytes, p.vocab, p.n,
+                                                                (int)segs);
+    count_launch();
+}
+
+// ---- host: small problems --------------------------------------------------------
+
+bool is_small(const XentP& p) {
+    // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
+    return (unsigned long long)p.n * p.vocab <= kSmallF32 &&
+           (unsigned long long)p.n * p.vocab * p.dim <= (p.dt == F32 ? kSmallF32 : kSmallBf16);
+}
+
+// The tile: 64 x 64 where that gives every SM one, else 16 x 32.
+struct SmallTile {
+    int m, n;
+};
+SmallTile small_tile(size_t M, size_t N) {
+    const size_t big = ((M + 63) / 64) * ((N + 63) / 64);
+    return big >= 148 ? SmallTile{64, 64} : SmallTile{16, 32};
+}
+// Slices of a long K: each at least 1024 k, up to what gives about two tiles an SM.
+int small_slices(size_t tiles, size_t K) {
+    if (K <= 2048) return 1;
+    const size_t s = std::min((K + 1023) / 1024, (296 + tiles - 1) / tiles);
+    return (int)std::max<size_t>(s, 1);
+}
+size_t tiles_of(const SmallTile& t, size_t M, size_t N) {
+    return ((M + t.m - 1) / t.m) * ((N + t.n - 1) / t.n);
+}
+int slices_of(const SmallTile& t, size_t M, size_t N, size_t K) { return small_slices(tiles_of(t, M, N), K); }
+
+// The two products of the gradient use one tile, the smaller of what either would take.
+SmallTile small_out_tile(const XentP& p) {
+    const SmallTile a = small_tile(p.n, p.dim), b = small_tile(p.vocab, p.dim);
+    return tiles_of({64, 64}, p.n, p.dim) + tiles_of({64, 64}, p.vocab, p.dim) >= 148 && a.m == b.m ? a
+                                                                                                : SmallTile{16, 32};
+}
+
+void small_add(SmallWork& w, SmallJob j, const SmallTile& t, int slices) {
+    j.tm = (j.M + t.m - 1) / t.m;
+    j.tn = (j.N + t.n - 1) / t.n;
+    j.kslice = ((j.K + slices - 1) / slices + KC - 1) / KC * KC;
+    slices = (j.K + j.kslice - 1) / j.kslice;
+    j.tiles = j.tm * j.tn * slices;
+    w.job[w.jobs++] = j;
+    w.tiles += j.tiles;
+}
+
+template <typename T, bool P>
+void run_small_t(Ctx& c, const SmallWork& w, const SmallTile& t) {
+    if (t.m == 64) k_small<T, P, 64, 64, 4, 4, 2><<<w.tiles, 512, 0, c.stream>>>(w);
+    else k_small<T, P, 16, 32, 4, 2, 8><<<w.tiles, 512, 0, c.stream>>>(w);
+    count_launch();
+}
+void run_small(Ctx& c, int dt, const SmallWork& w, const SmallTile& t) {
+    const bool out = w.job[0].kind == OUT;
+    if (dt == F32) out ? run_small_t<float, true>(c, w, t) : run_small_t<float, false>(c, w, t);
+    else out ? run_small_t<bf16, true>(c, w, t) : run_small_t<bf16, false>(c, w, t);
+}
+
+// Workspace, in bytes: forward part_m, part_s [segments][n] and zlabel [n];
+// backward P [n][vocab] and the slices' products.
+struct SmallPlan {
+    SmallTile z, out;
+    size_t segs, pm, ps, zl, p, dx, dw, total;
+    int sx, sw;  // slices of dx, dw
+};
+SmallPlan small_plan(const XentP& p, bool grad) {
+    SmallPlan q{};
+    q.z = small_tile(p.n, p.vocab);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at += up(bytes, 256);
+        return o;
+    };
+    if (!grad) {
+        q.segs = (p.vocab + q.z.n - 1) / q.z.n;
+        q.pm = take(4 * q.segs * p.n);
+        q.ps = take(4 * q.segs * p.n);
+        q.zl = take((size_t)4 * p.n);
+    } else {
+        q.out = small_out_tile(p);
+        q.sx = slices_of(q.out, p.n, p.dim, p.vocab);
+        q.sw = slices_of(q.out, p.vocab, p.dim, p.n);
+        q.p = take((size_t)4 * p.n * p.vocab);
+        q.dx = take(q.sx > 1 ? (size_t)4 * q.sx * p.n * p.dim : 0);
+        q.dw = take(q.sw > 1 ? (size_t)4 * q.sw * p.vocab * p.dim : 0);
+    }
+    q.total = std::max<size_t>(at, 256);
+    return q;
+}
+
+SmallJob small_logits(const XentP& p, int kind) {
+    SmallJob j{};
+    j.kind = kind;
+    j.A = p.x;
+    j.B = p.w;
+    j.lda = j.ldb = p.dim;
+    j.M = (int)p.n;
+    j.N = (int)p.vocab;
+    j.K = (int)p.dim;
+    j.labels = p.labels;
+    j.index_bytes = p.index_bytes;
+    j.vocab = p.vocab;
+    return j;
+}
+
+void run_sum(Ctx& c, const XentP& p, SumWork& s) {
+    s.labels = p.labels;
+    s.index_bytes = p.index_bytes;
+    s.vocab = p.vocab;
+    size_t n = 0;
+    for (const SumJob& j : s.job) n = std::max(n, j.slices ? (size_t)(j.M * j.N) : 0);
+    const dim3 grid(grid_for(c, n, 256, 8), 2);
+    if (p.dt == F32) k_sum<float><<<grid, 256, 0, c.stream>>>(s);
+    else k_sum<bf16><<<grid, 256, 0, c.stream>>>(s);
+    count_launch();
+}
+
+int small_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
+    const SmallPlan q = small_plan(p, false);
+    char* base = (char*)ws;
+    SmallJob j = small_logits(p, LSE);
+    j.part_m = (float*)(base + q.pm);
+    j.part_s = (float*)(base + q.ps);
+    j.zlabel = (float*)(base + q.zl);
+    SmallWork w{};
+    small_add(w, j, q.z, 1);
+    run_small(c, p.dt, w, q.z);
+    join(c, p, loss, lse, j.part_m, j.part_s, j.zlabel, q.segs);
+    pdl_record_all(c);
+    return finish(c);
+}
+
+int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dloss, const void* lse,
+                    void* ws) {
+    const SmallPlan q = small_plan(p, true);
+    char* base = (char*)ws;
+    SmallJob z = small_logits(p, GRAD);
+    z.lse = (const float*)lse;
+    z.p = (float*)(base + q.p);
+    SmallWork w{};
+    small_add(w, z, q.z, 1);
+    run_small(c, p.dt, w, q.z);
+    SmallWork o{};
+    // dx = dloss (P w)
+    SmallJob j = small_logits(p, OUT);
+    j.A = z.p;
+    j.B = p.w;
+    j.lda = p.vocab;
+    j.ldb = p.dim;
+    j.N = (int)p.dim;
+    j.K = (int)p.vocab;
+    j.partial = q.sx > 1;
+    j.out = j.partial ? base + q.dx : dx;
+    j.dloss = (const float*)dloss;
+    small_add(o, j, q.out, q.sx);
+    const int sx = o.job[0].tiles / (o.job[0].tm * o.job[0].tn);
+    // dw = P^T (dloss x)
+    j.a_mn = 1;
+    j.B = p.x;
+    j.bscale = (const float*)dloss;
+    j.dloss = nullptr;
+    j.M = (int)p.vocab;
+    j.K = (int)p.n;
+    j.partial = q.sw > 1;
+    j.out = j.partial ? base + q.dw : dw;
+    small_add(o, j, q.out, q.sw);
+    const int sw = o.job[1].tiles / (o.job[1].tm * o.job[1].tn);
+    run_small(c, p.dt, o, q.out);
+    if (q.sx > 1 || q.sw > 1) {
+        SumWork s{};
+        if (q.sx > 1) s.job[0] = {(const float*)(base + q.dx), dx, (const float*)dloss, nullptr, p.n, p.dim, sx};
+        if (q.sw > 1) s.job[1] = {(const float*)(base + q.dw), dw, nullptr, nullptr, p.vocab, p.dim, sw};
+        run_sum(c, p, s);
+    }
+    pdl_record_all(c);
+    return finish(c);
+}
+
 }  // namespace
 
-size_t xent_workspace(const XentP& p, bool grad) { return make_plan(p, grad).total; }
+size_t xent_workspace(const XentP& p, bool grad) {
+    return is_small(p) ? small_plan(p, grad).total : make_plan(p, grad).total;
+}
 
 int xent_error() {
     int v = 0;
@@ -1016,6 +1495,7 @@ int xent_error() {
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     if (p.n == 0) return OK;
+    if (is_small(p)) return small_xent(c, p, loss, lse, ws);
     const Plan q = make_plan(p, false);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), xip = in_place(p, p.x);
@@ -1054,11 +1534,8 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
         add_job(w, g, ma, mb, q.cg);
         if ((rc = run_work(c, w, q.cg, q.planes == 3))) return rc;
     }
-    k_xent_join<<<(p.n + 31) / 32, dim3(32, 32), 0, c.stream>>>(
-        (float*)loss, (float*)lse, (const float*)(base + q.pm), (const float*)(base + q.ps),
-        (const float*)(base + q.zl), p.labels, p.index_bytes, p.vocab, p.n,
-        (int)((p.vocab + q.seg - 1) / q.seg));
-    count_launch();
+    join(c, p, loss, lse, (const float*)(base + q.pm), (const float*)(base + q.ps),
+         (const float*)(base + q.zl), (p.vocab + q.seg - 1) / q.seg);
     pdl_record_all(c);
     return finish(c);
 }
@@ -1069,6 +1546,7 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
         NXV_CK(cudaMemsetAsync(dw, 0, (size_t)p.vocab * p.dim * dtype_bytes(p.dt), c.stream));
         return finish(c);
     }
+    if (is_small(p)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
     const Plan q = make_plan(p, true);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), six = q.planes == 3;
@@ -1122,24 +1600,29 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             // the sum so far is f32
             o.M = (int)p.n;
             o.K = (int)nv;
-            o.out_bf16 = !six && last;
-            o.out = six || last ? dx : base + q.acc;
-            o.acc_in = first ? nullptr : six ? (const float*)dx : (const float*)(base + q.acc);
-            o.dloss = last ? (const float*)dloss : nullptr;
+            if (q.sx > 1) {  // each slice's sum over the pieces; added up at the end
+                o.out = base + q.px;
+                o.acc_in = first ? nullptr : (const float*)(base + q.px);
+            } else {
+                o.out_bf16 = !six && last;
+                o.out = six || last ? dx : base + q.acc;
+                o.acc_in = first ? nullptr : six ? (const float*)dx : (const float*)(base + q.acc);
+                o.dloss = last ? (const float*)dloss : nullptr;
+            }
             o.labels = p.labels;
             o.index_bytes = p.index_bytes;
             o.vocab = p.vocab;
-            add_job(w, o, mgk, mwn, q.cg);
+            add_job(w, o, mgk, mwn, q.cg, q.ksx);
             o.dloss = nullptr;
-            o.factor = unit;
+            o.factor = q.sw > 1 ? nullptr : unit;
             // dw = unit P^T (dloss x / unit): K runs over the tokens
             o.M = (int)nv;
             o.K = (int)p.n;
             o.a_mn = 1;
-            o.out_bf16 = !six;
-            o.out = (char*)dw + v0 * p.dim * es;
+            o.out_bf16 = !six && q.sw == 1;
+            o.out = q.sw > 1 ? (void*)(base + q.pw) : (char*)dw + v0 * p.dim * es;
             o.acc_in = nullptr;
-            add_job(w, o, mgm, mxn, q.cg);
+            add_job(w, o, mgm, mxn, q.cg, q.ksw);
         }
         if (i < q.pieces) {
             const size_t v0 = i * q.vp, nv = std::min<size_t>(q.vp, p.vocab - v0);
@@ -1155,6 +1638,15 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             add_job(w, z, mxk, mwk, q.cg);
         }
         if ((rc = run_work(c, w, q.cg, six))) return rc;
+        SumWork s{};
+        if (i > 0 && q.sw > 1) {
+            const size_t v0 = (i - 1) * q.vp, nv = std::min<size_t>(q.vp, p.vocab - v0);
+            s.job[0] = {(const float*)(base + q.pw), (char*)dw + v0 * p.dim * es, nullptr, unit,
+                        (long long)nv, p.dim, q.sw};
+        }
+        if (i == q.pieces && q.sx > 1)
+            s.job[1] = {(const float*)(base + q.px), dx, (const float*)dloss, nullptr, p.n, p.dim, q.sx};
+        if (s.job[0].slices || s.job[1].slices) run_sum(c, p, s);
     }
     pdl_record_all(c);
     return finish(c);
