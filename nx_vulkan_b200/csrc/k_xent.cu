@@ -761,27 +761,37 @@ k_pack(bf16* __restrict__ dst, const T* __restrict__ src, long long rows, int di
         }
         const T* sr = src + r * dim;
         bf16* dr = dst + r * ld;
-        for (int c = lane * 8; c < ld; c += 256) {
-            alignas(16) T in[8];
-            if (vec && c + 8 <= dim) {
+        constexpr int U = 4;  // groups of 8 whose loads are in flight together
+        for (int c0 = lane * 8; c0 < ld; c0 += 256 * U) {
+            alignas(16) T in[U][8];
 #pragma unroll
-                for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++)
-                    reinterpret_cast<uint4*>(in)[q] = reinterpret_cast<const uint4*>(sr + c)[q];
-            } else {
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + 256 * u;
+                if (vec && c + 8 <= dim) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) in[e] = c + e < dim ? sr[c + e] : T(0.0f);
-            }
-            alignas(16) bf16 o[PLANES][8];
+                    for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++)
+                        reinterpret_cast<uint4*>(in[u])[q] = reinterpret_cast<const uint4*>(sr + c)[q];
+                } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float v = (float)in[e];
-                if (scale) v = has ? v * f : 0.0f;
-                if constexpr (PLANES == 1) o[0][e] = __float2bfloat16_rn(v);
-                else split3(v, o[0][e], o[1][e], o[2][e]);
+                    for (int e = 0; e < 8; e++) in[u][e] = c + e < dim ? sr[c + e] : T(0.0f);
+                }
             }
 #pragma unroll
-            for (int k = 0; k < PLANES; k++)
-                *reinterpret_cast<uint4*>(dr + k * plane + c) = *reinterpret_cast<uint4*>(o[k]);
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + 256 * u;
+                if (c >= ld) break;
+                alignas(16) bf16 o[PLANES][8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float v = (float)in[u][e];
+                    if (scale) v = has ? v * f : 0.0f;
+                    if constexpr (PLANES == 1) o[0][e] = __float2bfloat16_rn(v);
+                    else split3(v, o[0][e], o[1][e], o[2][e]);
+                }
+#pragma unroll
+                for (int k = 0; k < PLANES; k++)
+                    *reinterpret_cast<uint4*>(dr + k * plane + c) = *reinterpret_cast<uint4*>(o[k]);
+            }
         }
     }
 }
@@ -1271,7 +1281,7 @@ Plan make_plan(const XentP& p, bool grad) {
 // scale: the factors of the rows (dloss), in units of *unit; or null.
 void pack(Ctx& c, const XentP& p, bf16* dst, const void* src, size_t rows, int ld,
           const void* scale, const float* unit) {
-    const unsigned grid = grid_for(c, rows, 8, 8);
+    const unsigned grid = grid_for(c, rows, 8, 16);
     const bool vec = ((uintptr_t)src & 15) == 0 && p.dim * dtype_bytes(p.dt) % 16 == 0;
     if (p.dt == F32)
         k_pack<float, 3><<<grid, 256, 0, c.stream>>>(dst, (const float*)src, rows, p.dim, ld, vec,
@@ -1301,8 +1311,8 @@ void join(Ctx& c, const XentP& p, void* loss, void* lse, const float* pm, const 
 
 bool is_small(const XentP& p) {
     // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
-    return (unsigned long long)p.n * p.vocab <= kSmallF32 &&
-           (unsigned long long)p.n * p.vocab * p.dim <= (p.dt == F32 ? kSmallF32 : kSmallBf16);
+    const unsigned long long n = up(p.n, 16);  // whole row tiles
+    return n * p.vocab <= kSmallF32 && n * p.vocab * p.dim <= (p.dt == F32 ? kSmallF32 : kSmallBf16);
 }
 
 // The tile: 64 x 64 where that gives every SM one, else 16 x 32.
