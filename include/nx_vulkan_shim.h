@@ -253,13 +253,14 @@ int nxv_random_f64(void* out, unsigned long n, unsigned int seed, unsigned int d
 /* Layer norm of every row of x [rows, cols]: mean, rstd = 1 / sqrt(var + eps)
  * (var = mean of (x - mean)^2), y = (x - mean) rstd gamma + beta.  gamma, beta
  * [cols] and y have x's type; mean and rstd [rows] are f32 (f64 for f64) and
- * all arithmetic is in their type.  y may be x.  cols > 0, eps >= 0.
+ * all arithmetic is in their type.  y may be x.  1 <= cols <= 2^28, eps >= 0.
  * spv: layer_norm.spv. */
 int nxv_layer_norm(void* y, void* mean, void* rstd,
                    void* x, void* gamma, void* beta,
                    unsigned int rows, unsigned int cols, double eps,
                    unsigned int dtype, const char* spv_path);
 
+/* 0 bytes for arguments that the call would refuse. */
 unsigned long nxv_layer_norm_grad_workspace(unsigned int rows, unsigned int cols,
                                             unsigned int dtype);
 
@@ -586,6 +587,10 @@ int nxv_set_device(int id);
  * cudaStream_t (passed as void*); NULL restores the library's own stream.
  * To use the legacy default stream pass cudaStreamLegacy ((void*)1). */
 int nxv_set_stream(void* cuda_stream);
+
+/* 1 while the thread's stream for the current device is being captured into a
+ * CUDA graph, else 0; negative on error. */
+int nxv_stream_capturing(void);
 
 /* Wait for all work queued on the current device.  0, or -4 with the CUDA
  * error that a kernel raised. */

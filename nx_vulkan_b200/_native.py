@@ -88,6 +88,7 @@ SIGNATURES: dict[str, tuple] = {
     "nxv_init_devices": (C.c_int, [intp, C.c_int]),
     "nxv_set_device": (C.c_int, [C.c_int]),
     "nxv_set_stream": (C.c_int, [vp]),
+    "nxv_stream_capturing": (C.c_int, []),
     "nxv_synchronize": (C.c_int, []),
     "nxv_buf_copy_2d": (C.c_int, [vp, ul, ul, vp, ul, ul, ul, ul]),
     "nxv_buf_wrap": (vp, [vp, ul]),

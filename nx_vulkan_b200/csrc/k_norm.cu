@@ -309,6 +309,13 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
     constexpr int V = kV<T>, N = kN<T>, NP = kP<T>;
     __shared__ A red[2][32];
     const unsigned t = threadIdx.x, G = blockDim.x, lane = t & 31, warps = G >> 5;
+    auto total = [&](A v, int which) {
+        v = warp_sum(v);
+        if (warps == 1) return v;
+        if (lane == 0) red[which][t >> 5] = v;
+        __syncthreads();
+        return warp_sum(lane < warps ? red[which][lane] : A(0));
+    };
     const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= rows) return;  // whole warps: blockDim.y > 1 has no barriers
     const T* xr = x + row * cols;
@@ -318,13 +325,6 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
     for (int k = 0; k < NV; k++) raw_load<T, AL>(p[k], xr, t + k * G, cols, edge);
 #pragma unroll
     for (int k = 0; k < NV; k++) realign<T, AL>(p[k], xr, t + k * G, cols, edge, lane, 32);
-    auto total = [&](A v, int which) {
-        v = warp_sum(v);
-        if (warps == 1) return v;
-        if (lane == 0) red[which][t >> 5] = v;
-        __syncthreads();
-        return warp_sum(lane < warps ? red[which][lane] : A(0));
-    };
     W s = vset(A(0), (W*)0);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -774,7 +774,11 @@ void fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, c
              : k <= 4 ? k_norm_fwd<T, 4, AL>
              : k <= 8 ? k_norm_fwd<T, 8, AL>
                       : k_norm_fwd<T, 16, AL>;
-    f<<<(rows + ty - 1) / ty, dim3(tx, ty), 0, c.stream>>>(y, mean, rstd, x, g, b, rows, cols, eps);
+    for (size_t r0 = 0; r0 < rows; r0 += 1u << 30) {  // the grid's limit
+        const unsigned n = (unsigned)std::min<size_t>(rows - r0, 1u << 30);
+        f<<<(n + ty - 1) / ty, dim3(tx, ty), 0, c.stream>>>(y + r0 * cols, mean + r0, rstd + r0, x + r0 * cols, g,
+                                                          b, n, cols, eps);
+    }
 }
 
 template <typename T>

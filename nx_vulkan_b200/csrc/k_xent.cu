@@ -39,6 +39,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace nxv {
@@ -57,6 +58,7 @@ constexpr int SMEM = ST * ST_BYTES + 1024 + 256;
 constexpr int kThreads = 384;  // producer of A, MMA issuer, allocator, producer of B, 8 epilogue warps
 
 __device__ int g_xent_error;
+std::atomic<bool> g_xent_ran{false};  // a kernel that may set it was launched since the last look
 
 // ---- PTX ----------------------------------------------------------------------
 
@@ -1174,6 +1176,7 @@ int launch_work(Ctx& c, const Work& w) {
 }
 
 int run_work(Ctx& c, const Work& w, int cg, bool six) {
+    g_xent_ran.store(true);
     if (cg == 2) return six ? launch_work<2, true>(c, w) : launch_work<2, false>(c, w);
     return six ? launch_work<1, true>(c, w) : launch_work<1, false>(c, w);
 }
@@ -1226,7 +1229,7 @@ struct Plan {
     int sx, sw, ksx, ksw;     // slices of K of dx and of dw, and their length
 };
 
-constexpr size_t kPieceBytes = (size_t)128 << 20;
+constexpr size_t kPieceBytes = (size_t)256 << 20;
 constexpr size_t kTile = 2 * BT;
 
 Plan make_plan(const XentP& p, bool grad) {
@@ -1491,6 +1494,7 @@ size_t xent_workspace(const XentP& p, bool grad) {
 }
 
 int xent_error() {
+    if (!g_xent_ran.exchange(false)) return 0;
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_xent_error, sizeof(int)) != cudaSuccess) {
         cudaGetLastError();

@@ -539,6 +539,8 @@ int get_workspace(Ctx& c, void* handle, size_t bytes, const char* op, void** out
 
 }  // namespace
 
+constexpr unsigned kMaxNormCols = 1u << 28;  // 32-bit byte offsets within a row
+
 int nxv_layer_norm(void* y, void* mean, void* rstd, void* x, void* gamma, void* beta,
                    unsigned int rows, unsigned int cols, double eps, unsigned int dtype,
                    const char* spv_path) {
@@ -546,8 +548,8 @@ int nxv_layer_norm(void* y, void* mean, void* rstd, void* x, void* gamma, void* 
     std::string k = spv_base(spv_path);
     if (k != "layer_norm.spv") return bad_kernel(k);
     if (int rc = dtype_ok(dtype, BF16, "layer_norm")) return rc;
-    if (cols == 0 || !(eps >= 0.0 && eps < HUGE_VAL)) {
-        set_error("layer_norm: cols %u must be positive, eps %g finite and not negative", cols, eps);
+    if (cols == 0 || cols > kMaxNormCols || !(eps >= 0.0 && eps < HUGE_VAL)) {
+        set_error("layer_norm: cols %u out of range 1..2^28, or eps %g not finite or negative", cols, eps);
         return E_ARG;
     }
     BEGIN(y, mean, rstd, x, gamma, beta);
@@ -563,7 +565,7 @@ int nxv_layer_norm(void* y, void* mean, void* rstd, void* x, void* gamma, void* 
 
 unsigned long nxv_layer_norm_grad_workspace(unsigned int rows, unsigned int cols,
                                             unsigned int dtype) {
-    return dtype > BF16 ? 0 : norm_grad_workspace(rows, cols, (int)dtype);
+    return dtype > BF16 || cols == 0 || cols > kMaxNormCols ? 0 : norm_grad_workspace(rows, cols, (int)dtype);
 }
 
 int nxv_layer_norm_grad(void* dx, void* dgamma, void* dbeta, void* workspace, void* dy, void* x,
@@ -574,8 +576,8 @@ int nxv_layer_norm_grad(void* dx, void* dgamma, void* dbeta, void* workspace, vo
     std::string k = spv_base(spv_path);
     if (k != "layer_norm_grad.spv") return bad_kernel(k);
     if (int rc = dtype_ok(dtype, BF16, "layer_norm_grad")) return rc;
-    if (cols == 0) {
-        set_error("layer_norm_grad: cols must be positive");
+    if (cols == 0 || cols > kMaxNormCols) {
+        set_error("layer_norm_grad: cols %u out of range 1..2^28", cols);
         return E_ARG;
     }
     BEGIN(dx, dgamma, dbeta, workspace, dy, x, gamma, mean, rstd);
@@ -964,6 +966,11 @@ int nxv_leapfrog_logreg_f64_batched(void* q_chain, void* p_chain, void* grad_cha
 int nxv_init_devices(const int* ids, int n) { return init_devices(ids, n); }
 int nxv_set_device(int id) { return set_current(id); }
 int nxv_set_stream(void* cuda_stream) { return set_stream((cudaStream_t)cuda_stream); }
+
+int nxv_stream_capturing(void) {
+    BEGIN();
+    return capturing(c) ? 1 : 0;
+}
 
 int nxv_synchronize(void) {
     BEGIN();

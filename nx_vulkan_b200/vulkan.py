@@ -634,8 +634,8 @@ def fused_chain_imm(a, operands: Sequence, ops: Sequence, *, dtype="f32"):
 # wrap_tensor) in the order of the result; `workspace=` a buffer of the size
 # that the matching *_workspace function gives, for calls that may overlap with
 # others of the stream or are captured into a CUDA graph.  A captured call
-# needs both: memory of the pool may be handed to another call while the graph
-# still uses it.
+# needs both and is refused without: memory of the pool could be handed to
+# another call while the graph still uses it.
 
 DTYPES = {"f32": 0, "f64": 1, "bf16": 2}
 _DTYPE_BYTES = {"f32": 4, "f64": 8, "bf16": 2}
@@ -644,11 +644,17 @@ _DTYPE_BYTES = {"f32": 4, "f64": 8, "bf16": 2}
 def _out_buffers(out, sizes):
     """The caller's output buffers (checked) or new ones; (buffers, None) or (None, error)."""
     if out is None:
+        # a graph would keep memory that goes back to the pool
+        if _lib().nxv_stream_capturing() == 1:
+            return None, (ERROR, "alloc_failed")
         bufs = [_alloc(n) for n in sizes]
         return (None, (ERROR, "alloc_failed")) if None in bufs else (bufs, None)
-    if len(out) != len(sizes) or any(o.n_bytes < n for o, n in zip(out, sizes)):
+    if len(out) != len(sizes):
         return None, (ERROR, "size_mismatch")
-    return list(out), None
+    for o, n in zip(out, sizes):
+        if o.n_bytes < n:
+            return None, (ERROR, "size_mismatch")
+    return out, None
 
 
 def _dispatch_bufs(bufs, given, rc):
@@ -657,8 +663,7 @@ def _dispatch_bufs(bufs, given, rc):
     return (OK, bufs[0] if len(bufs) == 1 else tuple(bufs)) if rc == 0 else (ERROR, "dispatch_failed")
 
 
-def _u32(*vals):
-    return all(0 <= v < 1 << 32 for v in vals)
+_U32 = (1 << 32) - 1
 
 
 def layer_norm(x, gamma, beta, rows, cols, eps=1e-5, dtype="f32", out=None):
@@ -666,7 +671,7 @@ def layer_norm(x, gamma, beta, rows, cols, eps=1e-5, dtype="f32", out=None):
 
     Returns y (x's type) and every row's mean and 1 / sqrt(var + eps) (f32; f64
     for f64).  y may be x (out=)."""
-    if dtype not in DTYPES or not _u32(rows, cols) or cols == 0 or not 0.0 <= eps < math.inf:
+    if dtype not in DTYPES or not (0 <= rows <= _U32 and 0 < cols <= 1 << 28) or not 0.0 <= eps < math.inf:
         return (ERROR, "bad_op")
     es, st = _DTYPE_BYTES[dtype], 8 if dtype == "f64" else 4
     if x.n_bytes != rows * cols * es or gamma.n_bytes != cols * es or beta.n_bytes != cols * es:
@@ -688,7 +693,7 @@ def layer_norm_grad_workspace(rows, cols, dtype="f32") -> int:
 def layer_norm_grad(dy, x, gamma, mean, rstd, rows, cols, dtype="f32", out=None, workspace=None):
     """Gradients of layer_norm from dy [rows, cols] and the forward call's mean
     and rstd: dx [rows, cols] (may be dy or x, out=), dgamma and dbeta [cols]."""
-    if dtype not in DTYPES or not _u32(rows, cols) or cols == 0:
+    if dtype not in DTYPES or not (0 <= rows <= _U32 and 0 < cols <= 1 << 28):
         return (ERROR, "bad_op")
     es, st = _DTYPE_BYTES[dtype], 8 if dtype == "f64" else 4
     n = rows * cols * es
@@ -710,7 +715,7 @@ def dropout(x, p, seed, offset=0, dtype="f32", out=None):
 
     The mask is never stored: the gradient is dropout(dy, p, seed, offset).
     `out=` may be x."""
-    if dtype not in DTYPES or not 0.0 <= p <= 1.0 or not _u32(seed):
+    if dtype not in DTYPES or not 0.0 <= p <= 1.0 or not 0 <= seed <= _U32:
         return (ERROR, "bad_op")
     es = _DTYPE_BYTES[dtype]
     n = x.n_bytes // es
@@ -718,17 +723,18 @@ def dropout(x, p, seed, offset=0, dtype="f32", out=None):
         return (ERROR, "size_mismatch")
     if offset < 0 or offset + n > 1 << 32:
         return (ERROR, "bad_op")
-    o = _out_buffer(out, x.n_bytes)
-    if o is None:
-        return (ERROR, "alloc_failed" if out is None else "size_mismatch")
-    rc = _lib().nxv_dropout(o.handle, x.handle, n, p, seed, offset, DTYPES[dtype], b"dropout.spv")
-    return _dispatch_into(o, out, rc)
+    bufs, err = _out_buffers(None if out is None else (out,), (x.n_bytes,))
+    if err:
+        return err
+    rc = _lib().nxv_dropout(bufs[0].handle, x.handle, n, p, seed, offset, DTYPES[dtype],
+                            b"dropout.spv")
+    return _dispatch_bufs(bufs, out, rc)
 
 
 def _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes):
-    if dtype not in ("f32", "bf16") or index_bytes not in (4, 8) or not _u32(n, vocab, dim):
+    if dtype not in ("f32", "bf16") or index_bytes not in (4, 8):
         return (ERROR, "bad_op")
-    if vocab == 0 or dim == 0:
+    if not (0 <= n <= _U32 and 0 < vocab <= _U32 and 0 < dim <= _U32):
         return (ERROR, "bad_op")
     es = _DTYPE_BYTES[dtype]
     if (x.n_bytes != n * dim * es or w.n_bytes != vocab * dim * es

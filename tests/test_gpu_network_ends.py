@@ -684,8 +684,11 @@ def test_a_capture_needs_its_own_workspace(nxv, torch):
         said = _native.last_error()
         q = nxv.linear_cross_entropy(hs[1], hs[2], hs[3], 20, 30, 16, dtype="bf16", out=(hs[7], hs[4]))
         k = nxv.layer_norm_grad(hs[1], hs[1], hs[1], hs[4], hs[4], 20, 16, dtype="bf16", out=(hs[5], hs[6], hs[7]))
+        # ... and its own outputs
+        o = [nxv.dropout(hs[1], 0.5, 1), nxv.linear_cross_entropy(hs[1], hs[2], hs[3], 20, 30, 16, dtype="bf16")]
         lib.nxv_set_stream(1)
         loss.zero_()  # the graph is not empty
+    assert o[0] == o[1] == ("error", "alloc_failed")
     assert r == ("error", "dispatch_failed") and "workspace" in said
     assert q == ("error", "dispatch_failed") and k[0] == "error"
 

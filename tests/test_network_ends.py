@@ -57,9 +57,10 @@ def test_values_out_of_range(lib):
     nan, inf = float("nan"), float("inf")
     ln = lambda rows, cols, eps, dt: lib.nxv_layer_norm(*[P] * 6, rows, cols, eps, dt,  # noqa: E731
                                                         b"layer_norm.spv")
-    for args in ((2, 0, 1e-5, 0), (2, 4, -1e-5, 0), (2, 4, nan, 0), (2, 4, inf, 0), (2, 4, 1e-5, 3)):
+    for args in ((2, 0, 1e-5, 0), (2, (1 << 28) + 1, 1e-5, 0), (2, 4, -1e-5, 0), (2, 4, nan, 0), (2, 4, inf, 0), (2, 4, 1e-5, 3)):
         assert ln(*args) == -3
     assert lib.nxv_layer_norm_grad(*[P] * 9, 2, 0, 0, b"layer_norm_grad.spv") == -3
+    assert lib.nxv_layer_norm_grad(*[P] * 9, 2, (1 << 28) + 1, 0, b"layer_norm_grad.spv") == -3
     assert lib.nxv_layer_norm_grad(*[P] * 9, 2, 4, 3, b"layer_norm_grad.spv") == -3
     for n, p, off, dt in ((4, -0.1, 0, 0), (4, 1.1, 0, 0), (4, nan, 0, 0), (4, 0.1, 0, 3),
                           ((1 << 32) + 1, 0.1, 0, 0), (4, 0.1, (1 << 32) - 3, 0),
