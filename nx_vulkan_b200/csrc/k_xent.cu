@@ -866,20 +866,59 @@ k_xent_join(float* __restrict__ loss, float* __restrict__ lse, const float* __re
     }
 }
 
+// The same for few rows: a CTA per row.
+__global__ void __launch_bounds__(256)
+k_xent_join_row(float* __restrict__ loss, float* __restrict__ lse, const float* __restrict__ part_m,
+                const float* __restrict__ part_s, const float* __restrict__ zlabel,
+                const void* labels, int index_bytes, long long vocab, long long n, int segs) {
+    __shared__ float sh[8];
+    const long long row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < segs; t += 256) m = fmaxf(m, part_m[(size_t)t * n + row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) sh[warp] = m;
+    __syncthreads();
+    m = sh[lane & 7];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < segs; t += 256) {
+        const float om = part_m[(size_t)t * n + row], os = part_s[(size_t)t * n + row];
+        s += om == -INFINITY ? os : os * ex2((om - ref) * kLog2e);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    __syncthreads();  // the maxima have been read
+    if (lane == 0) sh[warp] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = ((sh[0] + sh[1]) + (sh[2] + sh[3])) + ((sh[4] + sh[5]) + (sh[6] + sh[7]));
+        const float ls = m == -INFINITY ? NAN : logf(s);  // as k_xent_join
+        lse[row] = m + ls;
+        const long long l = label_at(labels, index_bytes, row);
+        loss[row] = l >= 0 && l < vocab ? (m - zlabel[row]) + ls : 0.0f;
+    }
+}
+
 // ---- small problems ---------------------------------------------------------------
 //
 // For few multiply-adds per product the packing, the tensor maps and the
 // pipeline's start cost more than the products.  k_small does them with f32 FMAs straight from the tensors, a
 // TM x TN tile a CTA, KG groups of its threads taking every KG-th k of a chunk,
-// added in order at the end: two launches forward (tiles, join) and two or three
-// backward (P, both products, and where a long K is cut into slices, their sum).
+// added in order at the end: two launches forward (tiles, join) and two to four
+// backward (P, both products, in one launch where they take the same tile, and
+// where a long K is cut into slices, their sum).
 
-// The limits, from both paths' times, loss / gradient in us, small path first:
-// f32 16 x 200 x 100 10 / 15 and 23 / 39, 64 x 1001 x 1000 23 / 60 and 42 / 81, 512^3
-// 33 / 101 and 35 / 70; bf16 16 x 200 x 104 10 / 15 and 11 / 23, 64 x 1001 x 1000
-// 23 / 60 and 15 / 31.
-constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;
-constexpr int KC = 64;  // k of a chunk
+// The limits on n vocab dim, from both paths' times in us, this one's first.
+// Loss f32: 64 x 1001 x 1000 19 and 42, 512^3 33 and 35; bf16: 16 x 200 x 100 10 and 17,
+// 64 x 1001 x 1000 23 and 15.  Gradient f32: 16 x 200 x 100 15 and 39, 256 x 512 x 512
+// 80 and 66; bf16: 16 x 200 x 100 15 and 40, 64 x 300 x 400 27 and 28.
+constexpr unsigned long long kSmallLoss = 1ull << 26, kSmallGrad = 1ull << 24, kSmallBf16 = 1ull << 22;
+constexpr int KSTEP = 128;  // slices of K are multiples of this, and of a tile's chunk KC
 
 struct SmallJob {
     int kind;
@@ -889,7 +928,7 @@ struct SmallJob {
     long long lda, ldb;
     int M, N, K;
     int tm, tn, tiles;    // tiles of one slice, and of all
-    int kslice;           // the k of a slice, a multiple of KC
+    int kslice;           // the k of a slice
     const float* bscale;  // OUT: a factor of B's row k, 0 without a target; or null
     // as in Job
     float *part_m, *part_s, *zlabel;
@@ -910,22 +949,22 @@ __device__ __forceinline__ float f32_of(float v) { return v; }
 __device__ __forceinline__ float f32_of(bf16 v) { return __bfloat162float(v); }
 
 // P: OUT jobs; else LSE or GRAD.
-template <typename T, bool P, int TM, int TN, int RM, int RN, int KG>
+template <typename T, bool P, int TM, int TN, int RM, int RN, int KG, int KC>
 __global__ void __launch_bounds__(TM / RM * (TN / RN) * KG)
 k_small(const __grid_constant__ SmallWork w) {
     constexpr int GT = TM / RM * (TN / RN), NT = GT * KG;  // threads of a group, of the CTA
     constexpr int LA = TM * KC / NT, LB = TN * KC / NT;
     // the finished tile takes the place of the last chunk
-    static_assert(RM == 4 && (RN == 2 || RN == 4) && KC % KG == 0, "tile");
+    static_assert(RM == 4 && (RN == 2 || RN == 4) && KC % KG == 0 && KSTEP % KC == 0, "tile");
     __shared__ union alignas(16) {
         struct {
             float a[KC][TM + 4], b[KC][TN + 4];
         } in;
-        float z[TM][TN + 1];
+        float z[KG][TM][TN];
     } sh;
     auto& sa = sh.in.a;
     auto& sb = sh.in.b;
-    auto& z = sh.z;
+    auto& z = sh.z[0];
     const int tid = threadIdx.x;
     int lt = blockIdx.x, ji = 0;
     if (w.jobs > 1 && lt >= w.job[0].tiles) lt -= w.job[0].tiles, ji = 1;
@@ -1017,15 +1056,17 @@ k_small(const __grid_constant__ SmallWork w) {
         }
     }
     // the groups' sums, in order
-    for (int q = 0; q < KG; q++) {
-        __syncthreads();
-        if (grp == q) {
+    __syncthreads();
 #pragma unroll
-            for (int i = 0; i < RM; i++)
+    for (int i = 0; i < RM; i++)
 #pragma unroll
-                for (int j = 0; j < RN; j++)
-                    z[mr + i][nr + j] = q == 0 ? acc[i][j] : z[mr + i][nr + j] + acc[i][j];
-        }
+        for (int j = 0; j < RN; j++) sh.z[grp][mr + i][nr + j] = acc[i][j];
+    __syncthreads();
+    for (int x = tid; x < TM * TN; x += NT) {
+        float v = sh.z[0][x / TN][x % TN];
+#pragma unroll
+        for (int q = 1; q < KG; q++) v += sh.z[q][x / TN][x % TN];
+        z[x / TN][x % TN] = v;  // this thread's own element
     }
     __syncthreads();
     if (g.kind == LSE) {
@@ -1304,50 +1345,47 @@ bool in_place(const XentP& p, const void* t) {
 
 void join(Ctx& c, const XentP& p, void* loss, void* lse, const float* pm, const float* ps,
           const float* zl, size_t segs) {
-    k_xent_join<<<(p.n + 31) / 32, dim3(32, 32), 0, c.stream>>>((float*)loss, (float*)lse, pm, ps, zl,
-                                                                p.labels, p.index_bytes, p.vocab, p.n,
-                                                                (int)segs);
+    if (p.n <= 512)
+        k_xent_join_row<<<p.n, 256, 0, c.stream>>>((float*)loss, (float*)lse, pm, ps, zl, p.labels,
+                                                   p.index_bytes, p.vocab, p.n, (int)segs);
+    else
+        k_xent_join<<<(p.n + 31) / 32, dim3(32, 32), 0, c.stream>>>((float*)loss, (float*)lse, pm, ps,
+                                                                    zl, p.labels, p.index_bytes,
+                                                                    p.vocab, p.n, (int)segs);
     count_launch();
 }
 
 // ---- host: small problems --------------------------------------------------------
 
-bool is_small(const XentP& p) {
-    // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
+bool is_small(const XentP& p, bool grad) {
+    const unsigned long long most = p.dt == BF16 ? kSmallBf16 : grad ? kSmallGrad : kSmallLoss;
     const unsigned long long n = up(p.n, 16);  // whole row tiles
-    return n * p.vocab <= kSmallF32 && n * p.vocab * p.dim <= (p.dt == F32 ? kSmallF32 : kSmallBf16);
+    // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
+    return n * p.vocab <= most && n * p.vocab * p.dim <= most;
 }
 
-// The tile: 64 x 64 where that gives every SM one, else 16 x 32.
+// The tile: 64 x 64 where that gives every SM one and is not mostly empty, else 16 x 32.
 struct SmallTile {
     int m, n;
 };
 SmallTile small_tile(size_t M, size_t N) {
     const size_t big = ((M + 63) / 64) * ((N + 63) / 64);
-    return big >= 148 ? SmallTile{64, 64} : SmallTile{16, 32};
+    return M > 32 && N > 32 && big >= 148 ? SmallTile{64, 64} : SmallTile{16, 32};
 }
-// Slices of a long K: each at least 1024 k, up to what gives about two tiles an SM.
+// Slices of a long K where the tiles leave SMs idle: each at least 256 k.
 int small_slices(size_t tiles, size_t K) {
-    if (K <= 2048) return 1;
-    const size_t s = std::min((K + 1023) / 1024, (296 + tiles - 1) / tiles);
-    return (int)std::max<size_t>(s, 1);
+    if (K < 512 || tiles * 2 > 148) return 1;
+    return (int)std::min(K / 256, 148 / tiles);
 }
 size_t tiles_of(const SmallTile& t, size_t M, size_t N) {
     return ((M + t.m - 1) / t.m) * ((N + t.n - 1) / t.n);
 }
 int slices_of(const SmallTile& t, size_t M, size_t N, size_t K) { return small_slices(tiles_of(t, M, N), K); }
 
-// The two products of the gradient use one tile, the smaller of what either would take.
-SmallTile small_out_tile(const XentP& p) {
-    const SmallTile a = small_tile(p.n, p.dim), b = small_tile(p.vocab, p.dim);
-    return tiles_of({64, 64}, p.n, p.dim) + tiles_of({64, 64}, p.vocab, p.dim) >= 148 && a.m == b.m ? a
-                                                                                                : SmallTile{16, 32};
-}
-
 void small_add(SmallWork& w, SmallJob j, const SmallTile& t, int slices) {
     j.tm = (j.M + t.m - 1) / t.m;
     j.tn = (j.N + t.n - 1) / t.n;
-    j.kslice = ((j.K + slices - 1) / slices + KC - 1) / KC * KC;
+    j.kslice = ((j.K + slices - 1) / slices + KSTEP - 1) / KSTEP * KSTEP;
     slices = (j.K + j.kslice - 1) / j.kslice;
     j.tiles = j.tm * j.tn * slices;
     w.job[w.jobs++] = j;
@@ -1356,8 +1394,10 @@ void small_add(SmallWork& w, SmallJob j, const SmallTile& t, int slices) {
 
 template <typename T, bool P>
 void run_small_t(Ctx& c, const SmallWork& w, const SmallTile& t) {
-    if (t.m == 64) k_small<T, P, 64, 64, 4, 4, 2><<<w.tiles, 512, 0, c.stream>>>(w);
-    else k_small<T, P, 16, 32, 4, 2, 8><<<w.tiles, 512, 0, c.stream>>>(w);
+    if (t.m == 64) k_small<T, P, 64, 64, 4, 4, 2, 64><<<w.tiles, 512, 0, c.stream>>>(w);
+    else if (!P && w.job[0].K >= 512)  // a longer chunk hides more of its loads' latency
+        k_small<T, P, 16, 32, 4, 2, 8, 128><<<w.tiles, 512, 0, c.stream>>>(w);
+    else k_small<T, P, 16, 32, 4, 2, 8, 64><<<w.tiles, 512, 0, c.stream>>>(w);
     count_launch();
 }
 void run_small(Ctx& c, int dt, const SmallWork& w, const SmallTile& t) {
@@ -1369,7 +1409,7 @@ void run_small(Ctx& c, int dt, const SmallWork& w, const SmallTile& t) {
 // Workspace, in bytes: forward part_m, part_s [segments][n] and zlabel [n];
 // backward P [n][vocab] and the slices' products.
 struct SmallPlan {
-    SmallTile z, out;
+    SmallTile z, tx, tw;  // of the logits, of dx, of dw
     size_t segs, pm, ps, zl, p, dx, dw, total;
     int sx, sw;  // slices of dx, dw
 };
@@ -1388,9 +1428,10 @@ SmallPlan small_plan(const XentP& p, bool grad) {
         q.ps = take(4 * q.segs * p.n);
         q.zl = take((size_t)4 * p.n);
     } else {
-        q.out = small_out_tile(p);
-        q.sx = slices_of(q.out, p.n, p.dim, p.vocab);
-        q.sw = slices_of(q.out, p.vocab, p.dim, p.n);
+        q.tx = small_tile(p.n, p.dim);
+        q.tw = small_tile(p.vocab, p.dim);
+        q.sx = slices_of(q.tx, p.n, p.dim, p.vocab);
+        q.sw = slices_of(q.tw, p.vocab, p.dim, p.n);
         q.p = take((size_t)4 * p.n * p.vocab);
         q.dx = take(q.sx > 1 ? (size_t)4 * q.sx * p.n * p.dim : 0);
         q.dw = take(q.sw > 1 ? (size_t)4 * q.sw * p.vocab * p.dim : 0);
@@ -1463,8 +1504,12 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
     j.partial = q.sx > 1;
     j.out = j.partial ? base + q.dx : dx;
     j.dloss = (const float*)dloss;
-    small_add(o, j, q.out, q.sx);
+    small_add(o, j, q.tx, q.sx);
     const int sx = o.job[0].tiles / (o.job[0].tm * o.job[0].tn);
+    if (q.tx.m != q.tw.m) {
+        run_small(c, p.dt, o, q.tx);
+        o = SmallWork{};
+    }
     // dw = P^T (dloss x)
     j.a_mn = 1;
     j.B = p.x;
@@ -1474,9 +1519,10 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
     j.K = (int)p.n;
     j.partial = q.sw > 1;
     j.out = j.partial ? base + q.dw : dw;
-    small_add(o, j, q.out, q.sw);
-    const int sw = o.job[1].tiles / (o.job[1].tm * o.job[1].tn);
-    run_small(c, p.dt, o, q.out);
+    small_add(o, j, q.tw, q.sw);
+    const SmallJob& jw = o.job[o.jobs - 1];
+    const int sw = jw.tiles / (jw.tm * jw.tn);
+    run_small(c, p.dt, o, q.tw);
     if (q.sx > 1 || q.sw > 1) {
         SumWork s{};
         if (q.sx > 1) s.job[0] = {(const float*)(base + q.dx), dx, (const float*)dloss, nullptr, p.n, p.dim, sx};
@@ -1490,7 +1536,7 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
 }  // namespace
 
 size_t xent_workspace(const XentP& p, bool grad) {
-    return is_small(p) ? small_plan(p, grad).total : make_plan(p, grad).total;
+    return is_small(p, grad) ? small_plan(p, grad).total : make_plan(p, grad).total;
 }
 
 int xent_error() {
@@ -1509,7 +1555,7 @@ int xent_error() {
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     if (p.n == 0) return OK;
-    if (is_small(p)) return small_xent(c, p, loss, lse, ws);
+    if (is_small(p, false)) return small_xent(c, p, loss, lse, ws);
     const Plan q = make_plan(p, false);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), xip = in_place(p, p.x);
@@ -1560,7 +1606,7 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
         NXV_CK(cudaMemsetAsync(dw, 0, (size_t)p.vocab * p.dim * dtype_bytes(p.dt), c.stream));
         return finish(c);
     }
-    if (is_small(p)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
+    if (is_small(p, true)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
     const Plan q = make_plan(p, true);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), six = q.planes == 3;
