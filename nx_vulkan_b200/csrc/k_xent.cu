@@ -54,7 +54,9 @@ using bf16 = __nv_bfloat16;
 constexpr int BT = 128, BK = 64;  // BK bf16 = one 128-byte swizzle row
 constexpr int ST = 6;
 constexpr int OP_BYTES = BT * BK * 2, ST_BYTES = 2 * OP_BYTES;
-constexpr int SMEM = ST * ST_BYTES + 1024 + 256;
+constexpr int TR_BYTES = 8 * 32 * 33 * 4;  // a 32 x 32 transpose buffer per epilogue warp
+constexpr int SMEM = ST * ST_BYTES + 1024 + 256 + TR_BYTES;
+static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 constexpr int kThreads = 384;  // producer of A, MMA issuer, allocator, producer of B, 8 epilogue warps
 
 __device__ int g_xent_error;
@@ -319,6 +321,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // One thread's row of a tile: 32 columns at a time go through chunk().
 // n0: the columns' first column of D; left: columns of D from there.
+// SIX: no transpose buffer (its code costs registers that hold the sums).
+template <bool SIX>
 struct Row {
     const Job& g;
     const int row, n0, left;
@@ -334,8 +338,10 @@ struct Row {
     int align = 0;
     bool has = false;
 
-    __device__ __forceinline__ Row(const Job& j, int r, int n, uint32_t slice)
-        : g(j), row(r), n0(n), left(j.N - n), live(r < j.M) {
+    float* const tr;  // the warp's transpose buffer
+
+    __device__ __forceinline__ Row(const Job& j, int r, int n, uint32_t slice, float* t)
+        : g(j), row(r), n0(n), left(j.N - n), live(r < j.M), tr(t) {
         row_at = ((size_t)slice * g.M + row) * g.ldo;
         if (g.kind == OUT) {
             const int es = g.out_bf16 ? 2 : 4;
@@ -395,7 +401,7 @@ struct Row {
         }
         // ldg covers whole tiles, so the columns past N have room; no product reads them
         bf16* dst = g.g + (size_t)row * g.ldg + n0 + c0;
-        if (g.gplane == 0) {
+        if constexpr (!SIX) {
 #pragma unroll
             for (int q = 0; q < 2; q++) {
                 uint32_t u[8];
@@ -424,21 +430,38 @@ struct Row {
         }
     }
 
+    // Whole aligned rows of 32 columns: a lane stores its own row, 32 bytes at a
+    // time.  Else through the warp's transpose buffer: a row's columns are the
+    // lanes', so that what cannot be a wide store is at least a whole line.
     __device__ __forceinline__ void chunk_out(float (&v)[32], int c0) {
+        if (align >= 16 && c0 + 32 <= left) out_rows(v, c0);
+        else if constexpr (SIX) out_single(v, c0);
+        else out_columns(v, c0);
+    }
+
+    __device__ __forceinline__ void out_single(float (&v)[32], int c0) {
         if (!live) return;
-        const size_t at = row_at + n0 + c0;
-        const bool whole = align >= 16 && c0 + 32 <= left;
+        finish(v, c0, false);
+        float* o = (float*)g.out + row_at + n0 + c0;
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+            if (c0 + e < left) o[e] = v[e];
+    }
+
+    // The sum so far and the factors.
+    __device__ __forceinline__ void finish(float (&v)[32], int c0, bool wide) {
         if (g.acc_in) {
-            if (whole) {
+            const float* in = g.acc_in + row_at + n0 + c0;
+            if (wide) {
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
-                    const float4 a = reinterpret_cast<const float4*>(g.acc_in + at)[q];
+                    const float4 a = reinterpret_cast<const float4*>(in)[q];
                     v[4 * q] += a.x, v[4 * q + 1] += a.y, v[4 * q + 2] += a.z, v[4 * q + 3] += a.w;
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; e++)
-                    if (c0 + e < left) v[e] += g.acc_in[at + e];
+                    if (c0 + e < left) v[e] += in[e];
             }
         }
         if (g.dloss) {
@@ -450,35 +473,53 @@ struct Row {
 #pragma unroll
             for (int e = 0; e < 32; e++) v[e] *= f;
         }
-        if (g.out_bf16) {
+    }
+
+    __device__ __forceinline__ void out_columns(float (&v)[32], int c0) {
+        const int lane = threadIdx.x & 31, r0 = row - lane;
+        __syncwarp();  // the buffer's last chunk has been read
+#pragma unroll
+        for (int e = 0; e < 32; e++) tr[lane * 33 + e] = v[e];
+        __syncwarp();
+        const size_t at0 = row_at - (size_t)lane * g.ldo + n0 + c0 + lane;
+        const float f = g.factor ? *g.factor : 1.0f;
+        const bool in = c0 + lane < left;
+#pragma unroll 4
+        for (int r = 0; r < 32; r++) {
+            const float rdl = __shfl_sync(0xffffffffu, dl, r);
+            const bool rhas = __shfl_sync(0xffffffffu, has, r);
+            if (!in || r0 + r >= g.M) continue;
+            const size_t at = at0 + (size_t)r * g.ldo;
+            float x = tr[r * 33 + lane];
+            if (g.acc_in) x += g.acc_in[at];
+            if (g.dloss) x = rhas ? x * rdl : 0.0f;
+            x *= f;
+            if (g.out_bf16) ((bf16*)g.out)[at] = __float2bfloat16_rn(x);
+            else ((float*)g.out)[at] = x;
+        }
+    }
+
+    __device__ __forceinline__ void out_rows(float (&v)[32], int c0) {
+        if (!live) return;
+        const size_t at = row_at + n0 + c0;
+        finish(v, c0, true);
+        if (!SIX && g.out_bf16) {
             bf16* o = (bf16*)g.out + at;
-            if (whole) {
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    uint32_t u[8];
+            for (int q = 0; q < 2; q++) {
+                uint32_t u[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) u[e] = pack2(v[q * 16 + 2 * e], v[q * 16 + 2 * e + 1]);
-                    store32(o + q * 16, u, align);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                    if (c0 + e < left) o[e] = __float2bfloat16_rn(v[e]);
+                for (int e = 0; e < 8; e++) u[e] = pack2(v[q * 16 + 2 * e], v[q * 16 + 2 * e + 1]);
+                store32(o + q * 16, u, align);
             }
         } else {
             float* o = (float*)g.out + at;
-            if (whole) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t u[8];
+            for (int q = 0; q < 4; q++) {
+                uint32_t u[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) u[e] = __float_as_uint(v[q * 8 + e]);
-                    store32(o + q * 8, u, align);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                    if (c0 + e < left) o[e] = v[e];
+                for (int e = 0; e < 8; e++) u[e] = __float_as_uint(v[q * 8 + e]);
+                store32(o + q * 8, u, align);
             }
         }
     }
@@ -505,7 +546,15 @@ struct Row {
 // the tensor core's sums lose up to a step of the running sum per product,
 // with a bias, so every k-block's sum is added to f32 registers by the
 // epilogue warps (round to nearest) while the next one is made.  Measured for
-// 2048 x 10007 x 1000: error of the gradients 1.9e-5 without, see below.
+// 2048 x 10007 x 1000: error of the gradients 1.9e-5 without, 2.6e-7 with.
+// Bound by the tensor pipe, at the clock that its power leaves.  What it took: pair
+// tiles (a stage's 32 KB for 512 cycles of products), and issue loops without
+// divisions, one warp per operand and uniform (a stage took its one thread
+// ~1000 cycles to load before, whatever its size or the ring's depth, and ~500 to
+// multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms, 1.69 PFLOP/s (the
+// library's bare product of these sizes 1.47 ms in the same session); gradient 5.1
+// to 5.5 ms, 1.6 to 1.7 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
+// 2.2 and 8.7 ms, 1.5 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
 // flight are waited for (bounded), tensor memory is freed and g_xent_error set.
 template <int CG, bool SIX>
@@ -522,7 +571,7 @@ k_xgemm(const __grid_constant__ Work W) {
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* drain = acc_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    __shared__ volatile int s_err;
+    volatile int& s_err = *reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = CG == 2 ? (blockIdx.x & 1) : 0;
@@ -660,6 +709,7 @@ k_xgemm(const __grid_constant__ Work W) {
         const int q = warp & 3, h = (warp - 4) >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + h * HALF;
         const uint32_t b_free = in_leader(b_acce);
+        float* tr = reinterpret_cast<float*>(smem + ST * ST_BYTES + 256) + (warp - 4) * (32 * 33);
         uint32_t ph = 0;
         bool ok = true;
         for (uint32_t t = first; t < W.tiles && ok; t += step) {
@@ -672,9 +722,11 @@ k_xgemm(const __grid_constant__ Work W) {
             const int row = (int)(lt % g.tm * NC) + rank * BT + q * 32 + lane;
             const int n0 = (int)(lt / g.tm * NC) + h * HALF;
             if constexpr (SIX) {
-                float acc[HALF];
+                float acc[HALF / 32][32];
 #pragma unroll
-                for (int e = 0; e < HALF; e++) acc[e] = 0.0f;
+                for (int c = 0; c < HALF / 32; c++)
+#pragma unroll
+                    for (int e = 0; e < 32; e++) acc[c][e] = 0.0f;
                 for (int f = 0; f < KB; f++, ph++) {
                     const uint32_t buf = ph & 1;
                     ok = warp_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err);
@@ -685,25 +737,20 @@ k_xgemm(const __grid_constant__ Work W) {
                         float v[32];
                         tmem_ld32(v, lanes + buf * NC + c * 32);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) acc[c * 32 + e] += v[e];
+                        for (int e = 0; e < 32; e++) acc[c][e] += v[e];
                     }
                     TC_BEFORE();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_leader(b_free + buf * 8);
                 }
                 if (!ok) break;
-                Row r(g, row, n0, slice);
+                Row<SIX> r(g, row, n0, slice, tr);
 #pragma unroll
-                for (int c = 0; c < HALF / 32; c++) {
-                    float v[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = acc[c * 32 + e];
-                    r.chunk(v, c * 32);
-                }
+                for (int c = 0; c < HALF / 32; c++) r.chunk(acc[c], c * 32);
                 r.done(HALF);
             } else {
                 const uint32_t buf = ph & 1;
-                Row r(g, row, n0, slice);
+                Row<SIX> r(g, row, n0, slice, tr);
                 ok = warp_wait(b_accf + buf * 8, (ph >> 1) & 1, &s_err);
                 if (!ok) break;
                 ph++;
@@ -913,11 +960,12 @@ k_xent_join_row(float* __restrict__ loss, float* __restrict__ lse, const float* 
 // backward (P, both products, in one launch where they take the same tile, and
 // where a long K is cut into slices, their sum).
 
-// The limits on n vocab dim, from both paths' times in us, this one's first.
-// Loss f32: 64 x 1001 x 1000 19 and 42, 512^3 33 and 35; bf16: 16 x 200 x 100 10 and 17,
-// 64 x 1001 x 1000 23 and 15.  Gradient f32: 16 x 200 x 100 15 and 39, 256 x 512 x 512
-// 80 and 66; bf16: 16 x 200 x 100 15 and 40, 64 x 300 x 400 27 and 28.
-constexpr unsigned long long kSmallLoss = 1ull << 26, kSmallGrad = 1ull << 24, kSmallBf16 = 1ull << 22;
+// The limits on n vocab dim, from both paths' times in us (loss / gradient, this
+// path's first): f32 16 x 200 x 100 12 / 15 and 23 / 41, 64 x 1001 x 1000 19 / 59 and
+// 40 / 76, 256 x 512 x 512 21 / 54 and 35 / 74, 512^3 35 / 101 and 35 / 74; bf16
+// 200 x 200 x 100 11 / 19 and 23 / 45 (not 16-byte rows), 64 x 300 x 400 13 / 19 and
+// 13 / 25, 128 x 512 x 256 13 / 27 and 11 / 23, 64 x 1001 x 1000 21 / 60 and 16 / 31.
+constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;
 constexpr int KSTEP = 128;  // slices of K are multiples of this, and of a tile's chunk KC
 
 struct SmallJob {
@@ -1357,8 +1405,8 @@ void join(Ctx& c, const XentP& p, void* loss, void* lse, const float* pm, const 
 
 // ---- host: small problems --------------------------------------------------------
 
-bool is_small(const XentP& p, bool grad) {
-    const unsigned long long most = p.dt == BF16 ? kSmallBf16 : grad ? kSmallGrad : kSmallLoss;
+bool is_small(const XentP& p) {
+    const unsigned long long most = p.dt == BF16 ? kSmallBf16 : kSmallF32;
     const unsigned long long n = up(p.n, 16);  // whole row tiles
     // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
     return n * p.vocab <= most && n * p.vocab * p.dim <= most;
@@ -1536,7 +1584,7 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
 }  // namespace
 
 size_t xent_workspace(const XentP& p, bool grad) {
-    return is_small(p, grad) ? small_plan(p, grad).total : make_plan(p, grad).total;
+    return is_small(p) ? small_plan(p, grad).total : make_plan(p, grad).total;
 }
 
 int xent_error() {
@@ -1555,7 +1603,7 @@ int xent_error() {
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     if (p.n == 0) return OK;
-    if (is_small(p, false)) return small_xent(c, p, loss, lse, ws);
+    if (is_small(p)) return small_xent(c, p, loss, lse, ws);
     const Plan q = make_plan(p, false);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), xip = in_place(p, p.x);
@@ -1606,7 +1654,7 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
         NXV_CK(cudaMemsetAsync(dw, 0, (size_t)p.vocab * p.dim * dtype_bytes(p.dt), c.stream));
         return finish(c);
     }
-    if (is_small(p, true)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
+    if (is_small(p)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
     const Plan q = make_plan(p, true);
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), six = q.planes == 3;

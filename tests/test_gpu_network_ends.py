@@ -323,11 +323,12 @@ def test_dropout_of_nothing(nxv, torch):
 
 # ---- linear cross entropy ----------------------------------------------------------
 
-# up to 2^27 multiply-adds on one path, more on the tensor cores
+# up to 2^26 multiply-adds (bf16 2^23) on one path, more on the tensor cores
 XENT_SHAPES = [(1, 1, 1), (1, 10, 3), (3, 257, 13), (2, 256, 64), (130, 1000, 64), (129, 513, 65),
                (128, 256, 128), (257, 300, 1001), (5, 5003, 16), (300, 31, 200), (4099, 21, 17), (1, 70001, 5),
                (515, 515, 515), (513, 1001, 513), (129, 2049, 1025), (100, 40000, 64), (20000, 129, 64),
-               (3001, 100, 1000), (3, 20000, 3000), (2, 50001, 700), (8193, 12, 800), (40000, 300, 8), (9000, 70, 130)]
+               (3001, 100, 1000), (3, 20000, 3000), (2, 50001, 700), (8193, 12, 800), (40000, 300, 8), (9000, 70, 130),
+               (129, 600, 72), (200, 1100, 333)]
 
 
 def xent_inputs(torch, name, n, v, d, seed=0, scale=2.0):
