@@ -412,6 +412,27 @@ k_norm_fwd_long(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, 
     }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The value at p in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t peer_address(const void* p, unsigned rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float peer_value(const float* p, unsigned rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_address(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ double peer_value(const double* p, unsigned rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(peer_address(p, rank)) : "memory");
+    return v;
+}
+
 // Backward: how the rows are dealt out: G threads (a power of two, lg its
 // logarithm) take R rows at a time; rounds of all the CTA's groups.
 struct Deal {
@@ -474,14 +495,17 @@ __device__ __forceinline__ void group_sum(A (&v)[K], unsigned G, A (*red)[16]) {
 // so it adds up its columns' dy xh and dy in registers.  R rows at a time (bf16:
 // 2), while the next two rounds' come into L2.  At the end the groups' column
 // sums are added, in order, into row blockIdx.x of the partial sums
-// [2][gridDim.x][cols].  With t = x - mean, e = dy rstd:
+// [2][gridDim.x][cols]; or, where the grid is one cluster of up to 8 CTAs (dgamma is
+// given), over the CTAs' shared memory into dgamma and dbeta, which saves the fold's
+// launch.  With t = x - mean, e = dy rstd:
 //   dgamma += e t,  dbeta += dy,  dx = e gamma - rstd c1 - t rstd^2 c2,
 // c1 = mean(dy gamma), c2 = mean(dy gamma t).
 template <typename T, int NV, int R, bool AL>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
            const T* __restrict__ gamma, const acc_t<T>* __restrict__ mean,
-           const acc_t<T>* __restrict__ rstd, const __grid_constant__ Deal d) {
+           const acc_t<T>* __restrict__ rstd, T* dgamma, T* dbeta,
+           const __grid_constant__ Deal d) {
     using A = acc_t<T>;
     using W = vec_t<T>;
     constexpr int V = kV<T>, N = kN<T>, NP = kP<T>;
@@ -597,7 +621,17 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
         for (unsigned c = tid; c < cols; c += kBwdThreads) {
             A v = sh[c];
             for (unsigned j = 1; j < groups; j++) v += sh[(size_t)j * pad + c];
-            out[c] = v;
+            if (dgamma) sh[c] = v;  // this thread's own column
+            else out[c] = v;
+        }
+        if (dgamma) {
+            cluster_sync();
+            for (unsigned c = blockIdx.x * kBwdThreads + tid; c < cols; c += gridDim.x * kBwdThreads) {
+                A v = A(0);
+                for (unsigned j = 0; j < gridDim.x; j++) v += peer_value(&sh[c], j);
+                from_acc((which ? dbeta : dgamma)[c], v);
+            }
+            cluster_sync();  // the peers have read this CTA's sums
         }
     }
 }
@@ -827,9 +861,13 @@ size_t bwd_part_bytes(const BwdShape& q, unsigned cols, int dt) {
     return (size_t)2 * q.parts * cols * (dt == F64 ? 8 : 4);
 }
 
+// Few CTAs fold the weights' gradients among themselves.
+bool one_cluster(const BwdShape& q) { return q.strips == 0 && q.grid > 0 && q.grid <= 8; }
+
 template <typename T, bool AL>
-int bwd(Ctx& c, const BwdShape& q, T* dx, acc_t<T>* part, acc_t<T>* sums, const T* dy, const T* x,
-        const T* g, const acc_t<T>* mean, const acc_t<T>* rstd, unsigned rows, unsigned cols) {
+int bwd(Ctx& c, const BwdShape& q, T* dx, T* dg, T* db, acc_t<T>* part, acc_t<T>* sums, const T* dy,
+        const T* x, const T* g, const acc_t<T>* mean, const acc_t<T>* rstd, unsigned rows,
+        unsigned cols) {
     if (q.strips) {
         k_norm_bwd_sums<T, AL><<<std::min(rows, (unsigned)c.dev->sm_count * 4), 512, 0, c.stream>>>(
             sums, dy, x, g, mean, rstd, rows, cols);
@@ -842,7 +880,20 @@ int bwd(Ctx& c, const BwdShape& q, T* dx, acc_t<T>* part, acc_t<T>* sums, const 
     auto f = one ? k_norm_bwd<T, 1, kRows<T>, AL> : k_norm_bwd<T, kPer<T>, kRows<T>, AL>;
     const size_t bytes = (size_t)kBwdThreads * (one ? 1 : kPer<T>) * kV<T> * sizeof(acc_t<T>);
     NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    f<<<q.grid, kBwdThreads, bytes, c.stream>>>(dx, part, dy, x, g, mean, rstd, q.deal);
+    const bool fold = one_cluster(q);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(q.grid);
+    cfg.blockDim = dim3(kBwdThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = fold ? q.grid : 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NXV_CK(cudaLaunchKernelEx(&cfg, f, dx, part, dy, x, g, mean, rstd, fold ? dg : (T*)nullptr, db, q.deal));
     count_launch();
     return OK;
 }
@@ -854,14 +905,16 @@ int bwd_t(Ctx& c, int dt, void* dx, void* dg, void* db, void* ws, const void* dy
     const BwdShape q = bwd_shape(rows, cols, dt);
     if (rows > 0) {
         auto f = all_aligned<T>(cols, {dx, dy, x, g}) ? bwd<T, true> : bwd<T, false>;
-        const int rc = f(c, q, (T*)dx, (A*)ws, (A*)((char*)ws + bwd_part_bytes(q, cols, dt)),
+        const int rc = f(c, q, (T*)dx, (T*)dg, (T*)db, (A*)ws, (A*)((char*)ws + bwd_part_bytes(q, cols, dt)),
                          (const T*)dy, (const T*)x, (const T*)g, (const A*)mean, (const A*)rstd, rows,
                          cols);
         if (rc) return rc;
     }
-    k_norm_fold<T><<<dim3((cols + 31) / 32, 2), dim3(32, 32), 0, c.stream>>>(
-        (T*)dg, (T*)db, (const A*)ws, q.parts, cols);
-    count_launch();
+    if (!one_cluster(q)) {
+        k_norm_fold<T><<<dim3((cols + 31) / 32, 2), dim3(32, 32), 0, c.stream>>>(
+            (T*)dg, (T*)db, (const A*)ws, q.parts, cols);
+        count_launch();
+    }
     pdl_record_all(c);
     return finish(c);
 }
