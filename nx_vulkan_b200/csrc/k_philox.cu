@@ -270,6 +270,10 @@ __global__ void k_random_f64(double* __restrict__ out, size_t n, uint32_t seed, 
 // and infinities included).  thresh = ceil(p 2^24): the comparison of the
 // uniform (word >> 8) 2^-24 with p, in whole numbers.  f32 arithmetic for f32
 // and bf16 (bf16 rounded once at the store), f64 for f64.
+// f32 and f64 are bound by memory (2^26 f32 90 us, 6.0 TB/s), bf16 by the mask: two
+// elements take ten wide multiplies, which are issued at a fraction of the other
+// instructions' rate (2^27 bf16 128 us, 4.2 TB/s; a multiply less per counter, by
+// adding the multiplier to the neighbour's first product, changed nothing).
 __device__ __forceinline__ float drop_scaled(float x, double, float s) { return __fmul_rn(x, s); }
 __device__ __forceinline__ double drop_scaled(double x, double s, float) { return __dmul_rn(x, s); }
 __device__ __forceinline__ __nv_bfloat16 drop_scaled(__nv_bfloat16 x, double, float s) {
@@ -377,7 +381,7 @@ void dropout_t(Ctx& c, T* y, const T* x, size_t n, double p, uint32_t seed, uint
         cudaMemsetAsync(y, 0, n * sizeof(T), c.stream);
         return;
     }
-    const unsigned g = grid_for(c, vec ? (n + V - 1) / V : n, 256, 8);
+    const unsigned g = grid_for(c, vec ? (n + V - 1) / V : n, 256, 6);  // as many as stay resident
     if (!vec) k_dropout<T, 1, false><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
     else if (offset & 1) k_dropout<T, V, true><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
     else k_dropout<T, V, false><<<g, 256, 0, c.stream>>>(y, x, n, least, s64, s32, seed, offset);
