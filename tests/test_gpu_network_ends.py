@@ -76,7 +76,8 @@ def place(torch, t, shift):
 
 NORM_SHAPES = [(1, 1), (1, 2), (4, 7), (5, 32), (9, 33), (3, 256), (7, 1000), (2, 1023), (300, 129),
                (3, 4096), (2, 5001), (7, 5003), (2, 8192), (3, 12289), (1, 16384), (2, 20000), (1, 40001), (3, 70001),
-               (600, 64), (1200, 33), (700, 1025), (500, 20003)]
+               (600, 64), (1200, 33), (700, 1025), (500, 20003),
+               (2500, 3), (2400, 257), (2400, 1000), (5000, 104), (2400, 5001)]
 
 
 def norm_run(nxv, torch, x, g, b, eps, name, y=None):
@@ -224,6 +225,21 @@ def test_layer_norm_no_rows(nxv, torch):
     assert bool((dg == 0).all()) and bool((db == 0).all())
 
 
+def test_layer_norm_past_32_bits(nxv, torch):
+    """More than 2^31 elements: the last rows are right, and the weights' sums see them."""
+    r, c = (1 << 17) + 5, 16392
+    x = torch.empty(r, c, device="cuda", dtype=torch.bfloat16).normal_()
+    g, b = torch.randn(c, device="cuda").bfloat16(), torch.randn(c, device="cuda").bfloat16()
+    y, m, s = norm_run(nxv, torch, x, g, b, 1e-5, "bf16")
+    for part in (slice(0, 3), slice(r - 3, r)):
+        norm_check(torch, "bf16", x[part], g, b, 1e-5, y[part], m[part], s[part])
+    dy = torch.zeros_like(x)
+    dy[:2], dy[-2:] = torch.randn(2, c, device="cuda"), torch.randn(2, c, device="cuda")
+    dx, dg, db = grad_run(nxv, torch, dy, x, g, m, s, "bf16", dx=y)
+    ends = [0, 1, r - 2, r - 1]
+    grad_check(torch, "bf16", dy[ends], x[ends], g, m[ends], s[ends], dx[ends], dg, db)
+
+
 def test_layer_norm_grad_against_differences(nxv, torch):
     """Central differences of sum(dy * y) along a random direction of (x, gamma, beta), in f64:
     truncation h^2 / 6 times third derivatives of order 1, rounding 2^-53 / h."""
@@ -315,6 +331,16 @@ def test_dropout_at_the_end_of_the_stream(nxv, torch):
     want = [2.0 if (words(i >> 1, 42)[i & 1] >> 8) >= 1 << 23 else 0.0 for i in range(first, first + n)]
     assert y.tolist() == want
     assert nxv.dropout(wrap(nxv, x), 0.5, 42, offset=first + 1) == ("error", "bad_op")
+
+
+def test_dropout_past_32_bits(nxv, torch):
+    """More than 2^32 bytes and 2^31 elements: the end of the whole is the end in parts."""
+    n = (1 << 31) + 1037
+    x = torch.full((n,), 1.5, device="cuda", dtype=torch.bfloat16)
+    y, z = torch.empty_like(x), torch.empty(2000, device="cuda", dtype=torch.bfloat16)
+    ok(nxv.dropout(wrap(nxv, x), 0.25, 9, offset=5, dtype="bf16", out=wrap(nxv, y)))
+    ok(nxv.dropout(wrap(nxv, x[:2000]), 0.25, 9, offset=5 + n - 2000, dtype="bf16", out=wrap(nxv, z)))
+    assert torch.equal(y[-2000:], z) and 1300 < int((z != 0).sum()) < 1700
 
 
 def test_dropout_of_nothing(nxv, torch):
@@ -530,6 +556,42 @@ def test_rows_without_a_target_give_nothing(nxv, torch, name):
     labels[:] = -1
     dx, dw = xgrad_run(nxv, torch, dl, x, w, labels, lse, name)
     assert bool((dx == 0).all()) and bool((dw == 0).all())
+
+
+def test_linear_cross_entropy_past_32_bits(nxv, torch):
+    """Weights of more than 2^31 elements, classes behind them as labels."""
+    n, v, d = 130, (1 << 18) + 77, 8200
+    torch.manual_seed(3)
+    x = torch.randn(n, d, device="cuda").bfloat16()
+    w = torch.empty(v, d, device="cuda", dtype=torch.bfloat16).normal_() * (2 / d ** 0.5)
+    labels = torch.randint(v - 100, v, (n,), device="cuda")
+    labels[0], labels[1] = 0, -1
+    loss, lse = xent_run(nxv, torch, x, w, labels, "bf16")
+    z = torch.cat([x.double() @ w[i:i + 4096].double().t() for i in range(0, v, 4096)], 1)
+    want = torch.logsumexp(z, 1)
+    # a logit's additions, at the largest size of a row's products
+    size = [(x.double().abs() @ w[i:i + 4096].double().abs().t()).amax(1) for i in range(0, v, 4096)]
+    ez = (d / 4 + 8) * 2.0 ** -23 * torch.stack(size).amax(0)
+    tol = lse_tol(z, ez)
+    within(torch, lse, want, tol)
+    has = labels >= 0
+    within(torch, loss[has], (want - z.gather(1, labels.clamp(min=0)[:, None])[:, 0])[has], (tol + ez)[has])
+    dl = torch.full((n,), 1 / 129, device="cuda")
+    dx, dw = xgrad_run(nxv, torch, dl, x, w, labels, lse, "bf16")
+    p = torch.exp(z - lse.double()[:, None])
+    p[has, labels[has]] -= 1.0
+    g = torch.where(has[:, None], p * dl.double()[:, None], 0.0)
+    for part in (slice(0, 50), slice(v - 120, v)):
+        want = g[:, part].t() @ x.double()
+        size = g[:, part].abs().t() @ x.double().abs()
+        # two roundings to bf16 of every term and one of the sum; the logits' error
+        within(torch, dw[part], want, 2.0 ** -8 * want.abs() + (2.0 ** -7 + 2 * float(ez.max()) + 2.0 ** -12) * size)
+    want = torch.zeros(n, d, device="cuda", dtype=torch.float64)
+    size = torch.zeros_like(want)
+    for i in range(0, v, 4096):
+        want += g[:, i:i + 4096] @ w[i:i + 4096].double()
+        size += g[:, i:i + 4096].abs() @ w[i:i + 4096].double().abs()
+    within(torch, dx, want, 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * float(ez.max()) + 2.0 ** -12 + v / 16 * 2.0 ** -23) * size)
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16"])
