@@ -336,10 +336,10 @@ __device__ __forceinline__ void drop_16(uint32_t (&x)[4], const uint32_t* w, uin
 }
 
 // A thread takes VEC consecutive elements (16 bytes) of VEC / 2 counters; with
-// an odd offset (ODD) their words lie in VEC / 2 + 1 counters.  The elements behind the last whole vector, and every element of a
-// tensor that is not 16-byte aligned (VEC = 1), go one by one.  least: the
-// smallest word that keeps its element, thresh << 8 (the eight low bits do not
-// count); none does for p = 1, where all is zeros.
+// an odd offset (ODD) their words lie in VEC / 2 + 1 counters.  The elements behind
+// the last whole vector, and every element of a tensor that is not 16-byte aligned
+// (VEC = 1), go one by one.  least: the smallest word that keeps its element,
+// thresh << 8 (the eight low bits do not count).
 template <typename T, int VEC, bool ODD>
 __global__ void __launch_bounds__(256, 6)
 k_dropout(T* y, const T* x, size_t n, uint32_t least, double s64, float s32, uint32_t seed,
@@ -373,11 +373,12 @@ k_dropout(T* y, const T* x, size_t n, uint32_t least, double s64, float s32, uin
 template <typename T>
 void dropout_t(Ctx& c, T* y, const T* x, size_t n, double p, uint32_t seed, uint64_t offset) {
     constexpr int V = 16 / sizeof(T);
-    const uint32_t least = (uint32_t)ceil(p * 0x1.0p24) << 8;  // p 2^24 is exact
+    const double thresh = ceil(p * 0x1.0p24);  // p 2^24 is exact
+    const uint32_t least = (uint32_t)thresh << 8;
     const double s64 = 1.0 / (1.0 - p);
     const float s32 = (float)s64;
     const bool vec = ((((uintptr_t)x) | ((uintptr_t)y)) & 15) == 0;
-    if (p >= 1.0) {
+    if (thresh >= 0x1.0p24) {  // above the largest uniform: nothing is kept
         cudaMemsetAsync(y, 0, n * sizeof(T), c.stream);
         return;
     }
