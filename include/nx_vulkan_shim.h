@@ -253,7 +253,8 @@ int nxv_random_f64(void* out, unsigned long n, unsigned int seed, unsigned int d
 /* Layer norm of every row of x [rows, cols]: mean, rstd = 1 / sqrt(var + eps)
  * (var = mean of (x - mean)^2), y = (x - mean) rstd gamma + beta.  gamma, beta
  * [cols] and y have x's type; mean and rstd [rows] are f32 (f64 for f64) and
- * all arithmetic is in their type.  y may be x.  1 <= cols <= 2^28, eps >= 0.
+ * all arithmetic is in their type (rows whose squared deviations' sum overflows
+ * it have rstd 0).  y may be x.  1 <= cols <= 2^28, eps >= 0.
  * spv: layer_norm.spv. */
 int nxv_layer_norm(void* y, void* mean, void* rstd,
                    void* x, void* gamma, void* beta,
@@ -296,7 +297,7 @@ unsigned long nxv_linear_cross_entropy_workspace(unsigned int n, unsigned int vo
  * f32 or 2 bf16 (tcgen05; f32 as six bf16 partial products, f32 accuracy).
  * As logsumexp.spv: a row whose logits hold a NaN or +inf, or only -inf, has
  * lse NaN; in f32 an infinity in x or w makes every logit it meets NaN.
- * vocab, dim > 0.  spv: linear_cross_entropy.spv. */
+ * vocab > 0, 0 < dim <= 2^24.  spv: linear_cross_entropy.spv. */
 int nxv_linear_cross_entropy(void* loss, void* lse, void* workspace,
                              void* x, void* w, void* labels,
                              unsigned int n, unsigned int vocab, unsigned int dim,

@@ -39,7 +39,6 @@
 #include <limits.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 namespace nxv {
@@ -58,9 +57,6 @@ constexpr int TR_BYTES = 8 * 32 * 33 * 4;  // a 32 x 32 transpose buffer per epi
 constexpr int SMEM = ST * ST_BYTES + 1024 + 256 + TR_BYTES;
 static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 constexpr int kThreads = 384;  // producer of A, MMA issuer, allocator, producer of B, 8 epilogue warps
-
-__device__ int g_xent_error;
-std::atomic<bool> g_xent_ran{false};  // a kernel that may set it was launched since the last look
 
 // ---- PTX ----------------------------------------------------------------------
 
@@ -106,7 +102,6 @@ __device__ __noinline__ bool mbar_wait_long(uint32_t b, uint32_t parity, volatil
         }
     }
     *err = 1;
-    atomicExch(&g_xent_error, 1);
     return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t b, uint32_t parity, volatile int* err) {
@@ -275,8 +270,7 @@ struct Job {
     const float* lse;
     bf16* g;              // planes of [M][ldg]
     long long ldg, gplane;
-    // OUT
-    // OUT: with slices, f32 [slice][M][ldo] each
+    // OUT: with slices, out and acc_in are f32 [slice][M][ldo]
     const float* acc_in;  // f32 [M][ldo] to add, or null
     const float* dloss;   // [M]: the rows' factors, 0 for a row without a target; or null
     const float* factor;  // one factor of all, or null
@@ -297,6 +291,7 @@ struct alignas(64) Work {
     Job job[kMaxJobs];
     int jobs;
     uint32_t tiles;
+    int* err;             // wait_flag()
 };
 
 // The six partial products of f32, the smallest first.
@@ -556,7 +551,7 @@ struct Row {
 // to 5.5 ms, 1.6 to 1.7 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
 // 2.2 and 8.7 ms, 1.5 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
-// flight are waited for (bounded), tensor memory is freed and g_xent_error set.
+// flight are waited for (bounded), tensor memory is freed and the host's flag set.
 template <int CG, bool SIX>
 __global__ void __launch_bounds__(kThreads, 1)
 k_xgemm(const __grid_constant__ Work W) {
@@ -771,6 +766,7 @@ k_xgemm(const __grid_constant__ Work W) {
     __syncwarp();
     TC_BEFORE();
     __syncthreads();
+    if (tid == 0 && s_err) atomicExch_system(W.err, 1);
     if constexpr (CG == 2) cluster_sync();
     if (warp == 2) {
         TC_AFTER();
@@ -1264,8 +1260,8 @@ int launch_work(Ctx& c, const Work& w) {
     return OK;
 }
 
-int run_work(Ctx& c, const Work& w, int cg, bool six) {
-    g_xent_ran.store(true);
+int run_work(Ctx& c, Work& w, int cg, bool six) {
+    w.err = wait_flag();
     if (cg == 2) return six ? launch_work<2, true>(c, w) : launch_work<2, false>(c, w);
     return six ? launch_work<1, true>(c, w) : launch_work<1, false>(c, w);
 }
@@ -1588,17 +1584,8 @@ size_t xent_workspace(const XentP& p, bool grad) {
 }
 
 int xent_error() {
-    if (!g_xent_ran.exchange(false)) return 0;
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_xent_error, sizeof(int)) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    if (v) {
-        int z = 0;
-        cudaMemcpyToSymbol(g_xent_error, &z, sizeof(int));
-    }
-    return v;
+    int* f = wait_flag();
+    return f ? __atomic_exchange_n(f, 0, __ATOMIC_ACQ_REL) : 0;
 }
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {

@@ -132,6 +132,8 @@ int init_default() {
     return OK;
 }
 
+int* g_wait_flag = nullptr;
+
 int init_devices(const int* ids, int n) {
     if (!ids || n <= 0) return E_NULL;
     std::lock_guard<std::mutex> lk(g_init_mu);
@@ -139,6 +141,10 @@ int init_devices(const int* ids, int n) {
     for (int i = 0; i < n; i++) {
         int rc = init_one(ids[i]);
         if (rc != OK) return rc;
+    }
+    if (!g_wait_flag) {  // kept to the end of the process: graphs hold its address
+        NXV_CK(cudaHostAlloc(&g_wait_flag, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+        *g_wait_flag = 0;
     }
     g_default_device = ids[0];
     tl_device = ids[0];
@@ -252,6 +258,8 @@ int sync(Ctx& c) {
     NXV_CK(cudaStreamSynchronize(c.stream));
     return OK;
 }
+
+int* wait_flag() { return g_wait_flag; }
 
 bool capturing(Ctx& c) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;

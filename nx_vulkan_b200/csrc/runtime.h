@@ -105,6 +105,10 @@ struct ScratchGuard {
 // True while c.stream is being captured into a CUDA graph.
 bool capturing(Ctx& c);
 
+// Set (from the device too) when a bounded wait of a kernel ran out: host memory of
+// the process, read without a CUDA call.  Null before init.
+int* wait_flag();
+
 // Error reporting.
 void set_error(const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);

@@ -632,9 +632,10 @@ static int xent_args(unsigned n, unsigned vocab, unsigned dim, unsigned dtype,
         return E_ARG;
     }
     const unsigned most = 0x7ffffe00u;
+    const unsigned most_dim = 1u << 24;  // a tile's sum takes a fraction of its bounded wait
     // 32-bit counts of 128 x 128 tiles
     const unsigned long long a = n / 128 + 1, b = vocab / 128 + 1, d = dim / 128 + 1;
-    if (a * b + a * d + b * d >= 1ull << 31 || vocab == 0 || dim == 0 || n > most || vocab > most || dim > most ||
+    if (a * b + a * d + b * d >= 1ull << 31 || vocab == 0 || dim == 0 || n > most || vocab > most || dim > most_dim ||
         (index_bytes != 4 && index_bytes != 8)) {
         set_error("linear_cross_entropy: n %u / vocab %u / dim %u / index_bytes %u out of range", n,
                   vocab, dim, index_bytes);

@@ -686,7 +686,9 @@ def layer_norm(x, gamma, beta, rows, cols, eps=1e-5, dtype="f32", out=None):
 
 
 def layer_norm_grad_workspace(rows, cols, dtype="f32") -> int:
-    """Bytes of layer_norm_grad's workspace."""
+    """Bytes of layer_norm_grad's workspace (0 for what it would refuse)."""
+    if dtype not in DTYPES or not (0 <= rows <= _U32 and 0 < cols <= 1 << 28):
+        return 0
     return int(_lib().nxv_layer_norm_grad_workspace(rows, cols, DTYPES[dtype]))
 
 
@@ -734,7 +736,7 @@ def dropout(x, p, seed, offset=0, dtype="f32", out=None):
 def _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes):
     if dtype not in ("f32", "bf16") or index_bytes not in (4, 8):
         return (ERROR, "bad_op")
-    if not (0 <= n <= _U32 and 0 < vocab <= _U32 and 0 < dim <= _U32):
+    if not (0 <= n <= _U32 and 0 < vocab <= _U32 and 0 < dim <= 1 << 24):
         return (ERROR, "bad_op")
     es = _DTYPE_BYTES[dtype]
     if (x.n_bytes != n * dim * es or w.n_bytes != vocab * dim * es
@@ -744,7 +746,10 @@ def _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes):
 
 
 def linear_cross_entropy_workspace(n, vocab, dim, dtype="f32", grad=False) -> int:
-    """Bytes of the workspace of linear_cross_entropy (or of its gradient)."""
+    """Bytes of the workspace of linear_cross_entropy (or of its gradient; 0 for
+    what they would refuse)."""
+    if dtype not in DTYPES or not all(0 <= v <= _U32 for v in (n, vocab, dim)):
+        return 0
     return int(_lib().nxv_linear_cross_entropy_workspace(n, vocab, dim, DTYPES[dtype], int(grad)))
 
 
