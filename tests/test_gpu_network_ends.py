@@ -208,6 +208,33 @@ def test_layer_norm_grad_at_any_address(nxv, torch, name, shift):
     assert bool((room[:shift + 1] == 7).all()) and bool((room[shift + 1 + 9000:] == 7).all())
 
 
+@pytest.mark.parametrize("name", ["f32", "f64", "bf16"])
+@pytest.mark.parametrize("cols", [1, 2, 3, 5, 9])
+def test_layer_norm_of_short_rows_at_any_address(nxv, torch, name, cols):
+    """Rows shorter than 16 bytes in a tensor that starts between boundaries."""
+    for shift in (1, 3):
+        dy, x, g, m, s = (place(torch, t, shift)[0] for t in grad_inputs(torch, name, 70, cols))
+        dx, room = place(torch, torch.zeros_like(x), shift)
+        grad_check(torch, name, dy, x, g, m, s, *grad_run(nxv, torch, dy, x, g, m, s, name, dx=dx))
+        assert bool((room[:shift] == 7).all()) and bool((room[shift + 70 * cols:] == 7).all())
+        y, room = place(torch, torch.zeros_like(x), shift)
+        norm_check(torch, name, x, g, g, 1e-5, *norm_run(nxv, torch, x, g, g, 1e-5, name, y=y))
+        assert bool((room[:shift] == 7).all()) and bool((room[shift + 70 * cols:] == 7).all())
+
+
+@pytest.mark.parametrize("name", ["f32", "f64", "bf16"])
+@pytest.mark.parametrize("shape", [(5, 100), (700, 1000), (4, 40001)], ids=str)
+def test_layer_norm_grad_of_small_values(nxv, torch, name, shape):
+    """Rows of size 1e-18 and eps = 0: rstd's cube would overflow f32, no gradient does."""
+    dy, x, g, _, _ = grad_inputs(torch, name, *shape)
+    x = x * 1e-18
+    X = x.double()
+    m = X.mean(1)
+    s = 1 / (X - m[:, None]).square().mean(1).sqrt()
+    m, s = m.to(stat(torch, name)), s.to(stat(torch, name))
+    grad_check(torch, name, dy, x, g, m, s, *grad_run(nxv, torch, dy, x, g, m, s, name))
+
+
 @pytest.mark.parametrize("cols", [48, 999, 40001])
 @pytest.mark.parametrize("which", [0, 1])
 def test_layer_norm_grad_in_place(nxv, torch, cols, which):
@@ -341,6 +368,17 @@ def test_dropout_past_32_bits(nxv, torch):
     ok(nxv.dropout(wrap(nxv, x), 0.25, 9, offset=5, dtype="bf16", out=wrap(nxv, y)))
     ok(nxv.dropout(wrap(nxv, x[:2000]), 0.25, 9, offset=5 + n - 2000, dtype="bf16", out=wrap(nxv, z)))
     assert torch.equal(y[-2000:], z) and 1300 < int((z != 0).sum()) < 1700
+
+
+@pytest.mark.parametrize("name", ["f32", "f64", "bf16"])
+def test_dropout_of_nearly_all(nxv, torch, name):
+    """p above the largest uniform, 1 - 2^-24, keeps nothing."""
+    x = torch.full((5000,), 1.5, device="cuda", dtype=dt(torch, name))
+    for p in (1 - 2.0 ** -24, 1 - 2.0 ** -25, 1 - 2.0 ** -53, 1.0):
+        y = torch.full_like(x, 3.0)
+        ok(nxv.dropout(wrap(nxv, x), p, 7, dtype=name, out=wrap(nxv, y)))
+        # the first keeps the uniform 1 - 2^-24 alone, which these 5000 do not hold
+        assert bool((y == 0).all())
 
 
 def test_dropout_of_nothing(nxv, torch):

@@ -105,3 +105,16 @@ def test_the_mirror_refuses_too(lib):
     cg = nxv.linear_cross_entropy_grad
     assert cg(b(4), b(32), b(48), b(16), b(8), 2, 3, 4) == ("error", "size_mismatch")
     assert cg(b(8), b(32), b(48), b(16), b(8), 2, 3, 4, out=(b(32), b(40))) == ("error", "size_mismatch")
+
+
+def test_limits_of_the_workspaces_and_of_dim(lib):
+    from nx_vulkan_b200 import vulkan as nxv
+    big = (1 << 24) + 1
+    assert lib.nxv_linear_cross_entropy(*[P] * 6, 2, 3, big, 0, 8, b"linear_cross_entropy.spv") == -3
+    assert lib.nxv_linear_cross_entropy_grad(*[P] * 8, 2, 3, big, 2, 8, b"linear_cross_entropy_grad.spv") == -3
+    b = FakeBuf
+    assert nxv.linear_cross_entropy(b(8 * big), b(12 * big), b(16), 2, 3, big) == ("error", "bad_op")
+    for args in ((2, 0, 4), (2, 3, big), ((1 << 32) + 2, 3, 4), (2, 3, 4, "f64"), (2, 3, 4, "f16")):
+        assert nxv.linear_cross_entropy_workspace(*args) == 0
+    for args in ((2, 0), ((1 << 32) + 2, 4), (2, (1 << 28) + 1), (2, 4, "f16")):
+        assert nxv.layer_norm_grad_workspace(*args) == 0
