@@ -14,23 +14,23 @@
 // which cancels for rows with a large mean).
 //
 // Both directions are bound by memory: a row is read once, stays in registers
-// and is written once.  What counts is how many bytes are in flight: forward a
-// warp loads a whole row of up to 8 KB before it waits for any of it, and 20 warps
-// an SM do so; backward, where the column sums take the registers, one CTA an SM
-// holds some rows while the next ones are on their way to L2.  Pairs of f32 values go
-// through the packed two-f32 instructions.
-// Measured: [32768, 4096] bf16 forward 89 us (6.0 TB/s; one row per 128 threads
-// of 4 pieces each 105, with barriers between few warps 120 to 160), [16384, 8192]
-// bf16 backward 168 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
+// and is written once.  What counts is how many bytes are in flight: forward the
+// whole row is loaded before anything waits for any of it; backward, where the
+// column sums take the registers, one CTA an SM holds some rows while the next ones
+// are on their way to L2.  Pairs of f32 values go through the packed two-f32
+// instructions.
+// Measured: [32768, 4096] bf16 forward 84 us (6.4 TB/s), [16384, 8192] bf16 backward
+// 168 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
 //
-// Pieces are 16 bytes.  In a row that does not start on a 16-byte boundary
-// thread i still holds columns [i V, (i + 1) V), V = 16 / element size: it reads
-// the two aligned pieces that hold them and shifts.  For a store a lane joins its
-// neighbour's last bytes with its own first ones into an aligned piece; what is
-// left at the ends of a warp's stretch and of the row is stored element by element.
-// An aligned piece at a row's end holds bytes of the rows around it, which are ignored;
-// rows within 16 bytes of the tensor's ends are read element by element, so that
-// nothing outside the tensor is touched.
+// Pieces are 16 bytes.  A row that does not start on a 16-byte boundary is worked on in
+// the aligned pieces of its memory: x, dy and what is written lie at the same place of
+// theirs, so nothing is shifted but gamma and beta, once for rows that start at the
+// same place.  A piece at a row's end holds elements of the rows around it, which are
+// ignored and, in the result, written by their own rows; rows within 16 bytes of the
+// tensor's ends are read element by element, so that nothing outside the tensor is
+// touched.  (Pieces of the row's own columns, shifted at every load and store through
+// shuffles: [16384, 1001] f32 37 us forward and 68 backward, instead of 27 and 52.)
+// The kernels for rows beyond a CTA's registers read two aligned pieces for one.
 #include "kernels.h"
 #include "ops_common.cuh"
 
@@ -64,8 +64,9 @@ union Piece {
     __device__ Piece() {}
 };
 
-// w[k] = the four bytes from byte 4 k + o of the 32 bytes a || b, 0 <= o < 16.
-// w may be a or b.
+// w[k] = the four bytes from byte 4 k + o of the 32 bytes a || b, 0 <= o < 16, a
+// multiple of T's size.  w may be a or b.
+template <typename T>
 __device__ __forceinline__ void shift_bytes(uint32_t (&w)[4], const uint32_t (&a)[4],
                                             const uint32_t (&b)[4], unsigned o) {
     uint32_t c[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -73,12 +74,12 @@ __device__ __forceinline__ void shift_bytes(uint32_t (&w)[4], const uint32_t (&a
 #pragma unroll
         for (int k = 0; k < 6; k++) c[k] = c[k + 2];
     }
-    if (o & 4) {
+    if (sizeof(T) < 8 && (o & 4)) {
 #pragma unroll
         for (int k = 0; k < 5; k++) c[k] = c[k + 1];
     }
 #pragma unroll
-    for (int k = 0; k < 4; k++) w[k] = __funnelshift_r(c[k], c[k + 1], (o & 3) * 8);
+    for (int k = 0; k < 4; k++) w[k] = sizeof(T) < 4 ? __funnelshift_r(c[k], c[k + 1], (o & 3) * 8) : c[k];
 }
 
 __device__ __forceinline__ void load16(uint32_t (&w)[4], const void* p) {
@@ -161,13 +162,13 @@ template <typename T>
 __device__ __forceinline__ void keep_packed(Piece<T>& p) {
     asm volatile("" : "+r"(p.w[0]), "+r"(p.w[1]), "+r"(p.w[2]), "+r"(p.w[3]));
 }
-// v's values from element n on as zeros.
-__device__ __forceinline__ void keep_first(F2& v, int n) {
-    if (n < 2) v.y = 0.0f;
-    if (n < 1) v.x = 0.0f;
+// v's values outside columns [0, cols) as zeros; c: its first column.
+__device__ __forceinline__ void keep_inside(F2& v, int c, unsigned cols) {
+    if ((unsigned)c >= cols) v.x = 0.0f;
+    if ((unsigned)(c + 1) >= cols) v.y = 0.0f;
 }
-__device__ __forceinline__ void keep_first(double& v, int n) {
-    if (n < 1) v = 0.0;
+__device__ __forceinline__ void keep_inside(double& v, int c, unsigned cols) {
+    if ((unsigned)c >= cols) v = 0.0;
 }
 
 // Less than 16 bytes of the tensor before or behind the row, or no such row.
@@ -193,7 +194,7 @@ __device__ __forceinline__ void row_load(Piece<T>& v, const T* p, unsigned i, un
             uint32_t a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
             if (16 * i < end) load16(a, base);
             if (16 * i + 16 < end) load16(b, base + 16);
-            shift_bytes(v.w, a, b, s);
+            shift_bytes<T>(v.w, a, b, s);
             if (i * V + V > cols) {
 #pragma unroll
                 for (unsigned e = 0; e < V; e++)
@@ -208,42 +209,75 @@ __device__ __forceinline__ void row_load(Piece<T>& v, const T* p, unsigned i, un
     }
 }
 
-// The same in two steps, for loads that are to be in flight for long: the piece
-// as the aligned pieces lie in memory (the first of its two), and, at its use, the
-// rest from the next lane (the last of the `width` lanes that hold the row's
-// consecutive pieces loads it).  Whole warps.
+// ---- rows in the pieces of their memory
+//
+// Piece i of a row holds the aligned 16 bytes i of the memory that the row of x lies
+// in: columns i V - sh .., of which those outside [0, cols) belong to other rows
+// (sh = the elements before the row in its first piece; 0 with AL).
+
+__device__ __forceinline__ bool outside(int c, unsigned cols) { return (unsigned)c >= cols; }
+
+// Some of the piece's columns lie in the row and some do not.
 template <typename T, bool AL>
-__device__ __forceinline__ void raw_load(Piece<T>& v, const T* p, unsigned i, unsigned cols, bool edge) {
-    const unsigned s = AL ? 0 : (unsigned)((uintptr_t)p & 15);
-    if (s == 0 || edge) {
-        row_load<T, AL>(v, p, i, cols, edge);
-    } else {
+__device__ __forceinline__ bool cut(unsigned i, unsigned sh, unsigned cols) {
+    constexpr unsigned V = kV<T>;
+    return !AL && ((i == 0 && sh > 0) || (i * V < sh + cols && i * V + V > sh + cols));
+}
+
+// apart: element by element (an edge_row; a tensor that does not lie as x does);
+// otherwise the columns outside the row are whatever is there, until clear_cut.
+template <typename T, bool AL>
+__device__ __forceinline__ void piece_load(Piece<T>& v, const T* p, unsigned i, unsigned sh, unsigned cols,
+                                           bool apart) {
+    constexpr unsigned V = kV<T>;
+    if constexpr (AL) {
+        row_load<T, true>(v, p, i, cols, false);
+    } else if (!apart) {
         v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0;
-        if (16 * i < s + cols * (unsigned)sizeof(T)) load16(v.w, (const char*)p - s + 16 * (size_t)i);
+        if (i * V < sh + cols) load16(v.w, (const char*)p + 16 * (size_t)i - sh * sizeof(T));
+    } else {
+        const int c = (int)(i * V) - (int)sh;
+#pragma unroll
+        for (int e = 0; e < (int)V; e++) v.e[e] = outside(c + e, cols) ? T(0.0f) : p[c + e];
     }
 }
+// The columns outside the row of a piece that is cut as zeros.
+template <typename T>
+__device__ __forceinline__ void clear_cut(Piece<T>& v, unsigned i, unsigned sh, unsigned cols) {
+    const int c = (int)(i * kV<T>) - (int)sh;
+#pragma unroll
+    for (int e = 0; e < kV<T>; e++)
+        if (outside(c + e, cols)) v.e[e] = T(0.0f);
+}
 template <typename T, bool AL>
-__device__ __forceinline__ void realign(Piece<T>& v, const T* p, unsigned i, unsigned cols, bool edge,
-                                        unsigned lane, unsigned width) {
+__device__ __forceinline__ void piece_store(T* p, const Piece<T>& v, unsigned i, unsigned sh, unsigned cols,
+                                            bool apart) {
     constexpr unsigned V = kV<T>;
-    if constexpr (!AL) {
-        const unsigned s = edge ? 0 : (unsigned)((uintptr_t)p & 15);
-        uint32_t next[4], far[4] = {0, 0, 0, 0};
-        const bool last = lane + 1 == width;
-        if (last && s != 0 && 16 * i + 16 < s + cols * (unsigned)sizeof(T))
-            load16(far, (const char*)p - s + 16 * (size_t)i + 16);
+    if (AL || (!apart && !cut<T, AL>(i, sh, cols))) {
+        if (i * V < sh + cols)
+            *reinterpret_cast<uint4*>((char*)p + 16 * (size_t)i - sh * sizeof(T)) =
+                make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    } else {
+        const int c = (int)(i * V) - (int)sh;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            next[w] = __shfl_down_sync(0xffffffffu, v.w[w], 1);
-            if (last) next[w] = far[w];
+        for (int e = 0; e < (int)V; e++)
+            if (!outside(c + e, cols)) p[c + e] = v.e[e];
+    }
+}
+// The same columns of a vector of weights, what lies outside [0, cols) as zeros.
+template <typename T>
+__device__ __forceinline__ void weights_load(Piece<T>& v, const T* g, unsigned i, unsigned sh, unsigned cols) {
+    constexpr unsigned V = kV<T>;
+    // the aligned pieces i - 1 and i of the weights' own memory
+    if ((((uintptr_t)g & 15) == 0) && i * V + V <= cols && (i > 0 || sh == 0)) {
+        load16(v.w, g + (size_t)i * V);
+        if (sh) {
+            uint32_t a[4];
+            load16(a, g + (size_t)(i - 1) * V);
+            shift_bytes<T>(v.w, a, v.w, (V - sh) * (unsigned)sizeof(T));
         }
-        if (s == 0) return;
-        shift_bytes(v.w, v.w, next, s);
-        if (i * V + V > cols) {
-#pragma unroll
-            for (unsigned e = 0; e < V; e++)
-                if (i * V + e >= cols) v.e[e] = T(0.0f);
-        }
+    } else {
+        piece_load<T, false>(v, g, i, sh, cols, true);
     }
 }
 
@@ -274,7 +308,7 @@ __device__ __forceinline__ void row_store(T* p, const Piece<T>& v, unsigned i, u
             }
             return;
         }
-        shift_bytes(out, prev, v.w, 16 - s);
+        shift_bytes<T>(out, prev, v.w, 16 - s);
         // aligned piece i (the end of piece i - 1, the start of piece i): whole within the row
         const bool mine = lane > 0 && 16 * i + 16 <= s + bytes;
         const bool next = lane + 1 < width && 16 * i + 32 <= s + bytes;  // piece i + 1's lane will
@@ -302,35 +336,59 @@ __device__ __forceinline__ A rsqrt_exact(A v) {
 }
 
 // Forward: a row in the registers of a group of G = 32, 64, .. threads (blockDim.x),
-// blockDim.y rows a CTA (more than one only with one warp a row, where there
-// is no barrier).  Up to 16 pieces a thread are loaded before anything waits for
-// them: with 20 warps an SM, 160 KB in flight.
+// blockDim.y rows a CTA.  A thread's 4 or 8 (of the longest rows 16) pieces are loaded
+// before anything waits for them.
+// AL: more than one row a CTA only with one warp a row, where there is no barrier.
+// Otherwise the CTA's rows are 2^lgp apart, so that they start at the same place of
+// a piece, and share gamma and beta, shifted to it, in shared memory (2 `room`
+// elements): [16384, 1001] f32 27 us (every thread shifting them for itself 41 us).
 template <typename T, int NV, bool AL>
 __global__ void __launch_bounds__(NV > 8 ? 512 : 1024)
 k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const T* x,
            const T* __restrict__ gamma, const T* __restrict__ beta, unsigned rows, unsigned cols,
-           acc_t<T> eps) {
+           acc_t<T> eps, unsigned lgp, unsigned room) {
     using A = acc_t<T>;
     using W = vec_t<T>;
     constexpr int V = kV<T>, N = kN<T>, NP = kP<T>;
     __shared__ A red[2][32];
+    extern __shared__ __align__(16) unsigned char mem[];
     const unsigned t = threadIdx.x, G = blockDim.x, lane = t & 31, warps = G >> 5;
+    const unsigned w0 = threadIdx.y * warps;  // the row's first warp
     auto total = [&](A v, int which) {
         v = warp_sum(v);
         if (warps == 1) return v;
-        if (lane == 0) red[which][t >> 5] = v;
+        if (lane == 0) red[which][w0 + (t >> 5)] = v;
         __syncthreads();
-        return warp_sum(lane < warps ? red[which][lane] : A(0));
+        return warp_sum(lane < warps ? red[which][w0 + lane] : A(0));
     };
-    const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= rows) return;  // whole warps: blockDim.y > 1 has no barriers
+    const unsigned P = 1u << lgp;
+    const size_t row = AL ? (size_t)blockIdx.x * blockDim.y + threadIdx.y
+                          : (((size_t)(blockIdx.x >> lgp) * blockDim.y + threadIdx.y) << lgp) + (blockIdx.x & (P - 1));
+    if (AL && row >= rows) return;  // whole warps: blockDim.y > 1 has no barriers
+    const bool live = AL || row < rows;
     const T* xr = x + row * cols;
     Piece<T> p[NV];
+    const unsigned sh = AL ? 0 : (unsigned)((uintptr_t)xr & 15) / (unsigned)sizeof(T);
     const bool edge = edge_row<T>(row, rows, cols);
 #pragma unroll
-    for (int k = 0; k < NV; k++) raw_load<T, AL>(p[k], xr, t + k * G, cols, edge);
+    for (int k = 0; k < NV; k++) {
+        if (live) piece_load<T, AL>(p[k], xr, t + k * G, sh, cols, edge);
+        else p[k].w[0] = p[k].w[1] = p[k].w[2] = p[k].w[3] = 0;
+    }
+    T* sg = reinterpret_cast<T*>(mem);
+    if constexpr (!AL) {
+        for (unsigned i = threadIdx.y * G + t; i * V < room; i += G * blockDim.y) {
+            Piece<T> g, b;
+            weights_load(g, gamma, i, sh, cols);
+            weights_load(b, beta, i, sh, cols);
+            *reinterpret_cast<uint4*>(sg + (size_t)i * V) = make_uint4(g.w[0], g.w[1], g.w[2], g.w[3]);
+            *reinterpret_cast<uint4*>(sg + room + (size_t)i * V) = make_uint4(b.w[0], b.w[1], b.w[2], b.w[3]);
+        }
+        __syncthreads();
+    }
 #pragma unroll
-    for (int k = 0; k < NV; k++) realign<T, AL>(p[k], xr, t + k * G, cols, edge, lane, 32);
+    for (int k = 0; k < NV; k++)
+        if (cut<T, AL>(t + k * G, sh, cols)) clear_cut(p[k], t + k * G, sh, cols);
     W s = vset(A(0), (W*)0);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -344,31 +402,42 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
     s = vset(A(0), (W*)0);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const unsigned at = (t + k * G) * V;
-        if (at < cols) {
+        const unsigned i = t + k * G;
+        if (i * V < sh + cols) {
             W v[NP];
             keep_packed(p[k]);
             unpack(v, p[k]);
+            if (cut<T, AL>(i, sh, cols)) {
 #pragma unroll
-            for (int e = 0; e < NP; e++) {
-                W c = vadd(v[e], mm);
-                if (!AL && at + V > cols) keep_first(c, (int)(cols - at) - e * N);
-                s = vfma(c, c, s);
+                for (int e = 0; e < NP; e++) {
+                    W c = vadd(v[e], mm);
+                    keep_inside(c, (int)(i * V) - (int)sh + e * N, cols);
+                    s = vfma(c, c, s);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < NP; e++) {
+                    const W c = vadd(v[e], mm);
+                    s = vfma(c, c, s);
+                }
             }
         }
     }
     const A rs = rsqrt_exact(div_(total(vsum(s), 1), A(cols)) + eps);
+    if (!live) return;
     if (t == 0) {
         mean[row] = m;
         rstd[row] = rs;
     }
     const W rr = vset(rs, (W*)0);
+    const bool y_apart = !AL && (((uintptr_t)y ^ (uintptr_t)x) & 15);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        if (!AL || (t + k * G) * V < cols) {
+        const unsigned i = t + k * G;
+        if (i * V < sh + cols) {
             Piece<T> g, b;
-            row_load<T, AL>(g, gamma, t + k * G, cols, true);
-            row_load<T, AL>(b, beta, t + k * G, cols, true);
+            load16(g.w, AL ? gamma + (size_t)i * V : sg + (size_t)i * V);
+            load16(b.w, AL ? beta + (size_t)i * V : sg + room + (size_t)i * V);
             W v[NP], gv[NP], bv[NP];
             keep_packed(p[k]);
             unpack(v, p[k]);
@@ -377,7 +446,7 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
 #pragma unroll
             for (int e = 0; e < NP; e++) v[e] = vfma(vmul(vadd(v[e], mm), rr), gv[e], bv[e]);
             pack(p[k], v);
-            row_store<T, AL>(y + row * cols, p[k], t + k * G, cols, lane, 32, true);
+            piece_store<T, AL>(y + row * cols, p[k], i, sh, cols, y_apart);
         }
     }
 }
@@ -439,10 +508,13 @@ __device__ __forceinline__ double peer_value(const double* p, unsigned rank) {
     return v;
 }
 
-// Backward: how the rows are dealt out: G threads (a power of two, lg its
-// logarithm) take R rows at a time; rounds of all the CTA's groups.
+// Backward: how the rows are dealt out: G threads (a power of two, lg its logarithm)
+// take R rows at a time.  Rows r and r + 2^lgp start at the same place of a 16-byte
+// piece (lgp = 0 where all do), and a group takes rows of one such class only: a
+// thread's pieces then hold the same columns of all of them.  units: the most R
+// rows of a class.
 struct Deal {
-    unsigned rows, cols, G, lg, rounds;
+    unsigned rows, cols, G, lg, lgp, units;
 };
 constexpr int kBwdThreads = 512;
 
@@ -522,39 +594,58 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
     const unsigned tid = threadIdx.x, cols = d.cols, G = d.G;
     const A inv = A(1) / A(cols);
     const unsigned t = tid & (G - 1), q = tid >> d.lg, groups = kBwdThreads >> d.lg;
-    const unsigned width = G < 32 ? G : 32, lane = t & (width - 1);
+    // the group's class and its place among the class's groups
+    const unsigned P = 1u << d.lgp, all = gridDim.x * groups, id0 = blockIdx.x * groups, id = id0 + q;
+    const unsigned cls = id & (P - 1), mates = (all - cls + P - 1) >> d.lgp;
+    const unsigned fewest = max(all >> d.lgp, 1u);  // groups of a class
+    auto shift_of = [&](unsigned c) -> unsigned {
+        return AL ? 0 : (unsigned)((uintptr_t)(x + (size_t)c * cols) & 15) / (unsigned)sizeof(T);
+    };
+    const unsigned sh = shift_of(cls);
+    const bool dy_apart = !AL && (((uintptr_t)dy ^ (uintptr_t)x) & 15);
+    const bool dx_apart = !AL && (((uintptr_t)dx ^ (uintptr_t)x) & 15);
     Piece<T> g[NV];
     W ag[NV][NP], ab[NV][NP];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        row_load<T, AL>(g[k], gamma, t + k * G, cols, true);
+        piece_load<T, AL>(g[k], gamma, t + k * G, sh, cols, true);
 #pragma unroll
         for (int e = 0; e < NP; e++) ag[k][e] = ab[k][e] = vset(A(0), (W*)0);
     }
-    const unsigned per_round = groups * R;
-    auto prefetch = [&](unsigned u) {
-        if (u >= d.rounds) return;
-        const size_t r0 = (size_t)u * per_round;
-        const unsigned n = (unsigned)min((size_t)per_round, d.rows - r0);
-        prefetch_rows(x, r0, n, cols);
-        prefetch_rows(dy, r0, n, cols);
+    // the first of the R rows (P apart) of the group's turn `it`
+    auto first_row = [&](unsigned it) { return cls + (((size_t)(id >> d.lgp) + (size_t)it * mates) * R << d.lgp); };
+    auto prefetch = [&](unsigned it) {
+        if (groups >= P) {  // the CTA's rows are consecutive
+            const size_t r0 = ((size_t)(id0 >> d.lgp) + (size_t)it * fewest) * R << d.lgp;
+            if (tid != 0 || r0 >= d.rows) return;
+            const unsigned n = (unsigned)min((size_t)groups * R, d.rows - r0);
+            prefetch_rows(x, r0, n, cols);
+            prefetch_rows(dy, r0, n, cols);
+        } else if (t == 0) {
+            for (int r = 0; r < R; r++) {
+                const size_t row = first_row(it) + ((size_t)r << d.lgp);
+                if (row >= d.rows) return;
+                prefetch_rows(x, row, 1, cols);
+                prefetch_rows(dy, row, 1, cols);
+            }
+        }
     };
-    if (tid == 0) prefetch(blockIdx.x + gridDim.x);
-    for (unsigned u = blockIdx.x, turn = 0; u < d.rounds; u += gridDim.x, turn ^= 1) {
-        if (tid == 0) prefetch(u + 2 * gridDim.x);
+    prefetch(1);
+    for (unsigned it = 0, turn = 0; (size_t)(id0 >> d.lgp) + (size_t)it * fewest < d.units; it++, turn ^= 1) {
+        prefetch(it + 2);
         // this group's rows; the last ones may lie past the tensor
-        const size_t row0 = (size_t)u * per_round + (size_t)q * R;
+        const size_t row0 = first_row(it);
         Piece<T> vx[R][NV], vd[R][NV];
         A m[R], rs[R], sum[2 * R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const size_t row = row0 + r;
+            const size_t row = row0 + ((size_t)r << d.lgp);
             const bool live = row < d.rows, edge = edge_row<T>(row, d.rows, cols);
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 if (live) {
-                    raw_load<T, AL>(vx[r][k], x + row * cols, t + k * G, cols, edge);
-                    raw_load<T, AL>(vd[r][k], dy + row * cols, t + k * G, cols, edge);
+                    piece_load<T, AL>(vx[r][k], x + row * cols, t + k * G, sh, cols, edge);
+                    piece_load<T, AL>(vd[r][k], dy + row * cols, t + k * G, sh, cols, edge || dy_apart);
                 } else {
 #pragma unroll
                     for (int w = 0; w < 4; w++) vx[r][k].w[w] = vd[r][k].w[w] = 0;
@@ -565,14 +656,14 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
         }
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const size_t row = row0 + r;
-            const bool edge = edge_row<T>(row, d.rows, cols);
             const W mm = vset(-m[r], (W*)0), rr = vset(rs[r], (W*)0);
             W a0 = vset(A(0), (W*)0), a1 = a0;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
-                realign<T, AL>(vx[r][k], x + row * cols, t + k * G, cols, edge, lane, width);
-                realign<T, AL>(vd[r][k], dy + row * cols, t + k * G, cols, edge, lane, width);
+                if (cut<T, AL>(t + k * G, sh, cols)) {
+                    clear_cut(vx[r][k], t + k * G, sh, cols);
+                    clear_cut(vd[r][k], t + k * G, sh, cols);
+                }
                 keep_packed(g[k]);
                 W xv[NP], dv[NP], gv[NP];
                 unpack(xv, vx[r][k]);
@@ -580,7 +671,7 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
                 unpack(gv, g[k]);
 #pragma unroll
                 for (int e = 0; e < NP; e++) {
-                    // dy is zero past the row
+                    // dy is zero outside the row
                     const W tt = vadd(xv[e], mm), w = vmul(dv[e], gv[e]);
                     a0 = vadd(a0, w);
                     a1 = vfma(w, tt, a1);
@@ -593,7 +684,7 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
         group_sum<A, 2 * R>(sum, G, red[turn]);
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const size_t row = row0 + r;
+            const size_t row = row0 + ((size_t)r << d.lgp);
             const W mm = vset(-m[r], (W*)0), rr = vset(rs[r], (W*)0);
             const W c1 = vset(-rs[r] * (sum[2 * r] * inv), (W*)0);
             const W c2 = vset(-rs[r] * (rs[r] * (rs[r] * (sum[2 * r + 1] * inv))), (W*)0);
@@ -610,12 +701,13 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
                 for (int e = 0; e < NP; e++)
                     xv[e] = vfma(vadd(xv[e], mm), c2, vfma(vmul(dv[e], rr), gv[e], c1));
                 pack(vx[r][k], xv);
-                row_store<T, AL>(dx + row * cols, vx[r][k], t + k * G, cols, lane, width, row < d.rows);
+                if (row < d.rows) piece_store<T, AL>(dx + row * cols, vx[r][k], t + k * G, sh, cols, dx_apart);
             }
         }
     }
-    A* sh = reinterpret_cast<A*>(mem);
     const unsigned pad = (NV * V) << d.lg;  // a group's columns
+    A* sums = reinterpret_cast<A*>(mem);
+    A* folded = sums + (size_t)groups * pad;  // with dgamma
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         A* out = part + ((size_t)which * gridDim.x + blockIdx.x) * cols;
@@ -624,19 +716,20 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int e = 0; e < NP; e++)
-                *reinterpret_cast<W*>(&sh[(size_t)q * pad + (t + k * G) * V + e * N]) = which ? ab[k][e] : ag[k][e];
+                *reinterpret_cast<W*>(&sums[(size_t)q * pad + (t + k * G) * V + e * N]) = which ? ab[k][e] : ag[k][e];
         __syncthreads();
         for (unsigned c = tid; c < cols; c += kBwdThreads) {
-            A v = sh[c];
-            for (unsigned j = 1; j < groups; j++) v += sh[(size_t)j * pad + c];
-            if (dgamma) sh[c] = v;  // this thread's own column
+            A v = A(0);
+            for (unsigned j = 0; j < groups; j++)
+                v += sums[(size_t)j * pad + c + shift_of((id0 + j) & (P - 1))];
+            if (dgamma) folded[c] = v;
             else out[c] = v;
         }
         if (dgamma) {
             cluster_sync();
             for (unsigned c = blockIdx.x * kBwdThreads + tid; c < cols; c += gridDim.x * kBwdThreads) {
                 A v = A(0);
-                for (unsigned j = 0; j < gridDim.x; j++) v += peer_value(&sh[c], j);
+                for (unsigned j = 0; j < gridDim.x; j++) v += peer_value(&folded[c], j);
                 from_acc((which ? dbeta : dgamma)[c], v);
             }
             cluster_sync();  // the peers have read this CTA's sums
@@ -796,31 +889,55 @@ bool all_aligned(unsigned cols, std::initializer_list<const void*> ps) {
     return true;
 }
 
+// log2 of the rows after which a row starts at the same place of a 16-byte piece.
+template <typename T>
+unsigned row_classes(unsigned cols) {
+    unsigned lgp = 0;
+    while (((size_t)cols << lgp) % kV<T>) lgp++;
+    return lgp;
+}
+
 template <typename T, bool AL>
-void fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, const T* b,
+int fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, const T* b,
          unsigned rows, unsigned cols, acc_t<T> eps) {
-    const size_t nv = ((size_t)cols + kV<T> - 1) / kV<T>;
+    // a row that starts inside a piece may take one more
+    const size_t nv = ((size_t)cols + (AL ? 1 : 2) * (kV<T> - 1)) / kV<T>;
     if (nv > 16 * 512) {
         k_norm_fwd_long<T><<<std::min(rows, (unsigned)c.dev->sm_count * 2), 1024, 0, c.stream>>>(
             y, mean, rstd, x, g, b, rows, cols, eps);
-        return;
+        return OK;
     }
-    // Many rows: up to 16 pieces a thread, no barrier for rows of up to 8 KB.
-    // Few rows (less than 16 warps an SM with a warp each): 4, for latency.
-    const bool many = rows >= (unsigned)c.dev->sm_count * 16;
-    const unsigned per = many || nv > 4 * 512 ? 16 : 4;
-    const unsigned tx = (unsigned)((nv + per - 1) / per + 31) / 32 * 32;
-    const unsigned ty = tx == 32 ? 4 : 1, k = (unsigned)((nv + tx - 1) / tx);
+    // Pieces a thread: 8 where the rows come from memory, 4, with more threads a row,
+    // where they come from L2 and latency counts ([32768, 4096] bf16 84.0 us with 8, 84.5
+    // with 4, 89.2 with 16; [3000, 4096] 12.6, 10.5, 14.5).  Where gamma and beta are shifted
+    // into shared memory f32 and f64 gain from 8 sooner ([3000, 2049] f32 15.3 us and 16.5,
+    // [500, 4001] 10.3 and 8.4), bf16 later ([16384, 3001] 59.6 and 52.6, [8192, 8001] 72 and 78).
+    const size_t mb = ((size_t)rows * cols * sizeof(T)) >> 20;
+    unsigned per = (AL ? mb >= 64 : kV<T> == 8 ? nv > 768 : mb >= 16) ? 8 : 4;
+    while (nv > per * 512) per *= 2;
+    const unsigned tx = (unsigned)((nv + per - 1) / per + 31) / 32 * 32, k = (unsigned)((nv + tx - 1) / tx);
     auto f = k <= 1   ? k_norm_fwd<T, 1, AL>
              : k <= 2 ? k_norm_fwd<T, 2, AL>
              : k <= 4 ? k_norm_fwd<T, 4, AL>
              : k <= 8 ? k_norm_fwd<T, 8, AL>
                       : k_norm_fwd<T, 16, AL>;
-    for (size_t r0 = 0; r0 < rows; r0 += 1u << 30) {  // the grid's limit
-        const unsigned n = (unsigned)std::min<size_t>(rows - r0, 1u << 30);
-        f<<<(n + ty - 1) / ty, dim3(tx, ty), 0, c.stream>>>(y + r0 * cols, mean + r0, rstd + r0, x + r0 * cols, g,
-                                                          b, n, cols, eps);
+    unsigned ty = tx == 32 ? 4 : 1, lgp = 0;
+    const unsigned room = AL ? 0 : (unsigned)(nv * kV<T>), bytes = 2 * room * (unsigned)sizeof(T);
+    if (!AL) {
+        lgp = row_classes<T>(cols);
+        // Rows that share gamma and beta: 256 threads (of longer rows 512), as long as two
+        // CTAs an SM remain ([16384, 1001] f32 with 32, 128, 256, 512 threads 64, 29, 28, 29 us).
+        const unsigned most = tx == 32 ? 256 : 512;
+        for (ty = 1; 2 * ty * tx <= most && rows >= (size_t)c.dev->sm_count * 4 * ty; ty *= 2) {}
+        NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     }
+    const unsigned part = AL ? 1u << 30 : 1u << 27;  // rows of a launch, within the grid's limit
+    for (size_t r0 = 0; r0 < rows; r0 += part) {
+        const unsigned n = (unsigned)std::min<size_t>(rows - r0, part), P = 1u << lgp;
+        f<<<((n + P - 1) / P + ty - 1) / ty * P, dim3(tx, ty), bytes, c.stream>>>(
+            y + r0 * cols, mean + r0, rstd + r0, x + r0 * cols, g, b, n, cols, eps, lgp, room);
+    }
+    return OK;
 }
 
 template <typename T>
@@ -828,7 +945,7 @@ int fwd_t(Ctx& c, void* y, void* mean, void* rstd, const void* x, const void* g,
           unsigned rows, unsigned cols, double eps) {
     using A = acc_t<T>;
     auto f = all_aligned<T>(cols, {y, x, g, b}) ? fwd<T, true> : fwd<T, false>;
-    f(c, (T*)y, (A*)mean, (A*)rstd, (const T*)x, (const T*)g, (const T*)b, rows, cols, (A)eps);
+    if (int rc = f(c, (T*)y, (A*)mean, (A*)rstd, (const T*)x, (const T*)g, (const T*)b, rows, cols, (A)eps)) return rc;
     count_launch();
     pdl_record_all(c);
     return finish(c);
@@ -844,11 +961,13 @@ constexpr unsigned kBwdCtas = 148;  // of a B200; fixed, as the workspace's size
 template <typename T> constexpr int kPer = kV<T> == 8 ? 2 : 4;   // pieces a thread: at most 16 columns' sums
 template <typename T> constexpr int kRows = kV<T> == 8 ? 2 : 1;  // rows at a time
 template <typename T>
-BwdShape bwd_shape_t(unsigned rows, unsigned cols) {
-    const size_t nv = ((size_t)cols + kV<T> - 1) / kV<T>;
+BwdShape bwd_shape_t(unsigned rows, unsigned cols, bool aligned) {
+    constexpr unsigned V = kV<T>;
+    // a row that starts inside a piece may take one more
+    const size_t nv = ((size_t)cols + (aligned ? 1 : 2) * (V - 1)) / V;
     BwdShape q{};
     if (nv > (size_t)kBwdThreads * kPer<T>) {
-        q.strips = (unsigned)((nv + 255) / 256);
+        q.strips = (unsigned)(((size_t)cols + 256 * V - 1) / (256 * V));
         q.grid = q.parts = std::min((rows + 3) / 4, (kBwdCtas * 4 + q.strips - 1) / q.strips);
         return q;
     }
@@ -856,14 +975,18 @@ BwdShape bwd_shape_t(unsigned rows, unsigned cols) {
     d.rows = rows;
     d.cols = cols;
     for (d.G = 4, d.lg = 2; (size_t)d.G * kPer<T> < nv; d.lg++) d.G *= 2;
-    const size_t per_round = (size_t)(kBwdThreads / d.G) * kRows<T>;
-    d.rounds = (unsigned)((rows + per_round - 1) / per_round);
-    q.grid = q.parts = std::min(d.rounds, kBwdCtas);
+    d.lgp = aligned ? 0 : row_classes<T>(cols);
+    const size_t P = (size_t)1 << d.lgp, groups = kBwdThreads / d.G, per_round = groups * kRows<T>;
+    d.units = (unsigned)(((rows + P - 1) / P + kRows<T> - 1) / kRows<T>);
+    // and a group for every class that has a row
+    const size_t rounds = std::max((rows + per_round - 1) / per_round, (std::min<size_t>(rows, P) + groups - 1) / groups);
+    q.grid = q.parts = (unsigned)std::min<size_t>(rounds, kBwdCtas);
     return q;
 }
-BwdShape bwd_shape(unsigned rows, unsigned cols, int dt) {
-    return dt == F32 ? bwd_shape_t<float>(rows, cols) : dt == F64 ? bwd_shape_t<double>(rows, cols)
-                                                                  : bwd_shape_t<bf16>(rows, cols);
+BwdShape bwd_shape(unsigned rows, unsigned cols, int dt, bool aligned) {
+    return dt == F32   ? bwd_shape_t<float>(rows, cols, aligned)
+           : dt == F64 ? bwd_shape_t<double>(rows, cols, aligned)
+                       : bwd_shape_t<bf16>(rows, cols, aligned);
 }
 size_t bwd_part_bytes(const BwdShape& q, unsigned cols, int dt) {
     return (size_t)2 * q.parts * cols * (dt == F64 ? 8 : 4);
@@ -884,11 +1007,11 @@ int bwd(Ctx& c, const BwdShape& q, T* dx, T* dg, T* db, acc_t<T>* part, acc_t<T>
         count_launch(2);
         return OK;
     }
-    const bool one = ((size_t)cols + kV<T> - 1) / kV<T> <= q.deal.G;
+    const bool one = ((size_t)cols + (AL ? 1 : 2) * (kV<T> - 1)) / kV<T> <= q.deal.G;
     auto f = one ? k_norm_bwd<T, 1, kRows<T>, AL> : k_norm_bwd<T, kPer<T>, kRows<T>, AL>;
-    const size_t bytes = (size_t)kBwdThreads * (one ? 1 : kPer<T>) * kV<T> * sizeof(acc_t<T>);
-    NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     const bool fold = one_cluster(q);
+    const size_t bytes = ((size_t)kBwdThreads * (one ? 1 : kPer<T>) * kV<T> + (fold ? cols : 0)) * sizeof(acc_t<T>);
+    NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(q.grid);
     cfg.blockDim = dim3(kBwdThreads);
@@ -910,9 +1033,10 @@ template <typename T>
 int bwd_t(Ctx& c, int dt, void* dx, void* dg, void* db, void* ws, const void* dy, const void* x,
           const void* g, const void* mean, const void* rstd, unsigned rows, unsigned cols) {
     using A = acc_t<T>;
-    const BwdShape q = bwd_shape(rows, cols, dt);
+    const bool aligned = all_aligned<T>(cols, {dx, dy, x, g});
+    const BwdShape q = bwd_shape(rows, cols, dt, aligned);
     if (rows > 0) {
-        auto f = all_aligned<T>(cols, {dx, dy, x, g}) ? bwd<T, true> : bwd<T, false>;
+        auto f = aligned ? bwd<T, true> : bwd<T, false>;
         const int rc = f(c, q, (T*)dx, (T*)dg, (T*)db, (A*)ws, (A*)((char*)ws + bwd_part_bytes(q, cols, dt)),
                          (const T*)dy, (const T*)x, (const T*)g, (const A*)mean, (const A*)rstd, rows,
                          cols);
@@ -930,10 +1054,14 @@ int bwd_t(Ctx& c, int dt, void* dx, void* dg, void* db, void* ws, const void* dy
 }  // namespace
 
 // The backward kernel's partial rows of dgamma and dbeta, and for strips two
-// sums of every row.
+// sums of every row; for aligned tensors and for others.
 size_t norm_grad_workspace(unsigned rows, unsigned cols, int dt) {
-    const BwdShape q = bwd_shape(rows, cols, dt);
-    return bwd_part_bytes(q, cols, dt) + (q.strips ? (size_t)2 * rows * (dt == F64 ? 8 : 4) : 0);
+    size_t most = 0;
+    for (bool aligned : {false, true}) {
+        const BwdShape q = bwd_shape(rows, cols, dt, aligned);
+        most = std::max(most, bwd_part_bytes(q, cols, dt) + (q.strips ? (size_t)2 * rows * (dt == F64 ? 8 : 4) : 0));
+    }
+    return most;
 }
 
 int launch_layer_norm(Ctx& c, int dt, void* y, void* mean, void* rstd, const void* x,
