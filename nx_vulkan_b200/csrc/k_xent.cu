@@ -9,8 +9,8 @@
 //
 // Three matrix products of 2 n vocab dim operations each, and z once more in
 // the backward pass because it is not kept: 8 n vocab dim in all, on the
-// tcgen05 tensor cores.  All go through one kernel, k_xgemm, with an epilogue
-// each:
+// tcgen05 tensor cores (few rows and small problems have kernels of their own, further
+// down).  All go through one kernel, k_xgemm, with an epilogue each:
 //   LSE   the maximum and the sum of exponentials of every row over a segment
 //         of classes (8 bytes per row and segment instead of the logits) and
 //         the label's logit; a small kernel joins the segments;
@@ -1201,6 +1201,257 @@ k_sum(const __grid_constant__ SumWork w) {
     }
 }
 
+// ---- few rows ---------------------------------------------------------------------
+//
+// A few rows (one token's score, a handful of sequences): a product with them is a
+// pass over w, bound by its bytes, and the tensor cores' 128-row tiles would be empty.
+// k_few_z: x in shared memory as f32; a warp takes kFewC classes at a time, the lanes
+// 16 bytes each of their rows, and every value of x that is read serves kFewC
+// classes; then the lanes part the sums among them, one (class, row) each, which keeps
+// its own running maximum and sum (forward) or stores P (backward).
+// k_few_out: a thread holds some columns of x and of dx's sums in registers and goes
+// down a slab of classes: dx += P w, dw = P^T (dloss x), w read and dw written once.
+// All in f32, rounded once at the end.
+// Measured, 1 x 65536 x 2048: f32 86 us forward (w alone 82 at the measured copy rate),
+// 272 us the gradient (w twice and dw 246); bf16 50 and 147 us (41 and 123).
+
+constexpr unsigned kFewRows = 8, kFewC = 4;
+constexpr unsigned kFewX = 16384;       // values of x: 64 KB of shared memory
+constexpr unsigned kFewCtas = 148 * 2;  // fixed, as the workspace must not depend on the device
+
+struct Few {
+    const void *x, *w, *labels;
+    int index_bytes;
+    unsigned n, vocab, dim;
+    float *part_m, *part_s, *zlabel;  // forward: [CTA][n], [CTA][n], [n]
+    const float *lse, *dloss;
+    float* p;     // backward: [vocab][NB]
+    float* part;  // [slab][n][dim]
+    void *dx, *dw;
+    unsigned parts;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(float (&v)[VEC], const T* p) {
+    alignas(16) T e[VEC];
+    if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (VEC * sizeof(T) == 8) *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+    else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; i++) v[i] = f32_of(e[i]);
+}
+
+// VEC: 16 bytes of w where its rows are aligned, else 1.  blockIdx.y: NB of the rows
+// (the gradient has one such block only).
+template <typename T, int NB, int VEC, bool GRADIENT>
+__global__ void __launch_bounds__(256, 2)
+k_few_z(const __grid_constant__ Few f) {
+    constexpr int C = kFewC, M = C * NB, U = VEC > 1 ? 2 : 4;
+    extern __shared__ __align__(16) float xs[];  // [NB][dim]
+    __shared__ float sm[8][M], ss[8][M];
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = f.dim;
+    const unsigned r0 = blockIdx.y * NB, n = min(f.n - r0, (unsigned)NB);  // this CTA's rows
+    for (unsigned i = threadIdx.x; i < NB * d; i += 256)
+        xs[i] = i < n * d ? f32_of(((const T*)f.x)[(size_t)r0 * d + i]) : 0.0f;
+    __syncthreads();
+    // what the lane holds after the sums: class j of the C, row r
+    constexpr int LG = M == 4 ? 2 : M == 8 ? 3 : M == 16 ? 4 : 5;
+    const unsigned id = lane >> (5 - LG), j = id / NB, r = id % NB;
+    const bool mine = (lane & ((1u << (5 - LG)) - 1)) == 0;  // of lanes with the same value
+    const long long lab = r < n ? label_at(f.labels, f.index_bytes, r0 + r) : -1;
+    const bool has = lab >= 0 && lab < f.vocab;
+    const float lse = GRADIENT && r < n ? f.lse[r] : 0.0f;
+    float m = -INFINITY, s = 0.0f;
+    for (size_t v0 = ((size_t)blockIdx.x * 8 + warp) * C; v0 < f.vocab; v0 += (size_t)gridDim.x * 8 * C) {
+        const T* w[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) w[c] = (const T*)f.w + min(v0 + c, (size_t)f.vocab - 1) * d;
+        float acc[M];
+#pragma unroll
+        for (int i = 0; i < M; i++) acc[i] = 0.0f;
+#pragma unroll U
+        for (unsigned k = lane * VEC; k < d; k += 32 * VEC) {
+            float wv[C][VEC];
+#pragma unroll
+            for (int c = 0; c < C; c++) load_vec<T, VEC>(wv[c], w[c] + k);
+#pragma unroll
+            for (int q = 0; q < NB; q++) {
+                float xv[VEC];
+                if constexpr (VEC > 1) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 4) {
+                        const float4 a = *reinterpret_cast<const float4*>(&xs[q * d + k + e]);
+                        xv[e] = a.x, xv[e + 1] = a.y, xv[e + 2] = a.z, xv[e + 3] = a.w;
+                    }
+                } else {
+                    xv[0] = xs[q * d + k];
+                }
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) acc[c * NB + q] = fmaf(wv[c][e], xv[e], acc[c * NB + q]);
+            }
+        }
+        // the lanes' sums: every step halves the values a lane holds
+        __syncwarp();
+#pragma unroll
+        for (int h = M / 2, o = 16; o > 0; o >>= 1, h >>= 1) {
+            if (h > 0) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int i = 0; i < M / 2; i++)
+                    if (i < h) {
+                        const float keep = up ? acc[i + h] : acc[i], give = up ? acc[i] : acc[i + h];
+                        acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+            } else {
+                acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+            }
+        }
+        const float z = acc[0];
+        const size_t v = v0 + j;
+        if (v < f.vocab) {
+            if constexpr (GRADIENT) {
+                float p = ex2((z - lse) * kLog2e);
+                if ((long long)v == lab) p -= 1.0f;
+                if (mine) f.p[v * NB + r] = has ? p : 0.0f;
+            } else {
+                const float nm = fmaxf(m, z), ref = nm == -INFINITY ? 0.0f : nm;  // as in chunk_lse
+                s = s * ex2((m - ref) * kLog2e) + ex2((z - ref) * kLog2e);
+                m = nm;
+                if (mine && (long long)v == lab) f.zlabel[r0 + r] = z;
+            }
+        }
+    }
+    if constexpr (!GRADIENT) {
+        if (mine) sm[warp][id] = m, ss[warp][id] = s;
+        __syncthreads();
+        if (threadIdx.x < n) {
+            m = -INFINITY, s = 0.0f;
+            for (int i = 0; i < 8 * C; i++) m = fmaxf(m, sm[i / C][i % C * NB + threadIdx.x]);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            for (int i = 0; i < 8 * C; i++) {
+                const float om = sm[i / C][i % C * NB + threadIdx.x], os = ss[i / C][i % C * NB + threadIdx.x];
+                s += om == -INFINITY ? os : os * ex2((om - ref) * kLog2e);
+            }
+            f.part_m[(size_t)blockIdx.x * f.n + r0 + threadIdx.x] = m;
+            f.part_s[(size_t)blockIdx.x * f.n + r0 + threadIdx.x] = s;
+        }
+    }
+}
+
+// blockDim = (threads over columns, groups that take classes of their own), 256 in all;
+// blockIdx.x: 256-thread block of columns, blockIdx.y: slab.
+template <typename T, int NB, int VEC>
+__global__ void __launch_bounds__(256, NB * VEC > 32 ? 1 : 2)
+k_few_out(const __grid_constant__ Few f) {
+    constexpr int U = 8;  // classes whose loads are in flight together
+    __shared__ float red[256][VEC];
+    const unsigned tx = blockDim.x, t = threadIdx.x, ty = blockDim.y, g = threadIdx.y, d = f.dim;
+    const size_t c0 = ((size_t)blockIdx.x * tx + t) * VEC;
+    const bool in = c0 < d;  // whole vectors: d is a multiple of VEC
+    float x[NB][VEC], acc[NB][VEC];
+#pragma unroll
+    for (int r = 0; r < NB; r++) {
+        const long long l = r < (int)f.n ? label_at(f.labels, f.index_bytes, r) : -1;
+        const bool has = l >= 0 && l < f.vocab;
+        const float dl = has ? f.dloss[r] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            // a row without a target counts as zeros, whatever it holds
+            x[r][e] = in && has ? dl * f32_of(((const T*)f.x)[(size_t)r * d + c0 + e]) : 0.0f;
+            acc[r][e] = 0.0f;
+        }
+    }
+    const size_t groups = (size_t)gridDim.y * ty, per = (f.vocab + groups - 1) / groups;
+    const size_t first = ((size_t)blockIdx.y * ty + g) * per, last = min(first + per, (size_t)f.vocab);
+    if (in) {
+        for (size_t v0 = first; v0 < last; v0 += U) {
+            float w[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; u++) load_vec<T, VEC>(w[u], (const T*)f.w + min(v0 + u, last - 1) * d + c0);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const size_t v = v0 + u;
+                if (v >= last) break;
+                float p[NB];
+                if constexpr (NB >= 4) {
+#pragma unroll
+                    for (int r = 0; r < NB; r += 4) {
+                        const float4 a = *reinterpret_cast<const float4*>(f.p + v * NB + r);
+                        p[r] = a.x, p[r + 1] = a.y, p[r + 2] = a.z, p[r + 3] = a.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < NB; r++) p[r] = f.p[v * NB + r];
+                }
+                alignas(16) T o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    float q = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < NB; r++) {
+                        q = fmaf(p[r], x[r][e], q);
+                        acc[r][e] = fmaf(p[r], w[u][e], acc[r][e]);
+                    }
+                    if constexpr (sizeof(T) == 2) o[e] = __float2bfloat16_rn(q);
+                    else o[e] = q;
+                }
+                T* out = (T*)f.dw + v * d + c0;
+                if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(o);
+                else if constexpr (VEC * sizeof(T) == 8) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(o);
+                else out[0] = o[0];
+            }
+        }
+    }
+    // the groups' sums, in order
+#pragma unroll
+    for (int r = 0; r < NB; r++) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VEC; e++) red[g * tx + t][e] = acc[r][e];
+        __syncthreads();
+        if (g == 0 && in && r < (int)f.n) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                float v = red[t][e];
+                for (unsigned q = 1; q < ty; q++) v += red[q * tx + t][e];
+                f.part[((size_t)blockIdx.y * f.n + r) * d + c0 + e] = v;
+            }
+        }
+    }
+}
+
+// dx = dloss times the slabs' sums, added in a fixed order (32 strided sums of an
+// element, then a tree).
+template <typename T>
+__global__ void __launch_bounds__(1024)
+k_few_fold(const __grid_constant__ Few f) {
+    __shared__ float t[32][33];
+    const size_t all = (size_t)f.n * f.dim, i = (size_t)blockIdx.x * 32 + threadIdx.x;
+    float s = 0.0f;
+    if (i < all) {
+#pragma unroll 4
+        for (unsigned k = threadIdx.y; k < f.parts; k += 32) s += f.part[k * all + i];
+    }
+    t[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    s = t[threadIdx.x][threadIdx.y];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const size_t q = (size_t)blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && q < all) {
+        const unsigned r = (unsigned)(q / f.dim);
+        const long long l = label_at(f.labels, f.index_bytes, r);
+        const float v = l >= 0 && l < f.vocab ? s * f.dloss[r] : 0.0f;
+        if constexpr (sizeof(T) == 2) ((bf16*)f.dx)[q] = __float2bfloat16_rn(v);
+        else ((float*)f.dx)[q] = v;
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -1577,9 +1828,125 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
     return finish(c);
 }
 
+// ---- host: few rows ----------------------------------------------------------------
+
+unsigned few_pad(unsigned n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+// The rules' sides in us (this path's first), loss / gradient: f32 1 x 1000 x 1000 11 / 15
+// and 19 / 45, 1 x 65536 x 2048 86 / 272 and 621 / 1143, 8 x 65536 x 2048 97 / 361 and
+// 609 / 1078, forward only 16 x 65536 x 2048 178 and 462, 24 x 2100 x 1000 17 and 19; bf16 1 x 65536 x 2048 50 / 147 and 80 / 315, 3 x 20001 x 777 17 / 69
+// and 38 / 137, 8 x 65536 x 2048 93 / 320 and 79 / 298.
+bool is_few(const XentP& p, bool grad) {
+    if ((size_t)few_pad(p.n) * p.dim > kFewX) return false;
+    if (p.dt == BF16) return p.n <= (p.dim % 8 ? kFewRows : kFewRows / 2);
+    // more rows of f32 read w again, which costs less than making its planes
+    return p.n <= kFewRows || (!grad && p.n <= 3 * kFewRows && (size_t)p.vocab * p.dim >= 1u << 21);
+}
+
+// Workspace, in bytes: forward part_m, part_s [CTAs][n] and zlabel; backward P and
+// the slabs' sums.
+struct FewPlan {
+    unsigned ctas;      // of k_few_z
+    unsigned tx, gx, gy;  // of k_few_out
+    size_t pm, ps, zl, p, part, total;
+};
+// vec: columns of a thread of k_few_out
+FewPlan few_plan(const XentP& p, bool grad, unsigned vec) {
+    FewPlan q{};
+    q.ctas = (unsigned)std::min<size_t>(((size_t)p.vocab + 8 * kFewC - 1) / (8 * kFewC), kFewCtas);
+    const unsigned pieces = (p.dim + vec - 1) / vec;
+    for (q.tx = 32; q.tx < pieces && q.tx < 256; q.tx *= 2) {}
+    q.gx = (pieces + q.tx - 1) / q.tx;
+    const size_t classes = 8 * (256 / q.tx);  // of a slab, at least
+    q.gy = (unsigned)std::max<size_t>(1, std::min<size_t>((p.vocab + classes - 1) / classes, kFewCtas / q.gx));
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at += up(bytes, 256);
+        return o;
+    };
+    if (!grad) {
+        q.pm = take((size_t)4 * q.ctas * p.n);
+        q.ps = take((size_t)4 * q.ctas * p.n);
+        q.zl = take((size_t)4 * p.n);
+    } else {
+        q.p = take((size_t)4 * p.vocab * few_pad(p.n));
+        q.part = take((size_t)4 * q.gy * p.n * p.dim);
+    }
+    q.total = std::max<size_t>(at, 256);
+    return q;
+}
+// Columns of a thread of k_few_out: 16 bytes (with 8 rows of bf16 8 bytes, for the
+// registers) where w's and dw's rows are aligned to it, else 1.
+unsigned few_vec(const XentP& p, bool aligned) {
+    const unsigned most = p.dt == F32 || few_pad(p.n) == 8 ? 4 : 8;
+    return aligned && p.dim % most == 0 ? most : 1;
+}
+
+template <typename T, int NB, bool GRADIENT>
+int run_few_z(Ctx& c, const Few& f, unsigned ctas) {
+    const dim3 grid(ctas, (f.n + NB - 1) / NB);
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = f.dim % V == 0 && ((uintptr_t)f.w & 15) == 0;
+    auto k = vec ? k_few_z<T, NB, V, GRADIENT> : k_few_z<T, NB, 1, GRADIENT>;
+    const int bytes = (int)(NB * f.dim * 4);
+    NXV_CK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k<<<grid, 256, bytes, c.stream>>>(f);
+    count_launch();
+    return OK;
+}
+
+template <typename T, int NB>
+int few_t(Ctx& c, const XentP& p, Few f, bool grad, void* loss, void* lse, void* ws) {
+    char* base = (char*)ws;
+    int rc;
+    if (!grad) {
+        const FewPlan q = few_plan(p, false, 1);
+        f.part_m = (float*)(base + q.pm);
+        f.part_s = (float*)(base + q.ps);
+        f.zlabel = (float*)(base + q.zl);
+        if ((rc = run_few_z<T, NB, false>(c, f, q.ctas))) return rc;
+        join(c, p, loss, lse, f.part_m, f.part_s, f.zlabel, q.ctas);
+        return OK;
+    }
+    const unsigned vec = few_vec(p, (((uintptr_t)f.w | (uintptr_t)f.dw) & 15) == 0);
+    const FewPlan q = few_plan(p, true, vec);
+    f.p = (float*)(base + q.p);
+    f.part = (float*)(base + q.part);
+    f.parts = q.gy;
+    if ((rc = run_few_z<T, NB, true>(c, f, q.ctas))) return rc;
+    constexpr int V = sizeof(T) == 4 || NB == 8 ? 4 : 8;
+    const dim3 grid(q.gx, q.gy), block(q.tx, 256 / q.tx);
+    if (vec > 1) k_few_out<T, NB, V><<<grid, block, 0, c.stream>>>(f);
+    else k_few_out<T, NB, 1><<<grid, block, 0, c.stream>>>(f);
+    k_few_fold<T><<<(unsigned)(((size_t)p.n * p.dim + 31) / 32), dim3(32, 32), 0, c.stream>>>(f);
+    count_launch(2);
+    return OK;
+}
+
+// loss and lse are outputs of the forward call, lse an input of the gradient.
+int few(Ctx& c, const XentP& p, bool grad, void* loss, void* lse, void* dx, void* dw, const void* dloss, void* ws) {
+    Few f{};
+    f.x = p.x, f.w = p.w, f.labels = p.labels, f.index_bytes = p.index_bytes;
+    f.n = p.n, f.vocab = p.vocab, f.dim = p.dim;
+    f.lse = (const float*)lse, f.dloss = (const float*)dloss;
+    f.dx = dx, f.dw = dw;
+    const unsigned nb = few_pad(p.n);
+    int rc;
+#define FEW(T) (nb == 1   ? few_t<T, 1>(c, p, f, grad, loss, lse, ws) \
+                : nb == 2 ? few_t<T, 2>(c, p, f, grad, loss, lse, ws) \
+                : nb == 4 ? few_t<T, 4>(c, p, f, grad, loss, lse, ws) \
+                          : few_t<T, 8>(c, p, f, grad, loss, lse, ws))
+    rc = p.dt == F32 ? FEW(float) : FEW(bf16);
+#undef FEW
+    if (rc) return rc;
+    pdl_record_all(c);
+    return finish(c);
+}
+
 }  // namespace
 
 size_t xent_workspace(const XentP& p, bool grad) {
+    if (is_few(p, grad)) return std::max(few_plan(p, grad, 1).total, few_plan(p, grad, few_vec(p, true)).total);
     return is_small(p) ? small_plan(p, grad).total : make_plan(p, grad).total;
 }
 
@@ -1590,6 +1957,7 @@ int xent_error() {
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     if (p.n == 0) return OK;
+    if (is_few(p, false)) return few(c, p, false, loss, lse, nullptr, nullptr, nullptr, ws);
     if (is_small(p)) return small_xent(c, p, loss, lse, ws);
     const Plan q = make_plan(p, false);
     char* base = (char*)ws;
@@ -1641,6 +2009,7 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
         NXV_CK(cudaMemsetAsync(dw, 0, (size_t)p.vocab * p.dim * dtype_bytes(p.dt), c.stream));
         return finish(c);
     }
+    if (is_few(p, true)) return few(c, p, true, nullptr, const_cast<void*>(lse), dx, dw, dloss, ws);
     if (is_small(p)) return small_xent_grad(c, p, dx, dw, dloss, lse, ws);
     const Plan q = make_plan(p, true);
     char* base = (char*)ws;

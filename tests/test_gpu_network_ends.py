@@ -392,7 +392,11 @@ XENT_SHAPES = [(1, 1, 1), (1, 10, 3), (3, 257, 13), (2, 256, 64), (130, 1000, 64
                (128, 256, 128), (257, 300, 1001), (5, 5003, 16), (300, 31, 200), (4099, 21, 17), (1, 70001, 5),
                (515, 515, 515), (513, 1001, 513), (129, 2049, 1025), (100, 40000, 64), (20000, 129, 64),
                (3001, 100, 1000), (3, 20000, 3000), (2, 50001, 700), (8193, 12, 800), (40000, 300, 8), (9000, 70, 130),
-               (129, 600, 72), (200, 1100, 333)]
+               (129, 600, 72), (200, 1100, 333),
+               # up to 8 rows, with x in shared memory or (the last two) not
+               (1, 31, 2048), (8, 1000, 2048), (7, 30000, 1024), (1, 100003, 640), (6, 9999, 41), (4, 5000, 4096), (8, 33, 8),
+               (3, 1, 100), (2, 65536, 1000), (8, 700, 2056), (1, 500, 16392),
+               (9, 65536, 64), (17, 30001, 100), (24, 2048, 2048)]
 
 
 def xent_inputs(torch, name, n, v, d, seed=0, scale=2.0):
