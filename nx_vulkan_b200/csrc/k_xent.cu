@@ -529,11 +529,15 @@ struct Row {
     }
 };
 
-// Persistent: CTA (pair) b computes tiles b, b + CTAs (pairs), ... of the
-// jobs one after the other (row tile fastest, so that the CTAs at work share
-// the column operand's tiles in L2).  Jobs of one launch do not depend on each
-// other; the host puts the one with the longest K first, so that the short
-// tiles fill the last wave.
+__device__ __forceinline__ uint32_t tile_of(uint32_t round, uint32_t first, uint32_t step) {
+    return round * step + (round & 1 ? step - 1 - first : first);
+}
+
+// Persistent: the CTAs (pairs) take the tiles of the jobs in rounds (row tile fastest,
+// so that the CTAs at work share the column operand's tiles in L2).  Jobs of one
+// launch do not depend on each other; the host puts the one with the longest K first,
+// and every other round goes backwards, so that the last round's tiles go to those
+// whose first tile was short (2048 x 10007 x 1000 f32 gradient 612 us instead of 666).
 //   warps 0 and 3, lane 0: TMA producers, ST stages of 128 rows of A and of B;
 //   warp 1 lane 0 (of the leader): MMA issuer into one of two accumulators;
 //   warps 4-11: epilogue of the other (warp w: lanes 32 (w % 4), column half (w - 4) / 4).
@@ -549,7 +553,7 @@ struct Row {
 // multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms, 1.69 PFLOP/s (the
 // library's bare product of these sizes 1.47 ms in the same session); gradient 5.1
 // to 5.5 ms, 1.6 to 1.7 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
-// 2.2 and 8.7 ms, 1.5 PFLOP/s over the six partial products.
+// 2.1 and 8.3 ms, 1.6 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
 // flight are waited for (bounded), tensor memory is freed and the host's flag set.
 template <int CG, bool SIX>
@@ -619,8 +623,9 @@ k_xgemm(const __grid_constant__ Work W) {
         const uint32_t b_out = CG == 2 ? in_leader(b_full) : b_full;
         uint32_t s = 0, par = 1, issued = 0;  // the first pass over the ring finds it empty
         bool ok = true;
-        for (uint32_t t = first; t < W.tiles && ok; t += step) {
-            uint32_t j = 0, lt = t;
+        for (uint32_t round = 0; ok; round++) {
+            uint32_t j = 0, lt = tile_of(round, first, step);
+            if (lt >= W.tiles) break;
             while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
             const uint32_t tm = W.job[j].tm, slice = lt / W.job[j].plane;
             lt -= slice * W.job[j].plane;
@@ -663,8 +668,9 @@ k_xgemm(const __grid_constant__ Work W) {
         const bool one = elect_one();
         uint32_t s = 0, par = 0, ph = 0;
         bool ok = true;
-        for (uint32_t t = first; t < W.tiles && ok; t += step) {
-            uint32_t j = 0, lt = t;
+        for (uint32_t round = 0; ok; round++) {
+            uint32_t j = 0, lt = tile_of(round, first, step);
+            if (lt >= W.tiles) break;
             while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
             const bool a_mn = W.job[j].a_mn, b_mn = W.job[j].b_mn;
             const uint32_t id = idesc<CG>(a_mn, b_mn);
@@ -707,8 +713,9 @@ k_xgemm(const __grid_constant__ Work W) {
         float* tr = reinterpret_cast<float*>(smem + ST * ST_BYTES + 256) + (warp - 4) * (32 * 33);
         uint32_t ph = 0;
         bool ok = true;
-        for (uint32_t t = first; t < W.tiles && ok; t += step) {
-            uint32_t j = 0, lt = t;
+        for (uint32_t round = 0; ok; round++) {
+            uint32_t j = 0, lt = tile_of(round, first, step);
+            if (lt >= W.tiles) break;
             while (lt >= W.job[j].tiles) lt -= W.job[j++].tiles;
             const Job& g = W.job[j];
             const int KB = k_blocks(g, lt);
