@@ -296,7 +296,7 @@ unsigned long nxv_linear_cross_entropy_workspace(unsigned int n, unsigned int vo
  * a label outside [0, vocab) marks a row without a target (loss 0).  dtype 0
  * f32 or 2 bf16 (tcgen05; f32 as six bf16 partial products, f32 accuracy).
  * As logsumexp.spv: a row whose logits hold a NaN or +inf, or only -inf, has
- * lse NaN; in f32 an infinity in x or w makes every logit it meets NaN.
+ * lse NaN; in f32 an infinity in x or w may make every logit it meets NaN.
  * vocab > 0, 0 < dim <= 2^24.  spv: linear_cross_entropy.spv. */
 int nxv_linear_cross_entropy(void* loss, void* lse, void* workspace,
                              void* x, void* w, void* labels,

@@ -451,7 +451,8 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
     }
 }
 
-// Rows that 512 threads cannot hold: three passes over the row.
+// Rows that 512 threads, or gamma and beta that the shared memory, cannot hold: three
+// passes over the row.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_norm_fwd_long(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const T* x,
@@ -902,7 +903,7 @@ int fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, co
          unsigned rows, unsigned cols, acc_t<T> eps) {
     // a row that starts inside a piece may take one more
     const size_t nv = ((size_t)cols + (AL ? 1 : 2) * (kV<T> - 1)) / kV<T>;
-    if (nv > 16 * 512) {
+    if (nv > (AL ? 16 * 512 : 7168)) {  // 7168: gamma and beta in shared memory
         k_norm_fwd_long<T><<<std::min(rows, (unsigned)c.dev->sm_count * 2), 1024, 0, c.stream>>>(
             y, mean, rstd, x, g, b, rows, cols, eps);
         return OK;

@@ -77,7 +77,8 @@ def place(torch, t, shift):
 NORM_SHAPES = [(1, 1), (1, 2), (4, 7), (5, 32), (9, 33), (3, 256), (7, 1000), (2, 1023), (300, 129),
                (3, 4096), (2, 5001), (7, 5003), (2, 8192), (3, 12289), (1, 16384), (2, 20000), (1, 40001), (3, 70001),
                (600, 64), (1200, 33), (700, 1025), (500, 20003),
-               (2500, 3), (2400, 257), (2400, 1000), (5000, 104), (2400, 5001)]
+               (2500, 3), (2400, 257), (2400, 1000), (5000, 104), (2400, 5001),
+               (3, 14329), (3, 14343), (2, 28667), (2, 28681), (2, 30001), (2, 57337), (2, 57361)]
 
 
 def norm_run(nxv, torch, x, g, b, eps, name, y=None):
