@@ -789,37 +789,99 @@ k_xgemm(const __grid_constant__ Work W) {
 
 // ---- small kernels -----------------------------------------------------------------
 
-// Rows of src [rows][dim] as bf16 planes [planes][rows][ld], ld = dim rounded
-// up to 64: a warp per row, a lane 8 consecutive values at a time (the columns
+// The largest |dloss| of the rows with a target, 1 where there is none that is
+// positive and finite: the unit that dloss x is taken in, so that the equal
+// dloss of a mean leaves x as it is, with no rounding.  The whole CTA.
+template <int THREADS>
+__device__ __forceinline__ float largest_dloss(const float* __restrict__ dloss, const void* labels,
+                                               int index_bytes, long long vocab, long long n) {
+    __shared__ float s[THREADS / 32];
+    float m = 0.0f;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < n; i += THREADS) {
+        const long long l = label_at(labels, index_bytes, i);
+        const float v = fabsf(dloss[i]);
+        if (l >= 0 && l < vocab) m = fmaxf(m, v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = s[threadIdx.x & (THREADS / 32 - 1)];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m > 0.0f && m < INFINITY ? m : 1.0f;
+}
+__global__ void __launch_bounds__(1024)
+k_xent_unit(float* __restrict__ unit, const float* __restrict__ dloss, const void* labels,
+            int index_bytes, long long vocab, long long n) {
+    const float u = largest_dloss<1024>(dloss, labels, index_bytes, vocab, n);
+    if (threadIdx.x == 0) *unit = u;
+}
+
+// Up to this many rows k_pack finds the unit itself, every CTA for itself, which costs
+// less than a launch.
+constexpr long long kOwnUnit = 2048;
+
+// Tensors [rows][dim] as bf16 planes [planes][rows][ld], ld = dim rounded up to 64, one
+// after the other: a warp per row, a lane 8 consecutive values at a time (the columns
 // from dim on are written as zeros).  1 plane: rounded to bf16; 3: split3.
-// With scale, row i becomes (scale_i / *unit) x_i in f32 first, and a row without
-// a target becomes zeros, so that what its x holds (NaN, infinities) never meets
-// the zeros of its G row.
+// A scaled tensor's (the first job's) row i becomes (dloss_i / *unit) x_i in f32 first,
+// and a row without a target becomes zeros, so that what its x holds (NaN, infinities)
+// never meets the zeros of its G row.
+struct PackJob {
+    bf16* dst;
+    const void* src;
+    long long rows;
+    int vec;  // rows on 16-byte boundaries
+    int scaled;
+};
+struct PackWork {
+    PackJob job[3];
+    int jobs, dim, ld;
+    const float* dloss;
+    float* unit;
+    const void* labels;
+    int index_bytes;
+    long long vocab, n;
+};
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-k_pack(bf16* __restrict__ dst, const T* __restrict__ src, long long rows, int dim, int ld,
-       int vec, const float* __restrict__ scale, const float* __restrict__ unit, const void* labels,
-       int index_bytes, long long vocab) {
-    const long long plane = rows * ld;
-    const int lane = threadIdx.x & 31;
-    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
-         r += (long long)gridDim.x * 8) {
+k_pack(const __grid_constant__ PackWork w) {
+    long long all = 0;
+    for (int i = 0; i < w.jobs; i++) all += w.job[i].rows;
+    const int lane = threadIdx.x & 31, dim = w.dim, ld = w.ld;
+    float unit = 1.0f;
+    if (w.job[0].scaled && (long long)blockIdx.x * 8 < w.n) {  // this CTA has scaled rows
+        if (w.n <= kOwnUnit) {
+            unit = largest_dloss<256>(w.dloss, w.labels, w.index_bytes, w.vocab, w.n);
+            if (blockIdx.x == 0 && threadIdx.x == 0) *w.unit = unit;
+        } else {
+            unit = *w.unit;
+        }
+    }
+    for (long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); at < all; at += (long long)gridDim.x * 8) {
+        long long r = at;
+        int ji = 0;
+        while (r >= w.job[ji].rows) r -= w.job[ji++].rows;
+        const PackJob& g = w.job[ji];
+        const long long plane = g.rows * ld;
         float f = 1.0f;
         bool has = true;
-        if (scale) {
-            const long long l = label_at(labels, index_bytes, r);
-            has = l >= 0 && l < vocab;
-            f = __fdiv_rn(scale[r], *unit);
+        if (g.scaled) {
+            const long long l = label_at(w.labels, w.index_bytes, r);
+            has = l >= 0 && l < w.vocab;
+            f = __fdiv_rn(w.dloss[r], unit);
         }
-        const T* sr = src + r * dim;
-        bf16* dr = dst + r * ld;
+        const T* sr = (const T*)g.src + r * dim;
+        bf16* dr = g.dst + r * ld;
         constexpr int U = 4;  // groups of 8 whose loads are in flight together
         for (int c0 = lane * 8; c0 < ld; c0 += 256 * U) {
             alignas(16) T in[U][8];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int c = c0 + 256 * u;
-                if (vec && c + 8 <= dim) {
+                if (g.vec && c + 8 <= dim) {
 #pragma unroll
                     for (int q = 0; q < (int)(8 * sizeof(T) / 16); q++)
                         reinterpret_cast<uint4*>(in[u])[q] = reinterpret_cast<const uint4*>(sr + c)[q];
@@ -836,7 +898,7 @@ k_pack(bf16* __restrict__ dst, const T* __restrict__ src, long long rows, int di
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     float v = (float)in[u][e];
-                    if (scale) v = has ? v * f : 0.0f;
+                    if (g.scaled) v = has ? v * f : 0.0f;
                     if constexpr (PLANES == 1) o[0][e] = __float2bfloat16_rn(v);
                     else split3(v, o[0][e], o[1][e], o[2][e]);
                 }
@@ -845,30 +907,6 @@ k_pack(bf16* __restrict__ dst, const T* __restrict__ src, long long rows, int di
                     *reinterpret_cast<uint4*>(dr + k * plane + c) = *reinterpret_cast<uint4*>(o[k]);
             }
         }
-    }
-}
-
-// The largest |dloss| of the rows with a target, 1 where there is none that is
-// positive and finite: the unit that dloss x is taken in, so that the equal
-// dloss of a mean leaves x as it is, with no rounding.
-__global__ void __launch_bounds__(1024)
-k_xent_unit(float* __restrict__ unit, const float* __restrict__ dloss, const void* labels,
-            int index_bytes, long long vocab, long long n) {
-    __shared__ float s[32];
-    float m = 0.0f;
-    for (long long i = threadIdx.x; i < n; i += 1024) {
-        const long long l = label_at(labels, index_bytes, i);
-        if (l >= 0 && l < vocab) m = fmaxf(m, fabsf(dloss[i]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        m = s[threadIdx.x];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (threadIdx.x == 0) *unit = m > 0.0f && m < INFINITY ? m : 1.0f;
     }
 }
 
@@ -1578,7 +1616,12 @@ constexpr size_t kTile = 2 * BT;
 Plan make_plan(const XentP& p, bool grad) {
     Plan q{};
     q.planes = p.dt == F32 ? 3 : 1;
-    q.cg = p.n > BT && p.vocab > BT ? 2 : 1;
+    // Pairs' tiles read half as much per product, but where the single tiles of the logits
+    // fit the SMs at once these finish sooner (512 x 4000 x 768 bf16 14.4 / 38 us instead
+    // of 16.5 / 43, 400 x 1000 x 1000 f32 41 / 81 and 49 / 99; not 256 x 10000 x 512 f32,
+    // two rounds of single tiles, 46 / 115 and 40 / 111).
+    const size_t single = (((size_t)p.n + BT - 1) / BT) * (((size_t)p.vocab + BT - 1) / BT);
+    q.cg = p.n > BT && p.vocab > BT && single > 148 ? 2 : 1;
     q.seg = (size_t)BT * q.cg / 2;
     // whole 128-byte lines: a box row that straddles two costs two requests
     // (2048 x 8192 x 1000 f32: 750 instead of 510 cycles per stage)
@@ -1624,20 +1667,26 @@ Plan make_plan(const XentP& p, bool grad) {
     return q;
 }
 
-// scale: the factors of the rows (dloss), in units of *unit; or null.
-void pack(Ctx& c, const XentP& p, bf16* dst, const void* src, size_t rows, int ld,
-          const void* scale, const float* unit) {
+// Adds a tensor to what a launch of k_pack makes; a scaled one first.
+void pack_add(PackWork& w, const XentP& p, bf16* dst, const void* src, size_t rows, bool scaled = false) {
+    w.job[w.jobs++] = {dst, src, (long long)rows,
+                       ((uintptr_t)src & 15) == 0 && p.dim * dtype_bytes(p.dt) % 16 == 0, scaled};
+}
+void run_pack(Ctx& c, const XentP& p, PackWork& w, int ld) {
+    if (w.jobs == 0) return;
+    w.dim = (int)p.dim;
+    w.ld = ld;
+    w.labels = p.labels;
+    w.index_bytes = p.index_bytes;
+    w.vocab = p.vocab;
+    w.n = p.n;
+    size_t rows = 0;
+    for (int i = 0; i < w.jobs; i++) rows += w.job[i].rows;
     const unsigned grid = grid_for(c, rows, 8, 16);
-    const bool vec = ((uintptr_t)src & 15) == 0 && p.dim * dtype_bytes(p.dt) % 16 == 0;
-    if (p.dt == F32)
-        k_pack<float, 3><<<grid, 256, 0, c.stream>>>(dst, (const float*)src, rows, p.dim, ld, vec,
-                                                     (const float*)scale, unit, p.labels,
-                                                     p.index_bytes, p.vocab);
-    else
-        k_pack<bf16, 1><<<grid, 256, 0, c.stream>>>(dst, (const bf16*)src, rows, p.dim, ld, vec,
-                                                    (const float*)scale, unit, p.labels,
-                                                    p.index_bytes, p.vocab);
+    if (p.dt == F32) k_pack<float, 3><<<grid, 256, 0, c.stream>>>(w);
+    else k_pack<bf16, 1><<<grid, 256, 0, c.stream>>>(w);
     count_launch();
+    w = PackWork{};
 }
 
 // A tensor can feed TMA where it lies when its rows start on 16-byte boundaries.
@@ -1970,9 +2019,10 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
     char* base = (char*)ws;
     const bool wip = in_place(p, p.w), xip = in_place(p, p.x);
     const bf16* xp = (const bf16*)p.x;
+    PackWork packs{};
     if (!xip) {
         xp = (bf16*)(base + q.xp);
-        pack(c, p, (bf16*)xp, p.x, p.n, (int)q.dp, nullptr, nullptr);
+        pack_add(packs, p, (bf16*)xp, p.x, p.n);
     }
     CUtensorMap ma, mb;
     int rc;
@@ -1992,9 +2042,9 @@ int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {
         const bf16* wp = (const bf16*)p.w;
         if (!wip) {
             wp = (bf16*)(base + q.wp[0]);
-            pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * dtype_bytes(p.dt), nv, (int)q.dp,
-                 nullptr, nullptr);
+            pack_add(packs, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * dtype_bytes(p.dt), nv);
         }
+        run_pack(c, p, packs, (int)q.dp);
         if ((rc = make_map(&mb, wp, p.dim, nv, ldw, q.planes, nv * ldw, BT))) return rc;
         g.N = (int)nv;
         g.col0 = (long long)v0;
@@ -2025,16 +2075,21 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
     const bool xip = in_place(p, p.x);
     const size_t ldx = xip ? p.dim : q.dp, ldw = wip ? p.dim : q.dp;
     const bf16* xp = (const bf16*)p.x;
-    if (!xip) {
-        xp = (bf16*)(base + q.xp);
-        pack(c, p, (bf16*)xp, p.x, p.n, (int)q.dp, nullptr, nullptr);
-    }
     bf16* sp = (bf16*)(base + q.sp);  // dloss x / unit
     float* unit = (float*)(base + q.unit);
-    k_xent_unit<<<1, 1024, 0, c.stream>>>(unit, (const float*)dloss, p.labels, p.index_bytes,
-                                          p.vocab, p.n);
-    count_launch();
-    pack(c, p, sp, p.x, p.n, (int)q.dp, dloss, unit);
+    if (p.n > kOwnUnit) {
+        k_xent_unit<<<1, 1024, 0, c.stream>>>(unit, (const float*)dloss, p.labels, p.index_bytes,
+                                              p.vocab, p.n);
+        count_launch();
+    }
+    PackWork packs{};
+    packs.dloss = (const float*)dloss;
+    packs.unit = unit;
+    pack_add(packs, p, sp, p.x, p.n, true);
+    if (!xip) {
+        xp = (bf16*)(base + q.xp);
+        pack_add(packs, p, (bf16*)xp, p.x, p.n);
+    }
     const size_t gplane = (size_t)p.n * q.ldg;
     CUtensorMap mxk, mxn, mwk, mwn, mgk, mgm;
     int rc;
@@ -2100,8 +2155,9 @@ int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlo
             const bf16* wp = (const bf16*)p.w + (wip ? v0 * p.dim : 0);
             if (!wip) {
                 wp = (bf16*)(base + q.wp[i & 1]);
-                pack(c, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * es, nv, (int)q.dp, nullptr, nullptr);
+                pack_add(packs, p, (bf16*)wp, (const char*)p.w + v0 * p.dim * es, nv);
             }
+            run_pack(c, p, packs, (int)q.dp);
             if ((rc = make_map(&mwk, wp, p.dim, nv, ldw, q.planes, nv * ldw, BT))) return rc;
             z.N = (int)nv;
             z.col0 = (long long)v0;
