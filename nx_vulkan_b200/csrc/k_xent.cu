@@ -1002,11 +1002,12 @@ k_xent_join_row(float* __restrict__ loss, float* __restrict__ lse, const float* 
 // where a long K is cut into slices, their sum).
 
 // The limits on n vocab dim, from both paths' times in us (loss / gradient, this
-// path's first): f32 16 x 200 x 100 12 / 15 and 23 / 41, 64 x 1001 x 1000 19 / 59 and
-// 40 / 76, 256 x 512 x 512 21 / 54 and 35 / 74, 512^3 35 / 101 and 35 / 74; bf16
-// 200 x 200 x 100 11 / 19 and 23 / 45 (not 16-byte rows), 64 x 300 x 400 13 / 19 and
-// 13 / 25, 128 x 512 x 256 13 / 27 and 11 / 23, 64 x 1001 x 1000 21 / 60 and 16 / 31.
-constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;
+// path's first): f32 16 x 200 x 100 12 / 13 and 18 / 27, 64 x 1001 x 1000 19 / 58 and
+// 37 / 66, 100 x 100 x 1000 19 / 28 and 36 / 45, 256 x 512 x 512 21 / 53 and 25 / 41,
+// 512 x 512 x 256 21 / 56 and 19 / 37; bf16 200 x 200 x 100 10 / 19 and 14 / 25 (not
+// 16-byte rows), 64 x 300 x 400 12 / 19 and 12 / 23, 128 x 512 x 128 10 / 21 and 10 / 19,
+// 64 x 1001 x 1000 21 / 60 and 14 / 29.
+constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;  // f32 of more than 128 rows: half
 constexpr int KSTEP = 128;  // slices of K are multiples of this, and of a tile's chunk KC
 
 struct SmallJob {
@@ -1254,7 +1255,7 @@ k_sum(const __grid_constant__ SumWork w) {
 // 16 bytes each of their rows, and every value of x that is read serves kFewC
 // classes; then the lanes part the sums among them, one (class, row) each, which keeps
 // its own running maximum and sum (forward) or stores P (backward).
-// k_few_out: a thread holds some columns of x and of dx's sums in registers and goes
+// k_few_out: a thread holds (of up to 16 rows) some columns of x and of dx's sums in registers and goes
 // down a slab of classes: dx += P w, dw = P^T (dloss x), w read and dw written once.
 // All in f32, rounded once at the end.
 // Measured, 1 x 65536 x 2048: f32 86 us forward (w alone 82 at the measured copy rate),
@@ -1270,7 +1271,8 @@ struct Few {
     unsigned n, vocab, dim;
     float *part_m, *part_s, *zlabel;  // forward: [CTA][n], [CTA][n], [n]
     const float *lse, *dloss;
-    float* p;     // backward: [vocab][NB]
+    float* p;     // backward: [vocab][ldp], ldp = the rows padded to k_few_out's NB
+    unsigned ldp;
     float* part;  // [slab][n][dim]
     void *dx, *dw;
     unsigned parts;
@@ -1289,8 +1291,7 @@ __device__ __forceinline__ void load_vec(float (&v)[VEC], const T* p) {
     for (int i = 0; i < VEC; i++) v[i] = f32_of(e[i]);
 }
 
-// VEC: 16 bytes of w where its rows are aligned, else 1.  blockIdx.y: NB of the rows
-// (the gradient has one such block only).
+// VEC: 16 bytes of w where its rows are aligned, else 1.  blockIdx.y: NB of the rows.
 template <typename T, int NB, int VEC, bool GRADIENT>
 __global__ void __launch_bounds__(256, 2)
 k_few_z(const __grid_constant__ Few f) {
@@ -1308,7 +1309,7 @@ k_few_z(const __grid_constant__ Few f) {
     const bool mine = (lane & ((1u << (5 - LG)) - 1)) == 0;  // of lanes with the same value
     const long long lab = r < n ? label_at(f.labels, f.index_bytes, r0 + r) : -1;
     const bool has = lab >= 0 && lab < f.vocab;
-    const float lse = GRADIENT && r < n ? f.lse[r] : 0.0f;
+    const float lse = GRADIENT && r < n ? f.lse[r0 + r] : 0.0f;
     float m = -INFINITY, s = 0.0f;
     for (size_t v0 = ((size_t)blockIdx.x * 8 + warp) * C; v0 < f.vocab; v0 += (size_t)gridDim.x * 8 * C) {
         const T* w[C];
@@ -1362,7 +1363,7 @@ k_few_z(const __grid_constant__ Few f) {
             if constexpr (GRADIENT) {
                 float p = ex2((z - lse) * kLog2e);
                 if ((long long)v == lab) p -= 1.0f;
-                if (mine) f.p[v * NB + r] = has ? p : 0.0f;
+                if (mine) f.p[v * f.ldp + r0 + r] = has ? p : 0.0f;
             } else {
                 const float nm = fmaxf(m, z), ref = nm == -INFINITY ? 0.0f : nm;  // as in chunk_lse
                 s = s * ex2((m - ref) * kLog2e) + ex2((z - ref) * kLog2e);
@@ -1709,7 +1710,7 @@ void join(Ctx& c, const XentP& p, void* loss, void* lse, const float* pm, const 
 // ---- host: small problems --------------------------------------------------------
 
 bool is_small(const XentP& p) {
-    const unsigned long long most = p.dt == BF16 ? kSmallBf16 : kSmallF32;
+    const unsigned long long most = p.dt == BF16 ? kSmallBf16 : p.n > BT ? kSmallF32 / 2 : kSmallF32;
     const unsigned long long n = up(p.n, 16);  // whole row tiles
     // no overflow: the entry points bound the tiles, and so n vocab, below 2^45
     return n * p.vocab <= most && n * p.vocab * p.dim <= most;
@@ -1886,16 +1887,18 @@ int small_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dlos
 
 // ---- host: few rows ----------------------------------------------------------------
 
-unsigned few_pad(unsigned n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8; }
+unsigned few_pad(unsigned n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16; }
 // The rules' sides in us (this path's first), loss / gradient: f32 1 x 1000 x 1000 11 / 15
 // and 19 / 45, 1 x 65536 x 2048 86 / 272 and 621 / 1143, 8 x 65536 x 2048 97 / 361 and
-// 609 / 1078, forward only 16 x 65536 x 2048 178 and 462, 24 x 2100 x 1000 17 and 19; bf16 1 x 65536 x 2048 50 / 147 and 80 / 315, 3 x 20001 x 777 17 / 69
+// 609 / 1078, 16 x 65536 x 2048 178 / 786 and 462 / 914,
+// 16 x 4000 x 2000 gradient 65 and 132, forward only 24 x 2100 x 1000 17 and 19; bf16 1 x 65536 x 2048 50 / 147 and 80 / 315, 3 x 20001 x 777 17 / 69
 // and 38 / 137, 8 x 65536 x 2048 93 / 320 and 79 / 298.
 bool is_few(const XentP& p, bool grad) {
-    if ((size_t)few_pad(p.n) * p.dim > kFewX) return false;
+    if (std::min<size_t>(few_pad(p.n), 8) * p.dim > kFewX) return false;
     if (p.dt == BF16) return p.n <= (p.dim % 8 ? kFewRows : kFewRows / 2);
     // more rows of f32 read w again, which costs less than making its planes
-    return p.n <= kFewRows || (!grad && p.n <= 3 * kFewRows && (size_t)p.vocab * p.dim >= 1u << 21);
+    return p.n <= kFewRows ||
+           (p.n <= (grad ? 2 : 3) * kFewRows && (size_t)p.vocab * p.dim >= (grad ? 1u << 20 : 1u << 21));
 }
 
 // Workspace, in bytes: forward part_m, part_s [CTAs][n] and zlabel; backward P and
@@ -1931,10 +1934,10 @@ FewPlan few_plan(const XentP& p, bool grad, unsigned vec) {
     q.total = std::max<size_t>(at, 256);
     return q;
 }
-// Columns of a thread of k_few_out: 16 bytes (with 8 rows of bf16 8 bytes, for the
-// registers) where w's and dw's rows are aligned to it, else 1.
+// Columns of a thread of k_few_out: 16 bytes (with 8 rows of bf16 and 16 of f32 8 bytes,
+// for the registers) where w's and dw's rows are aligned to it, else 1.
 unsigned few_vec(const XentP& p, bool aligned) {
-    const unsigned most = p.dt == F32 || few_pad(p.n) == 8 ? 4 : 8;
+    const unsigned nb = few_pad(p.n), most = p.dt == F32 ? (nb == 16 ? 2 : 4) : (nb == 8 ? 4 : 8);
     return aligned && p.dim % most == 0 ? most : 1;
 }
 
@@ -1951,8 +1954,10 @@ int run_few_z(Ctx& c, const Few& f, unsigned ctas) {
     return OK;
 }
 
+// NB: the rows, padded; k_few_z takes 8 of them at most.
 template <typename T, int NB>
 int few_t(Ctx& c, const XentP& p, Few f, bool grad, void* loss, void* lse, void* ws) {
+    constexpr int NZ = NB > 8 ? 8 : NB;
     char* base = (char*)ws;
     int rc;
     if (!grad) {
@@ -1960,7 +1965,7 @@ int few_t(Ctx& c, const XentP& p, Few f, bool grad, void* loss, void* lse, void*
         f.part_m = (float*)(base + q.pm);
         f.part_s = (float*)(base + q.ps);
         f.zlabel = (float*)(base + q.zl);
-        if ((rc = run_few_z<T, NB, false>(c, f, q.ctas))) return rc;
+        if ((rc = run_few_z<T, NZ, false>(c, f, q.ctas))) return rc;
         join(c, p, loss, lse, f.part_m, f.part_s, f.zlabel, q.ctas);
         return OK;
     }
@@ -1969,8 +1974,9 @@ int few_t(Ctx& c, const XentP& p, Few f, bool grad, void* loss, void* lse, void*
     f.p = (float*)(base + q.p);
     f.part = (float*)(base + q.part);
     f.parts = q.gy;
-    if ((rc = run_few_z<T, NB, true>(c, f, q.ctas))) return rc;
-    constexpr int V = sizeof(T) == 4 || NB == 8 ? 4 : 8;
+    f.ldp = NB;
+    if ((rc = run_few_z<T, NZ, true>(c, f, q.ctas))) return rc;
+    constexpr int V = sizeof(T) == 4 ? (NB == 16 ? 2 : 4) : (NB == 8 ? 4 : 8);
     const dim3 grid(q.gx, q.gy), block(q.tx, 256 / q.tx);
     if (vec > 1) k_few_out<T, NB, V><<<grid, block, 0, c.stream>>>(f);
     else k_few_out<T, NB, 1><<<grid, block, 0, c.stream>>>(f);
@@ -1992,7 +1998,8 @@ int few(Ctx& c, const XentP& p, bool grad, void* loss, void* lse, void* dx, void
                 : nb == 2 ? few_t<T, 2>(c, p, f, grad, loss, lse, ws) \
                 : nb == 4 ? few_t<T, 4>(c, p, f, grad, loss, lse, ws) \
                           : few_t<T, 8>(c, p, f, grad, loss, lse, ws))
-    rc = p.dt == F32 ? FEW(float) : FEW(bf16);
+    if (nb == 16) rc = few_t<float, 16>(c, p, f, grad, loss, lse, ws);  // f32 only: is_few
+    else rc = p.dt == F32 ? FEW(float) : FEW(bf16);
 #undef FEW
     if (rc) return rc;
     pdl_record_all(c);

@@ -397,7 +397,7 @@ XENT_SHAPES = [(1, 1, 1), (1, 10, 3), (3, 257, 13), (2, 256, 64), (130, 1000, 64
                # up to 8 rows, with x in shared memory or (the last two) not
                (1, 31, 2048), (8, 1000, 2048), (7, 30000, 1024), (1, 100003, 640), (6, 9999, 41), (4, 5000, 4096), (8, 33, 8),
                (3, 1, 100), (2, 65536, 1000), (8, 700, 2056), (1, 500, 16392),
-               (9, 65536, 64), (17, 30001, 100), (24, 2048, 2048)]
+               (9, 65536, 64), (17, 30001, 100), (24, 2048, 2048), (16, 30000, 100), (12, 10001, 333), (13, 2000, 1000)]
 
 
 def xent_inputs(torch, name, n, v, d, seed=0, scale=2.0):
