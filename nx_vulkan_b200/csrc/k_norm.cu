@@ -20,7 +20,7 @@
 // are on their way to L2.  Pairs of f32 values go through the packed two-f32
 // instructions.
 // Measured: [32768, 4096] bf16 forward 84 us (6.4 TB/s), [16384, 8192] bf16 backward
-// 168 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
+// 166 us (4.9 TB/s; next row in registers 216, rows again from L2 187).
 //
 // Pieces are 16 bytes.  A row that does not start on a 16-byte boundary is worked on in
 // the aligned pieces of its memory: x, dy and what is written lie at the same place of
@@ -572,7 +572,8 @@ __device__ __forceinline__ void group_sum(A (&v)[K], unsigned G, A (*red)[16]) {
 
 // Persistent; a thread holds the same columns of every row that its group takes,
 // so it adds up its columns' dy xh and dy in registers.  R rows at a time (bf16:
-// 2), while the next two rounds' come into L2.  At the end the groups' column
+// 2; 1 and 3: [16384, 8192] 200 and 172 us instead of 165), while the next round's come
+// into L2 (of the next two: 167 us).  At the end the groups' column
 // sums are added, in order, into row blockIdx.x of the partial sums
 // [2][gridDim.x][cols]; or, where the grid is one cluster of up to 8 CTAs (dgamma is
 // given), over the CTAs' shared memory into dgamma and dbeta, which saves the fold's
@@ -631,9 +632,8 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
             }
         }
     };
-    prefetch(1);
     for (unsigned it = 0, turn = 0; (size_t)(id0 >> d.lgp) + (size_t)it * fewest < d.units; it++, turn ^= 1) {
-        prefetch(it + 2);
+        prefetch(it + 1);
         // this group's rows; the last ones may lie past the tensor
         const size_t row0 = first_row(it);
         Piece<T> vx[R][NV], vd[R][NV];
