@@ -856,3 +856,48 @@ def test_refusals_on_device(nxv, torch):
     refused(cg(W(256, 64), y), "shares memory")
     refused(cg(W(256, 64), W(300, 64)), "shares memory")
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 300, 48), (1, 1000, 333), (8, 2000, 77), (12, 30000, 100), (40, 300, 48), (200, 900, 70)],
+                         ids=str)
+def test_every_path_with_a_row_of_nan_int32_labels_and_a_replay(nxv, torch, name, shape):
+    """A workspace of just the stated size, kept to; a row without a target that holds NaN."""
+    from nx_vulkan_b200 import _native
+    n, v, d = shape
+    dl, x, w, labels, lse = xgrad_inputs(torch, name, n, v, d)
+    row = n // 2
+    labels[row] = -1
+    rooms, sized = [], []
+    for grad in (False, True):
+        need = nxv.linear_cross_entropy_workspace(n, v, d, name, grad=grad)
+        rooms.append(torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda"))
+        sized.append((need, wrap(nxv, rooms[-1][:need])))
+    want = [t.clone() for t in xgrad_run(nxv, torch, dl, x, w, labels, lse, name)]
+    loss = xent_run(nxv, torch, x, w, labels, name)[0].clone()
+    x[row], dl[row], lse[row] = float("nan"), float("nan"), float("nan")
+    labels = labels.int()
+    outs = [torch.full_like(loss, 9.0), torch.full_like(loss, 9.0)], [torch.full_like(x, 9.0), torch.full_like(w, 9.0)]
+
+    def both():
+        xent_run(nxv, torch, x, w, labels, name, workspace=sized[0][1], outs=outs[0])
+        xgrad_run(nxv, torch, dl, x, w, labels, lse, name, workspace=sized[1][1], outs=outs[1])
+
+    both()
+    torch.cuda.synchronize()
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        _native.load().nxv_set_stream(s.cuda_stream)
+        both()
+    _native.load().nxv_set_stream(1)
+    for replay in (False, True):
+        if replay:
+            for t in (*outs[0], *outs[1]):
+                t.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+        rest = torch.arange(n, device="cuda") != row
+        assert torch.equal(outs[0][0][rest], loss[rest]) and float(outs[0][0][row]) == 0.0
+        assert all(torch.equal(p, q) for p, q in zip(outs[1], want))
+    for room, (need, _) in zip(rooms, sized):
+        assert bool((room[need:] == 77).all())
