@@ -291,7 +291,7 @@ struct alignas(64) Work {
     Job job[kMaxJobs];
     int jobs;
     uint32_t tiles;
-    int* err;             // wait_flag()
+    int* err;             // wait_flag(c)
 };
 
 // The six partial products of f32, the smallest first.
@@ -1558,7 +1558,7 @@ int launch_work(Ctx& c, const Work& w) {
 }
 
 int run_work(Ctx& c, Work& w, int cg, bool six) {
-    w.err = wait_flag();
+    w.err = wait_flag(c);
     if (cg == 2) return six ? launch_work<2, true>(c, w) : launch_work<2, false>(c, w);
     return six ? launch_work<1, true>(c, w) : launch_work<1, false>(c, w);
 }
@@ -2011,11 +2011,6 @@ int few(Ctx& c, const XentP& p, bool grad, void* loss, void* lse, void* dx, void
 size_t xent_workspace(const XentP& p, bool grad) {
     if (is_few(p, grad)) return std::max(few_plan(p, grad, 1).total, few_plan(p, grad, few_vec(p, true)).total);
     return is_small(p) ? small_plan(p, grad).total : make_plan(p, grad).total;
-}
-
-int xent_error() {
-    int* f = wait_flag();
-    return f ? __atomic_exchange_n(f, 0, __ATOMIC_ACQ_REL) : 0;
 }
 
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws) {

@@ -79,8 +79,6 @@ size_t xent_workspace(const XentP& p, bool grad);
 int launch_xent(Ctx& c, const XentP& p, void* loss, void* lse, void* ws);
 int launch_xent_grad(Ctx& c, const XentP& p, void* dx, void* dw, const void* dloss,
                      const void* lse, void* ws);
-// Reads and clears the flag of its kernels' bounded waits (1 = one ran out).
-int xent_error();
 
 // leapfrog chains (k_leapfrog.cu)
 enum Family : int { FAM_NORMAL = 0, FAM_EXP = 1, FAM_STUDENTT = 2, FAM_CAUCHY = 3,

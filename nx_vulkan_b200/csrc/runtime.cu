@@ -33,6 +33,8 @@ thread_local bool tl_stream_set = false;
 thread_local int tl_cuda_current = -1;
 thread_local char tl_err[512] = {0};
 
+int* g_wait_flag = nullptr;
+
 std::mutex g_scratch_mu;
 // (device, stream, slot) -> (region, bytes)
 std::map<std::tuple<int, cudaStream_t, int>, std::pair<void*, size_t>> g_scratch;
@@ -69,6 +71,10 @@ int init_one(int id) {
     for (int s = 0; s < Device::kSlots; s++) {
         NXV_CK(cudaMallocHost(&d->staging[s], Device::kSlotBytes));
         NXV_CK(cudaEventCreateWithFlags(&d->slot_ev[s], cudaEventDisableTiming));
+    }
+    if (!g_wait_flag) {  // kept to the end of the process: graphs hold its address
+        NXV_CK(cudaHostAlloc(&g_wait_flag, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+        *g_wait_flag = 0;
     }
     g_devices[id] = d;
     tl_cuda_current = id;
@@ -132,8 +138,6 @@ int init_default() {
     return OK;
 }
 
-int* g_wait_flag = nullptr;
-
 int init_devices(const int* ids, int n) {
     if (!ids || n <= 0) return E_NULL;
     std::lock_guard<std::mutex> lk(g_init_mu);
@@ -141,10 +145,6 @@ int init_devices(const int* ids, int n) {
     for (int i = 0; i < n; i++) {
         int rc = init_one(ids[i]);
         if (rc != OK) return rc;
-    }
-    if (!g_wait_flag) {  // kept to the end of the process: graphs hold its address
-        NXV_CK(cudaHostAlloc(&g_wait_flag, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
-        *g_wait_flag = 0;
     }
     g_default_device = ids[0];
     tl_device = ids[0];
@@ -259,7 +259,9 @@ int sync(Ctx& c) {
     return OK;
 }
 
-int* wait_flag() { return g_wait_flag; }
+int* wait_flag(Ctx&) { return g_wait_flag; }
+
+bool wait_ran_out(Ctx&) { return __atomic_exchange_n(g_wait_flag, 0, __ATOMIC_ACQ_REL) != 0; }
 
 bool capturing(Ctx& c) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;

@@ -105,9 +105,11 @@ struct ScratchGuard {
 // True while c.stream is being captured into a CUDA graph.
 bool capturing(Ctx& c);
 
-// Set (from the device too) when a bounded wait of a kernel ran out: host memory of
-// the process, read without a CUDA call.  Null before init.
-int* wait_flag();
+// Where a kernel on c's device says (1) that a bounded wait of it ran out: host memory,
+// read without a CUDA call, there from the device's initialisation on.
+int* wait_flag(Ctx& c);
+// Reads and clears it.
+bool wait_ran_out(Ctx& c);
 
 // Error reporting.
 void set_error(const char* fmt, ...);

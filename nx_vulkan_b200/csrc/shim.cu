@@ -980,7 +980,7 @@ int nxv_synchronize(void) {
         set_error("tensor-core GEMM: a bounded pipeline wait ran out; results are invalid");
         return E_CUDA;
     }
-    if (rc == OK && xent_error()) {
+    if (rc == OK && wait_ran_out(c)) {
         set_error("linear cross entropy: a bounded pipeline wait ran out; results are invalid");
         return E_CUDA;
     }

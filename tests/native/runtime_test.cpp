@@ -1,0 +1,46 @@
+// Checks of runtime.cu's host logic over fake_cudart.cpp; the argument names one.
+// Exit status: 0 it holds, 1 it does not.
+#include <stdio.h>
+#include <string.h>
+
+#include "runtime.h"
+
+using namespace nxv;
+
+#define CHECK(x)                                       \
+    do {                                               \
+        if (!(x)) return printf("not so: %s\n", #x), 1; \
+    } while (0)
+
+// Either way of initialising gives the kernels a place for their report.
+static int init_default_has_wait_flag() {
+    Ctx c;
+    CHECK(init_default() == OK && begin(c, {}) == OK);
+    CHECK(wait_flag(c) != nullptr && *wait_flag(c) == 0);
+    CHECK(!wait_ran_out(c));
+    return 0;
+}
+static int init_devices_has_wait_flag() {
+    Ctx c;
+    const int ids[] = {1, 0};
+    CHECK(init_devices(ids, 2) == OK && begin(c, {}) == OK && c.dev->id == 1);
+    CHECK(wait_flag(c) != nullptr && *wait_flag(c) == 0);
+    *wait_flag(c) = 1;
+    CHECK(wait_ran_out(c));
+    CHECK(!wait_ran_out(c));
+    return 0;
+}
+
+int main(int argc, char** argv) {
+    const struct {
+        const char* name;
+        int (*run)();
+    } all[] = {
+        {"init_default_has_wait_flag", init_default_has_wait_flag},
+        {"init_devices_has_wait_flag", init_devices_has_wait_flag},
+    };
+    for (auto& t : all)
+        if (argc == 2 && !strcmp(argv[1], t.name)) return t.run();
+    for (auto& t : all) puts(t.name);
+    return argc == 1 ? 0 : 2;
+}
