@@ -898,12 +898,16 @@ unsigned row_classes(unsigned cols) {
     return lgp;
 }
 
+// Pieces of gamma and of beta that k_norm_fwd has room for in shared memory.
+constexpr size_t kWeightPieces = 7168;
+constexpr int kWeightBytes = 2 * kWeightPieces * 16;
+
 template <typename T, bool AL>
 int fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, const T* b,
          unsigned rows, unsigned cols, acc_t<T> eps) {
     // a row that starts inside a piece may take one more
     const size_t nv = ((size_t)cols + (AL ? 1 : 2) * (kV<T> - 1)) / kV<T>;
-    if (nv > (AL ? 16 * 512 : 7168)) {  // 7168: gamma and beta in shared memory
+    if (nv > (AL ? 16 * 512 : kWeightPieces)) {
         k_norm_fwd_long<T><<<std::min(rows, (unsigned)c.dev->sm_count * 2), 1024, 0, c.stream>>>(
             y, mean, rstd, x, g, b, rows, cols, eps);
         return OK;
@@ -930,7 +934,9 @@ int fwd(Ctx& c, T* y, acc_t<T>* mean, acc_t<T>* rstd, const T* x, const T* g, co
         // CTAs an SM remain ([16384, 1001] f32 with 32, 128, 256, 512 threads 64, 29, 28, 29 us).
         const unsigned most = tx == 32 ? 256 : 512;
         for (ty = 1; 2 * ty * tx <= most && rows >= (size_t)c.dev->sm_count * 4 * ty; ty *= 2) {}
-        NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        // the same for all widths: the attribute is the kernel's, not the call's, and another
+        // thread may set it between here and the launch
+        NXV_CK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kWeightBytes));
     }
     const unsigned part = AL ? 1u << 30 : 1u << 27;  // rows of a launch, within the grid's limit
     for (size_t r0 = 0; r0 < rows; r0 += part) {
