@@ -594,7 +594,9 @@ int nxv_set_stream(void* cuda_stream);
 int nxv_stream_capturing(void);
 
 /* Wait for all work queued on the current device.  0, or -4 with the CUDA
- * error that a kernel raised. */
+ * error that a kernel raised.  A pipeline wait of the linear cross entropy that
+ * ran out on the device (results are invalid) is told once to every thread
+ * that synchronizes the device: its next call returns -4. */
 int nxv_synchronize(void);
 
 /* Non-owning handle over existing device memory of n_bytes (e.g. a tensor

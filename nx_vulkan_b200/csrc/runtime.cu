@@ -33,7 +33,11 @@ thread_local bool tl_stream_set = false;
 thread_local int tl_cuda_current = -1;
 thread_local char tl_err[512] = {0};
 
-int* g_wait_flag = nullptr;
+int* g_wait_flags[kMaxDevices] = {};
+// How often a device's flag has been found set, and how often this thread has said so.
+std::mutex g_wait_mu;
+unsigned g_waits_out[kMaxDevices] = {};
+thread_local unsigned tl_waits_told[kMaxDevices] = {};
 
 std::mutex g_scratch_mu;
 // (device, stream, slot) -> (region, bytes)
@@ -72,9 +76,9 @@ int init_one(int id) {
         NXV_CK(cudaMallocHost(&d->staging[s], Device::kSlotBytes));
         NXV_CK(cudaEventCreateWithFlags(&d->slot_ev[s], cudaEventDisableTiming));
     }
-    if (!g_wait_flag) {  // kept to the end of the process: graphs hold its address
-        NXV_CK(cudaHostAlloc(&g_wait_flag, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
-        *g_wait_flag = 0;
+    if (!g_wait_flags[id]) {  // kept to the end of the process: graphs hold its address
+        NXV_CK(cudaHostAlloc(&g_wait_flags[id], sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+        *g_wait_flags[id] = 0;
     }
     g_devices[id] = d;
     tl_cuda_current = id;
@@ -259,9 +263,16 @@ int sync(Ctx& c) {
     return OK;
 }
 
-int* wait_flag(Ctx&) { return g_wait_flag; }
+int* wait_flag(Ctx& c) { return g_wait_flags[c.dev->id]; }
 
-bool wait_ran_out(Ctx&) { return __atomic_exchange_n(g_wait_flag, 0, __ATOMIC_ACQ_REL) != 0; }
+bool wait_ran_out(Ctx& c) {
+    const int id = c.dev->id;
+    std::lock_guard<std::mutex> lk(g_wait_mu);
+    if (__atomic_exchange_n(g_wait_flags[id], 0, __ATOMIC_ACQ_REL)) g_waits_out[id]++;
+    const bool news = g_waits_out[id] != tl_waits_told[id];
+    tl_waits_told[id] = g_waits_out[id];
+    return news;
+}
 
 bool capturing(Ctx& c) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;

@@ -108,7 +108,9 @@ bool capturing(Ctx& c);
 // Where a kernel on c's device says (1) that a bounded wait of it ran out: host memory,
 // read without a CUDA call, there from the device's initialisation on.
 int* wait_flag(Ctx& c);
-// Reads and clears it.
+// True when a wait ran out on c's device since this thread last asked (the first time: since
+// the start).  Every thread is told, whichever asks first: the results that are invalid may be
+// any thread's.
 bool wait_ran_out(Ctx& c);
 
 // Error reporting.

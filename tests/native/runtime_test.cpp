@@ -3,6 +3,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <thread>
+
 #include "runtime.h"
 
 using namespace nxv;
@@ -31,6 +33,36 @@ static int init_devices_has_wait_flag() {
     return 0;
 }
 
+// A wait that ran out on one device is no other device's report, nor taken by it.
+static int wait_report_is_its_devices() {
+    Ctx a, b;
+    const int ids[] = {0, 1};
+    CHECK(init_devices(ids, 2) == OK && begin(a, {}) == OK);
+    CHECK(set_current(1) == OK && begin(b, {}) == OK);
+    *wait_flag(a) = 1;
+    CHECK(!wait_ran_out(b));
+    CHECK(wait_ran_out(a));
+    CHECK(!wait_ran_out(a) && !wait_ran_out(b));
+    return 0;
+}
+// A thread that asks does not take the report from the other threads of the device; each is
+// told once.
+static int wait_report_reaches_every_thread() {
+    Ctx c;
+    CHECK(init_default() == OK && begin(c, {}) == OK);
+    CHECK(!wait_ran_out(c));
+    *wait_flag(c) = 1;
+    bool first = false, second = true;
+    std::thread([&] { first = wait_ran_out(c), second = wait_ran_out(c); }).join();
+    CHECK(first && !second);
+    CHECK(wait_ran_out(c));
+    CHECK(!wait_ran_out(c));
+    *wait_flag(c) = 1;
+    CHECK(wait_ran_out(c));
+    CHECK(!wait_ran_out(c));
+    return 0;
+}
+
 int main(int argc, char** argv) {
     const struct {
         const char* name;
@@ -38,6 +70,8 @@ int main(int argc, char** argv) {
     } all[] = {
         {"init_default_has_wait_flag", init_default_has_wait_flag},
         {"init_devices_has_wait_flag", init_devices_has_wait_flag},
+        {"wait_report_is_its_devices", wait_report_is_its_devices},
+        {"wait_report_reaches_every_thread", wait_report_reaches_every_thread},
     };
     for (auto& t : all)
         if (argc == 2 && !strcmp(argv[1], t.name)) return t.run();

@@ -33,3 +33,9 @@ def holds(exe, name):
 def test_every_way_to_initialise_has_a_wait_flag(exe, name):
     """The tensor-core cross entropy reports a wait that ran out there: without it, it would write to address 0."""
     holds(exe, name)
+
+
+@pytest.mark.parametrize("name", ["wait_report_is_its_devices", "wait_report_reaches_every_thread"])
+def test_a_wait_that_ran_out_is_told_to_whom_it_concerns(exe, name):
+    """The word that the kernel writes is written here by the test: no wait runs out."""
+    holds(exe, name)
