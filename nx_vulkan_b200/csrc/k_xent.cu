@@ -378,11 +378,13 @@ struct Row {
             s *= ex2((m - cm) * kLog2e);  // m = -inf: s is 0
             m = cm;
         }
-        // while every logit is -inf (or NaN), terms are taken against 0
-        const float ref = m == -INFINITY ? 0.0f : m * kLog2e;
+        // While every logit is -inf (or NaN), terms are taken against 0.  The difference first:
+        // the largest term is 1 then and the sum not below it, so no loss is negative (one
+        // fma with m log2e, rounded, puts all terms off by half a step of that product).
+        const float ref = m == -INFINITY ? 0.0f : m;
         float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < 32; e++) t[e & 3] += ex2(fmaf(v[e], kLog2e, -ref));
+        for (int e = 0; e < 32; e++) t[e & 3] += ex2((v[e] - ref) * kLog2e);
         s += (t[0] + t[1]) + (t[2] + t[3]);
     }
 

@@ -83,6 +83,28 @@ def test_large_logits(nxv, torch, shape, name):
 
 
 @pytest.mark.parametrize("name", TYPES)
+def test_loss_of_a_label_that_wins(nxv, torch, shape, name):
+    """The label's logit is L, all others are 0: the loss, log(1 + (v - 1) e^-L), is not below 0 and off by what the
+    terms and the logarithm are off, whatever L's size.  The largest term is exactly 1; the others are 2^-22 of
+    themselves off and 2^-24 of their exponent's size, twice; sums round by 2^-24 for each of a thread's 32 columns and
+    12 levels, but never below 1; logf is off by an ulp."""
+    n, v, d = shape
+    for L in (9.3125, 30.75, 50.125, 77.0, 101.25, 1003.0):
+        L = float(torch.tensor(L, dtype=dt(torch, name)))  # what x holds
+        x = torch.zeros(n, d, device="cuda", dtype=dt(torch, name))
+        w = torch.zeros(v, d, device="cuda", dtype=dt(torch, name))
+        labels = torch.arange(n, device="cuda") % min(v, d)
+        x[torch.arange(n), labels] = L
+        w[torch.arange(min(v, d)), torch.arange(min(v, d))] = 1.0
+        loss, lse = xent_run(nxv, torch, x, w, labels, name)
+        rest = (v - 1) * torch.exp(torch.tensor(-L, dtype=torch.float64))
+        assert float(loss.min()) >= 0.0, (L, float(loss.min()))
+        tol = float(rest) * (2.0 ** -22 + 2 * L * 2.0 ** -24) + 44 * 2.0 ** -24 * (1.0 if float(rest) > 2.0 ** -24 else 0.0)
+        within(torch, loss, torch.log1p(rest).cuda().expand(n), tol + 2.0 ** -23)
+        within(torch, lse, (L + torch.log1p(rest)).cuda().expand(n), tol + 2.0 ** -23 + L * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("name", TYPES)
 def test_bad_rows_stay_their_own(nxv, torch, shape, name):
     x, w, labels = xent_inputs(torch, name, *shape)
     bad = [3, 17, 140]
