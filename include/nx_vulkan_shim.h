@@ -254,8 +254,8 @@ int nxv_random_f64(void* out, unsigned long n, unsigned int seed, unsigned int d
  * (var = mean of (x - mean)^2), y = (x - mean) rstd gamma + beta.  gamma, beta
  * [cols] and y have x's type; mean and rstd [rows] are f32 (f64 for f64) and
  * all arithmetic is in their type (rows whose squared deviations' sum overflows
- * it have rstd 0).  y may be x.  1 <= cols <= 2^28, eps >= 0.
- * spv: layer_norm.spv. */
+ * it have rstd 0; the sums along very long rows are f64).  y may be x.
+ * 1 <= cols <= 2^28, eps >= 0.  spv: layer_norm.spv. */
 int nxv_layer_norm(void* y, void* mean, void* rstd,
                    void* x, void* gamma, void* beta,
                    unsigned int rows, unsigned int cols, double eps,

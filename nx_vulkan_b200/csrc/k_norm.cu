@@ -9,9 +9,10 @@
 //           dgamma_j = sum_rows dy_j xh_j,  dbeta_j = sum_rows dy_j
 //
 // Statistics, sums and the arithmetic are f32 for f32 and bf16 and f64 for
-// f64; a bf16 result is rounded once, at its store.  The variance is taken
-// from the centred values (two passes over registers, not E[x^2] - mean^2,
-// which cancels for rows with a large mean).
+// f64 (the sums along rows longer than a CTA's registers f64 for all); a bf16
+// result is rounded once, at its store.  The variance is taken from the centred
+// values (two passes over registers, not E[x^2] - mean^2, which cancels for rows
+// with a large mean).
 //
 // Both directions are bound by memory: a row is read once, stays in registers
 // and is written once.  What counts is how many bytes are in flight: forward the
@@ -452,16 +453,18 @@ k_norm_fwd(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const
 }
 
 // Rows that 512 threads, or gamma and beta that the shared memory, cannot hold: three
-// passes over the row.
+// passes over the row.  A thread adds up to 2^18 values one after the other, so the sums are
+// f64 (in f32 the mean of 2^28 values of N(1003, 1) is 2 off, of 2^26 0.16).  Two CTAs an
+// SM: 32 registers ([500, 65536] f32 99 us; 58 registers and one CTA 145).
 template <typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(1024, 2)
 k_norm_fwd_long(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, const T* x,
                 const T* __restrict__ gamma, const T* __restrict__ beta, unsigned rows,
                 unsigned cols, acc_t<T> eps) {
     using A = acc_t<T>;
-    __shared__ A red[2][32];
+    __shared__ double red[2][32];
     const unsigned lane = threadIdx.x & 31;
-    auto total = [&](A v, int which) {
+    auto total = [&](double v, int which) {
         v = warp_sum(v);
         if (lane == 0) red[which][threadIdx.x >> 5] = v;
         __syncthreads();
@@ -470,15 +473,15 @@ k_norm_fwd_long(T* y, acc_t<T>* __restrict__ mean, acc_t<T>* __restrict__ rstd, 
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * cols;
         T* yr = y + row * cols;
-        A s = A(0);
-        for (unsigned i = threadIdx.x; i < cols; i += 1024) s += to_acc(xr[i]);
-        const A m = div_(total(s, 0), A(cols));
-        s = A(0);
+        double s = 0.0;
+        for (unsigned i = threadIdx.x; i < cols; i += 1024) s += (double)to_acc(xr[i]);
+        const A m = (A)div_(total(s, 0), (double)cols);
+        s = 0.0;
         for (unsigned i = threadIdx.x; i < cols; i += 1024) {
-            const A d = to_acc(xr[i]) - m;
-            s += d * d;
+            const double d = (double)(to_acc(xr[i]) - m);
+            s = __fma_rn(d, d, s);
         }
-        const A rs = rsqrt_exact(div_(total(s, 1), A(cols)) + eps);
+        const A rs = rsqrt_exact((A)div_(total(s, 1), (double)cols) + eps);
         if (threadIdx.x == 0) {
             mean[row] = m;
             rstd[row] = rs;
@@ -738,17 +741,19 @@ k_norm_bwd(T* dx, acc_t<T>* __restrict__ part, const T* dy, const T* x,
     }
 }
 
-// A row's two sums over the 512 threads of a CTA: this thread's shares.
+// A row's two sums over the 512 threads of a CTA: this warp's shares.  In f64 from turn to
+// turn, as many as 2^15 for the longest rows.
 template <typename T, bool AL>
-__device__ __forceinline__ void row_sums(acc_t<T> (&sum)[2], const T* px, const T* pd, const T* gamma,
+__device__ __forceinline__ void row_sums(double (&sum)[2], const T* px, const T* pd, const T* gamma,
                                          acc_t<T> m, acc_t<T> rs, unsigned cols, bool edge) {
     using A = acc_t<T>;
     using W = vec_t<T>;
     constexpr int V = kV<T>, NP = kP<T>, B = 4;
     const unsigned nv = (cols + V - 1) / V;
     const W mm = vset(-m, (W*)0), rr = vset(rs, (W*)0);
-    W a0 = vset(A(0), (W*)0), a1 = a0;
+    sum[0] = sum[1] = 0.0;
     for (unsigned i0 = threadIdx.x; i0 < nv; i0 += B * 512) {
+        W a0 = vset(A(0), (W*)0), a1 = a0;
         Piece<T> x[B], dy[B];
 #pragma unroll
         for (int k = 0; k < B; k++) {
@@ -770,33 +775,34 @@ __device__ __forceinline__ void row_sums(acc_t<T> (&sum)[2], const T* px, const 
                 a1 = vfma(w, vmul(vadd(xv[e], mm), rr), a1);
             }
         }
+        sum[0] += (double)vsum(a0), sum[1] += (double)vsum(a1);
     }
-    sum[0] = warp_sum(vsum(a0)), sum[1] = warp_sum(vsum(a1));
+    sum[0] = warp_sum(sum[0]), sum[1] = warp_sum(sum[1]);
 }
 
 // Rows that the threads of a CTA cannot hold the column sums of (x and dy are read
 // twice; blocks of rows that stay in L2 in between measured slower, the launches
 // too small: [4096, 12000] f32 221 us instead of 178): the two sums of
 // every row first, then a pass in which a CTA takes a strip of 256 pieces of
-// columns of the rows 4 blockIdx.y .., + 4 gridDim.y, ...
+// columns of the rows 4 blockIdx.y .., + 4 gridDim.y, ...  The f32 sums with 32 registers
+// (40: 196 us).
 template <typename T, bool AL>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, AL && sizeof(T) == 4 ? 4 : 1)
 k_norm_bwd_sums(acc_t<T>* __restrict__ sums, const T* dy, const T* x, const T* __restrict__ gamma,
                 const acc_t<T>* __restrict__ mean, const acc_t<T>* __restrict__ rstd, unsigned rows,
                 unsigned cols) {
-    using A = acc_t<T>;
-    __shared__ A p[2][16];
+    __shared__ double p[2][16];
     for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        A s[2];
+        double s[2];
         row_sums<T, AL>(s, x + row * cols, dy + row * cols, gamma, mean[row], rstd[row], cols,
                         edge_row<T>(row, rows, cols));
         __syncthreads();
         if ((threadIdx.x & 31) == 0) p[0][threadIdx.x >> 5] = s[0], p[1][threadIdx.x >> 5] = s[1];
         __syncthreads();
         if (threadIdx.x < 2) {
-            A v = A(0);
+            double v = 0.0;
             for (int k = 0; k < 16; k++) v += p[threadIdx.x][k];
-            sums[2 * row + threadIdx.x] = v;
+            sums[2 * row + threadIdx.x] = (acc_t<T>)v;
         }
     }
 }
