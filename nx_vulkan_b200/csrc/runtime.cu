@@ -109,6 +109,7 @@ void set_error(const char* fmt, ...) {
 
 int cuda_fail(cudaError_t e, const char* what) {
     set_error("%s: %s", what, cudaGetErrorString(e));
+    cudaGetLastError();  // told; the next call's finish() must not find it
     return E_CUDA;
 }
 
@@ -298,6 +299,7 @@ void* scratch(Ctx& c, size_t bytes, int slot) {
     void* p = nullptr;
     if (cudaMallocAsync(&p, sz, c.stream) != cudaSuccess) {
         set_error("scratch allocation of %zu bytes failed", sz);
+        cudaGetLastError();
         return nullptr;
     }
     g_scratch[key] = std::make_pair(p, sz);

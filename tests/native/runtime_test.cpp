@@ -63,6 +63,27 @@ static int wait_report_reaches_every_thread() {
     return 0;
 }
 
+// A call that fails is told so itself; the next one on the thread is not.
+static int failed_scratch_is_its_call_s() {
+    Ctx c;
+    CHECK(init_default() == OK && begin(c, {}) == OK);
+    CHECK(scratch(c, (size_t)1 << 38) == nullptr);
+    CHECK(finish(c) == OK);
+    CHECK(scratch(c, 1000) != nullptr && finish(c) == OK);
+    return 0;
+}
+static int failed_call_is_its_call_s() {
+    Ctx c;
+    CHECK(init_default() == OK && begin(c, {}) == OK);
+    auto call = [] {
+        NXV_CK(cudaSetDevice(7));
+        return (int)OK;
+    };
+    CHECK(call() == E_CUDA);
+    CHECK(finish(c) == OK);
+    return 0;
+}
+
 int main(int argc, char** argv) {
     const struct {
         const char* name;
@@ -72,6 +93,8 @@ int main(int argc, char** argv) {
         {"init_devices_has_wait_flag", init_devices_has_wait_flag},
         {"wait_report_is_its_devices", wait_report_is_its_devices},
         {"wait_report_reaches_every_thread", wait_report_reaches_every_thread},
+        {"failed_scratch_is_its_call_s", failed_scratch_is_its_call_s},
+        {"failed_call_is_its_call_s", failed_call_is_its_call_s},
     };
     for (auto& t : all)
         if (argc == 2 && !strcmp(argv[1], t.name)) return t.run();

@@ -39,3 +39,9 @@ def test_every_way_to_initialise_has_a_wait_flag(exe, name):
 def test_a_wait_that_ran_out_is_told_to_whom_it_concerns(exe, name):
     """The word that the kernel writes is written here by the test: no wait runs out."""
     holds(exe, name)
+
+
+@pytest.mark.parametrize("name", ["failed_scratch_is_its_call_s", "failed_call_is_its_call_s"])
+def test_an_error_is_not_the_next_call_s(exe, name):
+    """A workspace that does not fit, a CUDA call that fails: the valid call after it is not refused for it."""
+    holds(exe, name)
