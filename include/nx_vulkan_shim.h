@@ -308,8 +308,12 @@ int nxv_linear_cross_entropy(void* loss, void* lse, void* workspace,
  * and the forward call's lse: G = (exp(z - lse) - [v = label]) dloss (0 for a
  * row without a target, whatever its x holds), dx = G w [n, dim], dw = G^T x
  * [vocab, dim] in x's type.  The vocabulary is processed in pieces; z is
- * computed again, and G of one piece is held in the workspace (bf16 G for
- * bf16).  Bit-reproducible.  spv: linear_cross_entropy_grad.spv. */
+ * computed again, and G of one piece is held in the workspace.  Bit-reproducible.
+ * bf16 on the tensor cores (more than a few rows, n vocab dim above 2^23;
+ * is_few and is_small in k_xent.cu): softmax - one-hot is rounded to bf16 before
+ * both products, dloss x (in units of the largest dloss: exact for a mean)
+ * before dw's, and the f32 sums may lose 2^-23 of themselves per 16 products;
+ * smaller calls keep all that in f32.  spv: linear_cross_entropy_grad.spv. */
 int nxv_linear_cross_entropy_grad(void* dx, void* dw, void* workspace,
                                   void* dloss, void* x, void* w, void* labels, void* lse,
                                   unsigned int n, unsigned int vocab, unsigned int dim,

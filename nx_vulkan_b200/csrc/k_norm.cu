@@ -20,8 +20,8 @@
 // column sums take the registers, one CTA an SM holds some rows while the next ones
 // are on their way to L2.  Pairs of f32 values go through the packed two-f32
 // instructions.
-// Measured: [32768, 4096] bf16 forward 84 us (6.4 TB/s), [16384, 8192] bf16 backward
-// 166 us (4.9 TB/s; next row in registers 216, rows again from L2 187).
+// Measured: [32768, 4096] bf16 forward 84 us over the same tensors (6.4 TB/s), 90 to 92
+// over changing ones (5.9), [16384, 8192] bf16 backward 165 to 169 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
 //
 // Pieces are 16 bytes.  A row that does not start on a 16-byte boundary is worked on in
 // the aligned pieces of its memory: x, dy and what is written lie at the same place of

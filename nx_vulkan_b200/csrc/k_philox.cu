@@ -270,10 +270,12 @@ __global__ void k_random_f64(double* __restrict__ out, size_t n, uint32_t seed, 
 // and infinities included).  thresh = ceil(p 2^24): the comparison of the
 // uniform (word >> 8) 2^-24 with p, in whole numbers.  f32 arithmetic for f32
 // and bf16 (bf16 rounded once at the store), f64 for f64.
-// f32 and f64 are bound by memory (2^26 f32 90 us, 6.0 TB/s), bf16 by the mask: two
-// elements take ten wide multiplies, which are issued at a fraction of the other
-// instructions' rate (2^27 bf16 128 us, 4.2 TB/s; a multiply less per counter, by
-// adding the multiplier to the neighbour's first product, changed nothing).
+// f32 and f64 are bound by memory (2^26 f32 90 us, 6.0 TB/s).  2^27 bf16 takes 130 us
+// (4.1 TB/s), with neither memory nor a pipe full: the wide multiplies, ten for two
+// elements, keep their pipe 69 % busy and warps wait for it (3.1 per issue) and more for
+// their loads (4.1), one of which a thread has in flight; a multiply less per counter
+// changed nothing.  Unaligned tensors go element by element, a whole counter each: 2^27
+// bf16 423 us, 2^26 f32 219.
 __device__ __forceinline__ float drop_scaled(float x, double, float s) { return __fmul_rn(x, s); }
 __device__ __forceinline__ double drop_scaled(double x, double s, float) { return __dmul_rn(x, s); }
 __device__ __forceinline__ __nv_bfloat16 drop_scaled(__nv_bfloat16 x, double, float s) {

@@ -19,12 +19,17 @@
 //   OUT   dx = dloss (sum over pieces of P w), the sum in f32, and
 //         dw_piece = P^T (dloss x).
 //
-// Types.  bf16: the operands go to the tensor core as they are; sums are f32.
+// Types.  bf16: the operands go to the tensor core as they are; sums are f32, all of K
+// in the tensor core's accumulator, which may lose up to 2^-23 of the running sum per 16
+// products, towards zero (8192 x 65536 x 2048: the loss is 6.7e-7 from its formula in 64
+// bits, in f32 sums that round to nearest 7e-8).
 // Two roundings to bf16 stand between the inputs and the sums of the gradient
 // (2^-8 relative to each term at most, like the rounding of the inputs): P
 // without the factor dloss, so that the label's entry, near -1, is nearly exact
 // (with it, all rows of a mean loss would round the same value, by up to 2^-8),
 // and dloss x, in units of the largest dloss, which leaves x as it is for a mean.
+// Against 64 bits, P's rounding adds 2.7e-4 to dx and dw (2-norms), beside the 1.65e-3
+// of their own rounding to bf16.  Few rows and small problems keep both in f32.
 // f32: every f32 value is the sum of three bf16 values, b0 = bf16(v),
 // b1 = bf16(v - b0), b2 = bf16(v - b0 - b1) (exact but for values below 2^-110),
 // and a product is the six partial products b_i b_j with i + j <= 2; the three
@@ -552,9 +557,9 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t round, uint32_t first, uint
 // tiles (a stage's 32 KB for 512 cycles of products), and issue loops without
 // divisions, one warp per operand and uniform (a stage took its one thread
 // ~1000 cycles to load before, whatever its size or the ring's depth, and ~500 to
-// multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms, 1.69 PFLOP/s (the
-// library's bare product of these sizes 1.47 ms in the same session); gradient 5.1
-// to 5.5 ms, 1.6 to 1.7 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
+// multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms in short runs (1.69
+// PFLOP/s), 1.44 to 1.51 in a loop (1.5; the library's bare product of these sizes 1.47);
+// gradient 4.8 ms at first, 5.5 to 5.6 in a loop, 1.6 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
 // 2.1 and 8.3 ms, 1.6 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
 // flight are waited for (bounded), tensor memory is freed and the host's flag set.
@@ -1008,7 +1013,10 @@ k_xent_join_row(float* __restrict__ loss, float* __restrict__ lse, const float* 
 // 37 / 66, 100 x 100 x 1000 19 / 28 and 36 / 45, 256 x 512 x 512 21 / 53 and 25 / 41,
 // 512 x 512 x 256 21 / 56 and 19 / 37; bf16 200 x 200 x 100 10 / 19 and 14 / 25 (not
 // 16-byte rows), 64 x 300 x 400 12 / 19 and 12 / 23, 128 x 512 x 128 10 / 21 and 10 / 19,
-// 64 x 1001 x 1000 21 / 60 and 14 / 29.
+// 64 x 1001 x 1000 21 / 60 and 14 / 29.  Above the f32 limit, 64 x 2000 x 1000 29 / 103
+// and 37 / 70, 128 x 1001 x 1000 29 / 84 and 39 / 70, 64 x 4000 x 1000 51 / 187 and 41 /
+// 85: the forward call alone would gain up to 2^27, one limit serves both.  Above the bf16
+// limit, 64 x 1001 x 250 13 / 26 and 15 / 27, 128 x 512 x 256 12 / 27 and 13 / 19.
 constexpr unsigned long long kSmallF32 = 1ull << 26, kSmallBf16 = 1ull << 23;  // f32 of more than 128 rows: half
 constexpr int KSTEP = 128;  // slices of K are multiples of this, and of a tile's chunk KC
 

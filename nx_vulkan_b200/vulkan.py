@@ -776,7 +776,9 @@ def linear_cross_entropy_grad(dloss, x, w, labels, lse, n, vocab, dim, dtype="f3
                               out=None, workspace=None):
     """Gradients of linear_cross_entropy from dloss (f32 [n], the gradient of
     every row's loss: 1 / n for their mean) and the forward call's lse: dx [n,
-    dim] and dw [vocab, dim] in x's type."""
+    dim] and dw [vocab, dim] in x's type.  Large bf16 calls round softmax -
+    one-hot and dloss x to bf16 before the products (the tensor cores' operands);
+    few rows and small problems keep them in f32."""
     err = _xent_check(x, w, labels, n, vocab, dim, dtype, index_bytes)
     if err:
         return err
