@@ -21,7 +21,8 @@
 // are on their way to L2.  Pairs of f32 values go through the packed two-f32
 // instructions.
 // Measured: [32768, 4096] bf16 forward 84 us over the same tensors (6.4 TB/s), 90 to 92
-// over changing ones (5.9), [16384, 8192] bf16 backward 165 to 169 us (4.8 TB/s; next row in registers 216, rows again from L2 187).
+// over changing ones (5.9), [16384, 8192] bf16 backward 165 to 169 us (4.8 TB/s; next
+// row in registers 216, rows again from L2 187).
 //
 // Pieces are 16 bytes.  A row that does not start on a 16-byte boundary is worked on in
 // the aligned pieces of its memory: x, dy and what is written lie at the same place of
@@ -785,7 +786,7 @@ __device__ __forceinline__ void row_sums(double (&sum)[2], const T* px, const T*
 // too small: [4096, 12000] f32 221 us instead of 178): the two sums of
 // every row first, then a pass in which a CTA takes a strip of 256 pieces of
 // columns of the rows 4 blockIdx.y .., + 4 gridDim.y, ...  The f32 sums with 32 registers
-// (40: 196 us).
+// ([4096, 12000] with both kernels 180 us; with 40 registers 196).
 template <typename T, bool AL>
 __global__ void __launch_bounds__(512, AL && sizeof(T) == 4 ? 4 : 1)
 k_norm_bwd_sums(acc_t<T>* __restrict__ sums, const T* dy, const T* x, const T* __restrict__ gamma,

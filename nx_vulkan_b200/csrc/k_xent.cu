@@ -559,8 +559,8 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t round, uint32_t first, uint
 // ~1000 cycles to load before, whatever its size or the ring's depth, and ~500 to
 // multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms in short runs (1.69
 // PFLOP/s), 1.44 to 1.51 in a loop (1.5; the library's bare product of these sizes 1.47);
-// gradient 4.8 ms at first, 5.5 to 5.6 in a loop, 1.6 PFLOP/s over its four products; 8192 x 32768 x 1024 f32
-// 2.1 and 8.3 ms, 1.6 PFLOP/s over the six partial products.
+// gradient 4.8 ms at first, 5.5 to 5.6 in a loop, 1.6 PFLOP/s over its four products;
+// 8192 x 32768 x 1024 f32 2.1 and 8.3 ms, 1.6 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
 // flight are waited for (bounded), tensor memory is freed and the host's flag set.
 template <int CG, bool SIX>
