@@ -560,7 +560,7 @@ __device__ __forceinline__ uint32_t tile_of(uint32_t round, uint32_t first, uint
 // multiply).  Measured, 8192 x 65536 x 2048 bf16: loss 1.30 ms in short runs (1.69
 // PFLOP/s), 1.44 to 1.51 in a loop (1.5; the library's bare product of these sizes 1.47);
 // gradient 4.8 ms at first, 5.5 to 5.6 in a loop, 1.6 PFLOP/s over its four products;
-// 8192 x 32768 x 1024 f32 2.1 and 8.3 ms, 1.6 PFLOP/s over the six partial products.
+// 8192 x 32768 x 1024 f32 2.2 and 8.1 ms (2.35 and 8.2 in a loop), 1.6 PFLOP/s over the six partial products.
 // Every wait is bounded; on a timeout each role stops, loads and products in
 // flight are waited for (bounded), tensor memory is freed and the host's flag set.
 template <int CG, bool SIX>
@@ -1268,7 +1268,7 @@ k_sum(const __grid_constant__ SumWork w) {
 // k_few_out: a thread holds (of up to 16 rows) some columns of x and of dx's sums in registers and goes
 // down a slab of classes: dx += P w, dw = P^T (dloss x), w read and dw written once.
 // All in f32, rounded once at the end.
-// Measured, 1 x 65536 x 2048: f32 86 us forward (w alone 82 at the measured copy rate),
+// Measured, 1 x 65536 x 2048: f32 86 us forward (88 to 94 in a loop; w alone 82 at the measured copy rate),
 // 272 us the gradient (w twice and dw 246); bf16 50 and 147 us (41 and 123).
 
 constexpr unsigned kFewRows = 8, kFewC = 4;
